@@ -1,0 +1,332 @@
+// Writing the 4-bit key/value cache and reading it back (the format: fp4_unit.cuh).
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "fp4_unit.cuh"
+
+namespace {
+
+using namespace mrun;
+using bf16 = __nv_bfloat16;
+
+// ------------------------------------------------------------------------------------------
+// Per head of every token: q = rotate(rmsnorm(q) * w_q) in bfloat16, in place or into rows of its own; k the
+// same and v as it is into the unit that the token's slot names.  The arithmetic of q is that of
+// qk_norm_rope_cache.
+//
+// A key is quantised from its unrounded value, and which side of a border between two codes a value
+// falls on decides a whole step of the code.  So that the codes are those of the formula and do not depend on
+// the order of a sum, a key's norm and rotation are computed in 64 bits (B200 has 64 such lanes a
+// multiprocessor beside 128 of 32 bits; a key is an eighth to a third of a row).  A value is a bfloat16 and its quotient by a
+// scale of 4 bits is told from every border (at most 3 bits) in 32 bits.
+// ------------------------------------------------------------------------------------------
+constexpr int HEADS_PER_GROUP = 4;      // heads of a token that a group of lanes takes, one after the other
+
+// The byte of the scale nearest to `wanted` (>= 0), ties to the even byte.  `wanted` has a bit set below
+// its 24 wherever something was cut off, so that this is the only rounding.
+__device__ __forceinline__ unsigned scale_byte(float wanted) {
+    const unsigned bits = __float_as_uint(wanted);
+    const unsigned normal = ((bits + 0x7FFFFu + ((bits >> 20) & 1u)) >> 20) - (112u << 3);
+    const unsigned byte = wanted < 6.103515625e-05f ? __float2uint_rn(wanted * 131072.f) : normal;
+    return min(byte, (unsigned)FP4_MAX_SCALE);
+}
+__device__ __forceinline__ float scale_value(unsigned byte) {
+    return __half2float(__ushort_as_half((unsigned short)(byte << 7)));
+}
+
+// Two 4-bit floats, `lo` in the low half of the byte: nearest, ties to the even code, at most 6.
+__device__ __forceinline__ unsigned codes_of(float lo, float hi) {
+    unsigned short out;
+    asm("{\n.reg .b8 c;\ncvt.rn.satfinite.e2m1x2.f32 c, %1, %2;\nmov.b16 %0, {c, 0};\n}" : "=h"(out) : "f"(hi), "f"(lo));
+    return out;
+}
+
+// `v` cut to 32 bits with the last bit set where something was cut off.
+__device__ __forceinline__ float cut_sticky(double v) {
+    const float f = __double2float_rz(v);
+    return (double)f == v ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+
+// The codes (8 features a lane, four bytes) and the scale of the 16 features that two neighbouring lanes hold.
+__device__ __forceinline__ unsigned quantise(const double (&x)[8], unsigned mask, unsigned& scale) {
+    double largest = 0.0;
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const double a = fabs(x[e]);
+        finite = finite && a < INFINITY;
+        largest = fmax(largest, a);
+    }
+    largest = fmax(largest, __shfl_xor_sync(mask, largest, 1));
+    finite = __shfl_xor_sync(mask, (int)finite, 1) && finite;
+    scale = finite ? scale_byte(cut_sticky(fmin(largest / 6.0, 10240.0))) : (unsigned)FP4_NAN_SCALE;
+    if (!finite) return 0u;
+    const double s = scale_value(scale);
+    // A shade more than 1 / s, so that a quotient that is a border exactly is not cut below it.
+    const double inverse = s > 0.0 ? 1.0 / s * (1.0 + 8.8817841970012523e-16) : 0.0;
+    unsigned out = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f[i] = __double2float_rz(x[e + i] * inverse);
+            if ((double)f[i] * s != x[e + i]) f[i] = __uint_as_float(__float_as_uint(f[i]) | 1u);
+        }
+        out |= codes_of(f[0], f[1]) << (4 * e);
+    }
+    return out;
+}
+__device__ __forceinline__ unsigned quantise(const float (&x)[8], unsigned mask, unsigned& scale) {
+    float largest = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float a = fabsf(x[e]);
+        finite = finite && a < INFINITY;
+        largest = fmaxf(largest, a);
+    }
+    largest = fmaxf(largest, __shfl_xor_sync(mask, largest, 1));
+    finite = __shfl_xor_sync(mask, (int)finite, 1) && finite;
+    scale = finite ? scale_byte(fminf(__fdiv_rn(largest, 6.f), 10240.f)) : (unsigned)FP4_NAN_SCALE;
+    const float s = scale_value(scale);
+    if (!(s > 0.f)) return 0u;
+    unsigned out = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) out |= codes_of(__fdiv_rn(x[e], s), __fdiv_rn(x[e + 1], s)) << (4 * e);
+    return out;
+}
+
+// Norm and rotation of one head, eight features a lane, in 32 or 64 bits.  `other_lane`: the lane that holds the
+// rotation's partners; STAGED: they are fetched one by one through `stage`, a row of D of its own.
+template <typename F, int D, bool STAGED>
+__device__ __forceinline__ void norm_rotate(F (&v)[8], const float* __restrict__ weight, float eps, const float2* __restrict__ cs,
+                                            int half, int part, unsigned mask, F* stage) {
+    constexpr int LANES = D / 8;
+    if (weight) {
+        F ss = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+        const F inv = sizeof(F) == 4 ? (F)rsqrtf((float)ss / (float)D + eps) : (F)rsqrt((double)ss / (double)D + (double)eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * (F)weight[part * 8 + e];
+    }
+    if (half == 0) return;
+    if constexpr (STAGED) {
+        __syncwarp(mask);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) stage[part * 8 + e] = v[e];
+        __syncwarp(mask);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int j = part * 8 + e;
+            if (j < half) v[e] = v[e] * (F)cs[j].x - stage[j + half] * (F)cs[j].y;
+            else if (j < 2 * half) v[e] = v[e] * (F)cs[j - half].x + stage[j - half] * (F)cs[j - half].y;
+        }
+    } else {
+        // rotary_dim is a multiple of 16: a lane's partners are another lane's eight features
+        const int away = half / 8;
+        const bool low = part < away, turns = part < 2 * away;
+        const int partner = turns ? (low ? part + away : part - away) : part;
+        const int base = (int)(threadIdx.x & 31) - part;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const F other = __shfl_sync(mask, v[e], base + partner);
+            if (turns) {
+                const float2 c = cs[(low ? part : partner) * 8 + e];
+                v[e] = low ? v[e] * (F)c.x - other * (F)c.y : v[e] * (F)c.x + other * (F)c.y;
+            }
+        }
+    }
+}
+
+template <int D, bool STAGED>
+__global__ void __launch_bounds__(256)
+qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, long q_stride,
+                              const float* __restrict__ q_weight, const float* __restrict__ k_weight, float eps,
+                              const float2* __restrict__ rot, int half, const int* __restrict__ slots,
+                              unsigned char* __restrict__ cache, int tokens, int heads, int kv_heads, int page_size, long pages) {
+    using Unit = Fp4Unit<D>;
+    constexpr int LANES = D / 8;
+    __shared__ double stage_all[STAGED ? 256 / LANES * D : 1];
+    const int per_token = heads + 2 * kv_heads;
+    const int groups_per_token = (per_token + HEADS_PER_GROUP - 1) / HEADS_PER_GROUP;
+    const long group = ((long)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
+    const int part = threadIdx.x % LANES;
+    if (group >= (long)tokens * groups_per_token) return;          // all lanes of a group together
+    const int t = (int)(group / groups_per_token);
+    const int head0 = (int)(group - (long)t * groups_per_token) * HEADS_PER_GROUP;
+    const int head1 = min(per_token, head0 + HEADS_PER_GROUP);
+    const unsigned lane = threadIdx.x & 31;
+    const unsigned mask = ((1u << LANES) - 1u) << (lane & ~(unsigned)(LANES - 1));
+    double* stage = stage_all + (STAGED ? threadIdx.x / LANES * D : 0);
+    const float2* cs = rot + (size_t)t * half;
+
+    // a slot outside the cache (a padding row's -1) writes nothing
+    const int slot = slots ? slots[t] : -1;
+    const int page = slot >= 0 ? slot / page_size : -1;
+    const bool writes = page >= 0 && page < pages;
+    const int off = slot - page * page_size, r = off & (FP4_TOKENS - 1);
+    const int units = page_size / FP4_TOKENS;
+
+    for (int head = head0; head < head1; ++head) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(qkv + ((size_t)t * per_token + head) * D + part * 8);
+        float x[8];
+        {
+            const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = __bfloat1622float2(pairs[e]);
+                x[2 * e] = f.x; x[2 * e + 1] = f.y;
+            }
+        }
+        if (head < heads) {
+            norm_rotate<float, D, STAGED>(x, q_weight, eps, cs, half, part, mask, reinterpret_cast<float*>(stage));
+            uint4 packed;
+            __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+            *reinterpret_cast<uint4*>(q_out + (size_t)t * q_stride + (size_t)head * D + part * 8) = packed;
+            continue;
+        }
+        if (!writes) continue;
+        const bool is_k = head < heads + kv_heads;
+        const int kv_head = is_k ? head - heads : head - heads - kv_heads;
+        unsigned char* unit = cache + (((size_t)page * kv_heads + kv_head) * units + off / FP4_TOKENS) * Unit::BYTES;
+        unsigned scale, codes;
+        if (is_k) {
+            double y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[e];
+            norm_rotate<double, D, STAGED>(y, k_weight, eps, cs, half, part, mask, stage);
+            codes = quantise(y, mask, scale);
+        } else {
+            codes = quantise(x, mask, scale);
+        }
+        // eight features are four bytes of one piece: D = 128 has pieces of eight bytes, D = 64 of four
+        *reinterpret_cast<unsigned*>(unit + (is_k ? Unit::k_code(r, part * 4) : Unit::v_code(r, part * 4))) = codes;
+        if ((part & 1) == 0) unit[is_k ? Unit::k_scale(r, part / 2) : Unit::v_scale(r, part / 2)] = (unsigned char)scale;
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// Reading back into rows [page, kv head, row, :] of bfloat16 keys and values (exact: a value has at most 6
+// significant bits).  A block takes 16 rows of one kv head, a thread eight features of a key and of a value.
+//   ids      output page i is cache page ids[i]
+//   ranges   output page i holds tokens ranges[i].y .. of the request in block-table row ranges[i].x, its first
+//            ranges[i].z rows; the rest are zeros
+// A page outside the cache gives zeros.
+// ------------------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned half2_of_codes(unsigned byte) {
+    unsigned out;
+    asm("{\n.reg .b8 c, z;\nmov.b16 {c, z}, %1;\ncvt.rn.f16x2.e2m1x2 %0, c;\n}" : "=r"(out) : "h"((unsigned short)byte));
+    return out;
+}
+
+template <int D>
+__global__ void __launch_bounds__(2 * D)
+fp4_rows_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ ids, const int4* __restrict__ ranges,
+                const int* __restrict__ block_tables, int table_rows, int max_blocks, bf16* __restrict__ k_out, bf16* __restrict__ v_out,
+                int kv_heads, int page_size, int out_page, long pages) {
+    using Unit = Fp4Unit<D>;
+    constexpr int LANES = D / 8;
+    const int units_out = out_page / FP4_TOKENS, units_in = page_size / FP4_TOKENS;
+    const int i = blockIdx.x / units_out, unit_out = blockIdx.x - i * units_out, kv_head = blockIdx.y;
+    const int part = threadIdx.x % LANES, r = threadIdx.x / LANES;
+    long page = -1;
+    int unit_in = unit_out, rows = FP4_TOKENS;
+    if (ids) {
+        page = ids[i];
+    } else {
+        const int4 range = ranges[i];
+        const int unit = range.y / FP4_TOKENS + unit_out, block = unit / units_in;      // a range begins with a unit
+        unit_in = unit - block * units_in;
+        rows = range.z - unit_out * FP4_TOKENS;
+        if (rows > 0 && range.x >= 0 && range.x < table_rows && block < max_blocks) page = block_tables[(size_t)range.x * max_blocks + block];
+    }
+    uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (page >= 0 && page < pages && r < rows) {
+        const unsigned char* unit = cache + ((size_t)(page * kv_heads + kv_head) * units_in + unit_in) * Unit::BYTES;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            const unsigned codes = *reinterpret_cast<const unsigned*>(unit + (kv ? Unit::v_code(r, part * 4) : Unit::k_code(r, part * 4)));
+            const float s = scale_value(unit[kv ? Unit::v_scale(r, part / 2) : Unit::k_scale(r, part / 2)]);
+            __nv_bfloat162* pairs = reinterpret_cast<__nv_bfloat162*>(&out[kv]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned h = half2_of_codes((codes >> (8 * e)) & 0xFFu);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                pairs[e] = __floats2bfloat162_rn(f.x * s, f.y * s);
+            }
+        }
+    }
+    const size_t row = ((size_t)i * kv_heads + kv_head) * out_page + unit_out * FP4_TOKENS + r;
+    *reinterpret_cast<uint4*>(k_out + row * D + part * 8) = out[0];
+    *reinterpret_cast<uint4*>(v_out + row * D + part * 8) = out[1];
+}
+
+template <int D>
+cudaError_t launch_store(const void* qkv, void* q_out, long q_stride, const float* q_weight, const float* k_weight, float eps,
+                         const float* rot, int rotary_dim, const int* slots, void* cache, int tokens, int heads, int kv_heads,
+                         int page_size, long pages, cudaStream_t stream) {
+    const long groups = (long)tokens * ((heads + 2 * kv_heads + HEADS_PER_GROUP - 1) / HEADS_PER_GROUP);
+    const dim3 grid((unsigned)((groups * (D / 8) + 255) / 256));
+    return launch_kernel(rotary_dim % 16 ? qk_norm_rope_cache_fp4_kernel<D, true> : qk_norm_rope_cache_fp4_kernel<D, false>, grid,
+                         dim3(256), 0, stream, (const bf16*)qkv, (bf16*)q_out, q_stride, q_weight, k_weight, eps, (const float2*)rot,
+                         rotary_dim / 2, slots, (unsigned char*)cache, tokens, heads, kv_heads, page_size, pages);
+}
+
+}  // namespace
+
+#define MRUN_REQUIRE_FP4(head_dim, page_size, name)                                                                   \
+    MRUN_REQUIRE((head_dim) == 64 || (head_dim) == 128, "%s: head_dim=%d: the 4-bit cache takes heads of 64 or 128 features", name, head_dim); \
+    MRUN_REQUIRE((page_size) > 0 && (page_size) % mrun::FP4_TOKENS == 0, "%s: page_size=%d is not a multiple of 16", name, page_size)
+
+MRUN_API int mrun_qk_norm_rope_cache_fp4(const void* qkv, void* q_out, long q_stride, const float* q_weight, const float* k_weight,
+                                         float eps, const float* rot, int rotary_dim, const int* slots, void* cache, int tokens,
+                                         int heads, int kv_heads, int head_dim, int page_size, long pages, cudaStream_t stream) {
+    const char* name = "qk_norm_rope_cache_fp4";
+    MRUN_REQUIRE(tokens >= 0 && heads > 0 && kv_heads > 0 && pages >= 0, "%s: bad sizes", name);
+    MRUN_REQUIRE_FP4(head_dim, page_size, name);
+    MRUN_REQUIRE(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 2 == 0,
+                 "%s: rotary_dim=%d must be even and at most head_dim=%d", name, rotary_dim, head_dim);
+    MRUN_REQUIRE(rotary_dim == 0 || rot, "%s: rotary_dim=%d without a table", name, rotary_dim);
+    MRUN_REQUIRE((q_weight == nullptr) == (k_weight == nullptr), "%s: q and k norm weights come together", name);
+    MRUN_REQUIRE(slots == nullptr || cache, "%s: slots without a cache", name);
+    MRUN_REQUIRE(((uintptr_t)qkv & 15) == 0 && ((uintptr_t)q_out & 15) == 0 && q_stride % 8 == 0 && ((uintptr_t)cache & 15) == 0,
+                 "%s: rows and pages start on 16 bytes", name);
+    MRUN_REQUIRE(((uintptr_t)rot & 7) == 0, "%s: the table starts on 8 bytes", name);
+    if (tokens == 0) return 0;
+    MRUN_CHECK_CUDA(head_dim == 64 ? launch_store<64>(qkv, q_out, q_stride, q_weight, k_weight, eps, rot, rotary_dim, slots, cache, tokens,
+                                                      heads, kv_heads, page_size, pages, stream)
+                                   : launch_store<128>(qkv, q_out, q_stride, q_weight, k_weight, eps, rot, rotary_dim, slots, cache, tokens,
+                                                       heads, kv_heads, page_size, pages, stream),
+                    name);
+    MRUN_CHECK_LAUNCH(name);
+    return 0;
+}
+
+// Either `ids` or `ranges` (with the block tables), int [n] or [n, 4]; out_page: rows of an output page.
+MRUN_API int mrun_fp4_rows(const void* cache, const int* ids, const void* ranges, const int* block_tables, int table_rows, int max_blocks,
+                           void* k_out, void* v_out, int n, int kv_heads, int head_dim, int page_size, int out_page, long pages,
+                           cudaStream_t stream) {
+    const char* name = "fp4_rows";
+    MRUN_REQUIRE(n >= 0 && kv_heads > 0 && kv_heads < 65536 && pages >= 0, "%s: bad sizes", name);
+    MRUN_REQUIRE_FP4(head_dim, page_size, name);
+    MRUN_REQUIRE(out_page > 0 && out_page % FP4_TOKENS == 0 && (ranges || out_page == page_size), "%s: out_page=%d", name, out_page);
+    MRUN_REQUIRE((ids != nullptr) != (ranges != nullptr) && (!ranges || block_tables), "%s: pages or ranges of block tables", name);
+    MRUN_REQUIRE((((uintptr_t)cache | (uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)ranges) & 15) == 0, "%s: pages start on 16 bytes", name);
+    if (n == 0) return 0;
+    const long blocks = (long)n * (out_page / FP4_TOKENS);
+    MRUN_REQUIRE(blocks < (1L << 31), "%s: %d pages are more than a launch takes", name, n);
+    const dim3 grid((unsigned)blocks, (unsigned)kv_heads);
+    const auto launch = [&](auto kernel) {
+        return launch_kernel(kernel, grid, dim3(2 * head_dim), 0, stream, (const unsigned char*)cache, ids, (const int4*)ranges, block_tables,
+                             table_rows, max_blocks, (bf16*)k_out, (bf16*)v_out, kv_heads, page_size, out_page, pages);
+    };
+    MRUN_CHECK_CUDA(head_dim == 64 ? launch(fp4_rows_kernel<64>) : launch(fp4_rows_kernel<128>), name);
+    MRUN_CHECK_LAUNCH(name);
+    return 0;
+}

@@ -22,7 +22,9 @@ the fused norm/rotary/cache kernel just before.
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 import math
+from dataclasses import dataclass
 from typing import Optional
 
 import numpy as np
@@ -479,3 +481,153 @@ def prefill_uses_tcgen05(library, ratio: int, page_size: int) -> bool:
     if have is None:
         have = _tc5_prefill[library.path] = int(library._dll.mrun_attn_prefill_tc5_rows())
     return have > 0
+
+
+# ------------------------------------------------------------------ the 4-bit cache
+# Segments of up to this many tokens take the kernel for single tokens, row by row; longer ones have their keys
+# and values read back.
+FP4_SHORT = 4
+FP4_SCRATCH_ROWS = 128     # rows of a page that is read back: a key tile of the tcgen05 prompt kernel
+_fp4_slots = {}            # (device, head size, heads a block) -> blocks of the decode kernel that the device holds
+
+
+@dataclass
+class _Pages:
+    """Keys and values read back, as the kernels over bfloat16 pages take a cache."""
+    k: torch.Tensor
+    v: torch.Tensor
+
+
+@dataclass
+class _View:
+    block_tables: torch.Tensor
+    max_blocks: int
+
+
+def _fp4_blocks(library, device: torch.device, head_dim: int, ratio: int) -> tuple:
+    """(blocks of the decode kernel that the device holds, heads that a block takes)."""
+    rows = 8 if ratio <= 8 else 16
+    found = _fp4_slots.get((device, head_dim, rows))
+    if found is None:
+        per_sm = library.function("mrun_attn_fp4_occupancy")(head_dim, ratio)
+        if per_sm < 1:
+            raise ops.KernelError("paged_attention_fp4: the device does not take the decode kernel")
+        found = _fp4_slots[(device, head_dim, rows)] = per_sm * ops.sm_count(device)
+    return found, rows
+
+
+FP4_MAX_TOKENS = 512       # tokens of one launch of the decode kernel
+
+
+def _fp4_tokens(q, q_stride: int, out, cache, group, heads: int, head_dim: int, scale: float, window: int, token_slot, positions,
+                rows, tokens: int, max_kv_len: int) -> None:
+    """Single tokens: those of the step, or the rows ``rows`` of it."""
+    pages, kv_heads, units, _ = cache.shape
+    ratio = heads // kv_heads
+    library = _lib.fp4()
+    slots, block_heads = _fp4_blocks(library, q.device, head_dim, ratio)
+    pairs_a_token = kv_heads * -(-ratio // block_heads)
+    for first in range(0, tokens, FP4_MAX_TOKENS):
+        n = min(FP4_MAX_TOKENS, tokens - first)
+        # no more blocks than tiles of 64 keys (an unaligned window touches one more)
+        most = n * pairs_a_token * (-(-min(max_kv_len, window if window > 0 else max_kv_len) // 64) + 1)
+        blocks = max(1, min(slots, most))
+        part_o = torch.empty((blocks, 2, block_heads, head_dim), dtype=torch.float32, device=q.device)
+        part_ml = torch.empty((blocks, 2, block_heads, 2), dtype=torch.float32, device=q.device)
+        here = slice(first, first + n)
+        library.call("mrun_attn_fp4_decode", _address(q if rows is not None else q[here]), q_stride,
+                     _address(out if rows is not None else out[here]), _address(cache), _address(group.block_tables),
+                     group.block_tables.shape[0], group.block_tables.shape[1], _address(token_slot[here]), _address(positions[here]),
+                     _address(rows[here] if rows is not None else None), n, heads, kv_heads, head_dim, units * ops.FP4_TOKENS, pages,
+                     scale, window, _address(part_o), _address(part_ml), blocks, _queue())
+
+
+def _fp4_portions(ctx, window: int, short: int):
+    """What a step's prompt portions need, made once per step: ``(rows, positions, slots)`` of the tokens of its short segments and
+    their number, and for the others the ranges of tokens to read back, a step context over them and their block tables."""
+    key = ("fp4_portions", window, short)
+    found = ctx.shared.get(key)
+    if found is not None:
+        return found
+    few, many = [], []
+    for seg in ctx.segments:
+        (few if seg.q_len <= short else many).append(seg)
+    rows = [seg.q_start + i for seg in few for i in range(seg.q_len)]
+    positions = [seg.pos_start + i for seg in few for i in range(seg.q_len)]
+    slots = [seg.slot for seg in few for _ in range(seg.q_len)]
+    ranges, tables = [], []
+    for seg in many:
+        end = seg.pos_start + seg.q_len
+        first = _first_visible(seg.pos_start, window) // FP4_SCRATCH_ROWS
+        table = [-1] * first
+        for block in range(first, -(-end // FP4_SCRATCH_ROWS)):
+            table.append(len(ranges))
+            ranges.append((seg.slot, block * FP4_SCRATCH_ROWS, min(FP4_SCRATCH_ROWS, end - block * FP4_SCRATCH_ROWS), 0))
+        tables.append(table)
+    width = max((len(table) for table in tables), default=0)
+    token_row = np.full(ctx.num_tokens, -1, dtype=np.int32)
+    for i, seg in enumerate(many):
+        token_row[seg.q_start:seg.q_start + seg.q_len] = i
+    parts = [np.asarray(ranges, dtype=np.int32).reshape(-1), np.asarray(rows, dtype=np.int32), np.asarray(positions, dtype=np.int32),
+             np.asarray(slots, dtype=np.int32), token_row,
+             np.asarray([table + [-1] * (width - len(table)) for table in tables], dtype=np.int32).reshape(-1)]
+    sent = ctx.upload(np.concatenate(parts))
+    at = np.cumsum([0] + [part.size for part in parts]).tolist()
+    take = lambda i: sent[at[i]:at[i + 1]]
+    singles = (take(1), take(2), take(3), len(rows))
+    longer = None
+    if many:
+        segments = [dataclasses.replace(seg, slot=i) for i, seg in enumerate(many)]
+        inner = dataclasses.replace(ctx, segments=segments, num_segments=len(segments), token_slot=take(4), shared={},
+                                    max_q_len=max(seg.q_len for seg in many), page_size=FP4_SCRATCH_ROWS)
+        longer = (take(0).view(-1, 4), inner, _View(take(5).view(len(many), width), width))
+    found = ctx.shared[key] = (singles, longer)
+    return found
+
+
+def _first_visible(position: int, window: int) -> int:
+    if window > 0:
+        return max(0, position - window + 1)
+    return position - position % -window if window < 0 else 0
+
+
+def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache: torch.Tensor, group, ctx, heads: int, head_dim: int,
+                        scale: float, window: int = 0) -> torch.Tensor:
+    """:func:`paged_attention` over a 4-bit cache (``cache``: pages of :func:`mrun_b200.kernels.ops.fp4_cache_shape`): bfloat16, heads
+    of 64 or 128 features, pages of a multiple of 16 tokens, any number of query heads a kv head.
+
+    Single tokens, and segments of up to ``FP4_SHORT``, read the 4-bit pages as they are (every step of single tokens may be
+    captured in a graph).  The keys and values of longer segments are read back in bfloat16, 128 tokens a page, for the time of
+    the call (4 * head_dim bytes a token and kv head of the segments' contexts), and go to the prompt kernels.  A page outside the cache is not
+    seen; a row that sees nothing is zeros.  A value that is NaN makes NaN of the rows that see it, and may of other rows of
+    the same prompt portion."""
+    pages, kv_heads, page_size = ops.check_fp4_cache(cache, head_dim)
+    if heads < 1 or heads % kv_heads:
+        raise ops.KernelError(f"paged_attention_fp4: heads={heads} is not a multiple of kv_heads={kv_heads}")
+    tokens = ctx.num_tokens
+    if out.shape != (tokens, heads * head_dim):
+        raise ops.KernelError(f"paged_attention_fp4: out is {tuple(out.shape)}, expected {(tokens, heads * head_dim)}")
+    if page_size != ctx.page_size:
+        raise ops.KernelError(f"paged_attention_fp4: the cache has pages of {page_size} tokens, the step of {ctx.page_size}")
+    if q.dim() != 2 or q.shape[0] != tokens or q.stride(1) != 1 or (tokens > 1 and q.stride(0) != q_stride) or q.shape[1] < heads * head_dim:
+        raise ops.KernelError(f"paged_attention_fp4: q is {tuple(q.shape)} with strides {q.stride()}, expected {tokens} rows of "
+                              f"{heads * head_dim} features every {q_stride}")
+    ops._check(q, "q", torch.bfloat16, dense=False)
+    ops._check(out, "out", torch.bfloat16); ops._check(cache, "cache", torch.uint8)
+    for name, t in (("block_tables", group.block_tables), ("positions", ctx.positions), ("token_slot", ctx.token_slot)):
+        ops._check(t, name, torch.int32)
+    if ctx.all_decode:
+        _fp4_tokens(q, q_stride, out, cache, group, heads, head_dim, scale, window, ctx.token_slot, ctx.positions, None, tokens, ctx.max_kv_len)
+        return out
+    if tokens > ctx.real_tokens:
+        out[ctx.real_tokens:].zero_()
+    # the prompt kernels over tensor cores take up to 64 query heads a kv head
+    short = FP4_SHORT if heads // kv_heads <= 64 else tokens
+    (rows, positions, slots, n), longer = _fp4_portions(ctx, window, short)
+    if n:
+        _fp4_tokens(q, q_stride, out, cache, group, heads, head_dim, scale, window, slots, positions, rows, n, ctx.max_kv_len)
+    if longer is not None:
+        ranges, inner, view = longer
+        k, v = ops.fp4_ranges(cache, head_dim, group.block_tables, ranges, FP4_SCRATCH_ROWS)
+        paged_attention(q, q_stride, out, _Pages(k, v), view, inner, heads, scale, window)
+    return out

@@ -191,6 +191,14 @@ def build_core() -> str:
     return build_library("mrun_core", CORE_SOURCES, {})
 
 
+FP4_SOURCES = ("common.cu", "cache_fp4.cu", "attention_fp4.cu")
+
+
+def build_fp4() -> str:
+    """The kernels of the 4-bit key/value cache (head sizes 64 and 128)."""
+    return build_library("mrun_fp4", FP4_SOURCES, {})
+
+
 ATTENTION_SOURCES = ("common.cu", "attention_mma.cu", "attention_decode_tma.cu", "attention_tc5.cu")
 
 
@@ -221,6 +229,6 @@ COMMON_VALUE_DIMS = ((192, 128), (192, 64), (32, 16), (64, 128), (128, 64), (80,
 def build_all() -> list[str]:
     """Every library the package loads for the configurations it measures and tests; other head
     sizes are built when a model with them is first run."""
-    return ([build_host(), build_core()] + [build_attention(d) for d in COMMON_HEAD_DIMS]
+    return ([build_host(), build_core(), build_fp4()] + [build_attention(d) for d in COMMON_HEAD_DIMS]
             + [build_attention(d, v) for d, v in COMMON_VALUE_DIMS]
             + [build_attention(d, v, scored=True) for d, v in COMMON_SCORED_DIMS])

@@ -103,6 +103,7 @@ def call_count() -> int:
 
 
 _core: Library | None = None
+_fp4: Library | None = None
 _attention: Dict[tuple, Library] = {}
 
 
@@ -116,6 +117,14 @@ def core() -> Library:
             raise KernelError(f"{lib.path} was not built for sm_100a")
         _core = lib
     return _core
+
+
+def fp4() -> Library:
+    """The kernels of the 4-bit key/value cache, built at first use."""
+    global _fp4
+    if _fp4 is None:
+        _fp4 = Library(build.build_fp4())
+    return _fp4
 
 
 def attention(head_dim: int, value_dim: int | None = None, scored: bool = False) -> Library:

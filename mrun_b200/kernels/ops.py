@@ -257,6 +257,103 @@ def qk_norm_rope_cache(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: i
                      kv_heads, head_dim, page_size, _queue())
 
 
+FP4_TOKENS = 16            # tokens of a unit of the 4-bit cache
+FP4_HEAD_DIMS = (64, 128)
+
+
+def fp4_unit_bytes(head_dim: int) -> int:
+    """Bytes that 16 tokens of one kv head take in the 4-bit cache: half a byte a feature of the key and of the value
+    and a byte a group of 16 features (the layout is with ``csrc/fp4_unit.cuh``)."""
+    if head_dim not in FP4_HEAD_DIMS:
+        raise KernelError(f"the 4-bit cache takes heads of 64 or 128 features, not {head_dim}")
+    return FP4_TOKENS * (head_dim + head_dim // 8)
+
+
+def fp4_cache_shape(pages: int, kv_heads: int, page_size: int, head_dim: int) -> tuple:
+    """The shape of a 4-bit cache's pages (uint8): a page of a kv head is a run of units of 16 tokens."""
+    if page_size < 1 or page_size % FP4_TOKENS:
+        raise KernelError(f"the 4-bit cache takes pages of a multiple of {FP4_TOKENS} tokens, not {page_size}")
+    return (pages, kv_heads, page_size // FP4_TOKENS, fp4_unit_bytes(head_dim))
+
+
+def check_fp4_cache(cache: torch.Tensor, head_dim: int, kv_heads: Optional[int] = None) -> tuple:
+    """(pages, kv heads, page size) of a 4-bit cache's pages, from their shape."""
+    if cache.dim() != 4 or cache.shape[3] != fp4_unit_bytes(head_dim) or cache.shape[1] < 1 or cache.shape[2] < 1 \
+            or (kv_heads is not None and cache.shape[1] != kv_heads):
+        raise KernelError(f"the 4-bit cache is {tuple(cache.shape)}, expected [pages, {kv_heads or 'kv heads'}, page_size / {FP4_TOKENS}, "
+                          f"{fp4_unit_bytes(head_dim)}] for heads of {head_dim} features")
+    return cache.shape[0], cache.shape[1], cache.shape[2] * FP4_TOKENS
+
+
+def qk_norm_rope_cache_fp4(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+                           q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float,
+                           rot: Optional[torch.Tensor], rotary_dim: int, slots: Optional[torch.Tensor],
+                           cache: Optional[torch.Tensor], q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """As :func:`qk_norm_rope_cache` for bfloat16 rows and a 4-bit cache (``cache``: pages of :func:`fp4_cache_shape`): q in place,
+    or into the rows ``q_out`` (which may be strided) with ``qkv`` left as it is; k (normed, rotated, not rounded in between) and v
+    quantised into the places that ``slots`` names (page * page_size + offset, each at most once; outside the cache: not written).
+    Returns q's rows."""
+    if qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * kv_heads) * head_dim:
+        raise KernelError(f"qk_norm_rope_cache_fp4: qkv is {tuple(qkv.shape)}, expected width {(heads + 2 * kv_heads) * head_dim}")
+    if head_dim not in FP4_HEAD_DIMS:
+        raise KernelError(f"the 4-bit cache takes heads of 64 or 128 features, not {head_dim}")
+    tokens = qkv.shape[0]
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and w.numel() != head_dim:
+            raise KernelError(f"qk_norm_rope_cache_fp4: {name} has {w.numel()} elements, head_dim is {head_dim}")
+    if rot is not None and rot.shape != (tokens, rotary_dim // 2, 2):
+        raise KernelError(f"qk_norm_rope_cache_fp4: rot is {tuple(rot.shape)}, expected {(tokens, rotary_dim // 2, 2)}")
+    if slots is not None and (cache is None or slots.shape != (tokens,)):
+        raise KernelError("qk_norm_rope_cache_fp4: one slot per token is needed, and the cache they lie in")
+    if q_out is not None and q_out.shape != (tokens, heads * head_dim):
+        raise KernelError(f"qk_norm_rope_cache_fp4: q_out is {tuple(q_out.shape)}, expected {(tokens, heads * head_dim)}")
+    pages, page_size = 0, FP4_TOKENS
+    if slots is not None:
+        pages, _, page_size = check_fp4_cache(cache, head_dim, kv_heads)
+        _check(slots, "slots", torch.int32); _check(cache, "cache", torch.uint8)
+    _check(qkv, "qkv", torch.bfloat16)
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("rot", rot)):
+        if t is not None:
+            _check(t, name, torch.float32)
+    q, stride = qkv[:, :heads * head_dim], qkv.shape[1]
+    if q_out is not None:
+        _check(q_out, "q_out", torch.bfloat16, dense=False)
+        q, stride = q_out, _strided_rows(q_out, "q_out")
+    _lib.fp4().call("mrun_qk_norm_rope_cache_fp4", _address(qkv), _address(q), stride, _address(q_weight), _address(k_weight), eps,
+                    _address(rot), rotary_dim if rot is not None else 0, _address(slots), _address(cache if slots is not None else None),
+                    tokens, heads, kv_heads, head_dim, page_size, pages, _queue())
+    return q
+
+
+def fp4_pages(cache: torch.Tensor, head_dim: int, pages: torch.Tensor):
+    """(keys, values): bfloat16 [n, kv heads, page_size, head_dim] each, what the pages ``pages`` (int32 [n]) of a 4-bit cache hold,
+    exactly; a page outside the cache reads as zeros."""
+    if pages.dim() != 1:
+        raise KernelError(f"fp4_pages: pages is {tuple(pages.shape)}, expected a list")
+    held, kv_heads, page_size = check_fp4_cache(cache, head_dim)
+    _check(cache, "cache", torch.uint8); _check(pages, "pages", torch.int32)
+    k = torch.empty((pages.numel(), kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty_like(k)
+    _lib.fp4().call("mrun_fp4_rows", _address(cache), _address(pages), _address(None), _address(None), 0, 0, _address(k), _address(v),
+                    pages.numel(), kv_heads, head_dim, page_size, page_size, held, _queue())
+    return k, v
+
+
+def fp4_ranges(cache: torch.Tensor, head_dim: int, block_tables: torch.Tensor, ranges: torch.Tensor, rows: int):
+    """(keys, values): bfloat16 [n, kv heads, rows, head_dim] each.  Entry i holds tokens ``ranges[i][1]`` .. (a multiple of 16) of the
+    request in row ``ranges[i][0]`` of the block tables: its first ``ranges[i][2]`` rows, then zeros (int32 [n, 4], the last
+    unused).  ``rows``: a multiple of 16."""
+    if ranges.dim() != 2 or ranges.shape[1] != 4 or block_tables.dim() != 2:
+        raise KernelError(f"fp4_ranges: ranges {tuple(ranges.shape)}, block_tables {tuple(block_tables.shape)}")
+    held, kv_heads, page_size = check_fp4_cache(cache, head_dim)
+    _check(cache, "cache", torch.uint8); _check(ranges, "ranges", torch.int32); _check(block_tables, "block_tables", torch.int32)
+    k = torch.empty((ranges.shape[0], kv_heads, rows, head_dim), dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty_like(k)
+    _lib.fp4().call("mrun_fp4_rows", _address(cache), _address(None), _address(ranges), _address(block_tables), block_tables.shape[0],
+                    block_tables.shape[1], _address(k), _address(v), ranges.shape[0], kv_heads, head_dim, page_size, rows, held, _queue())
+    return k, v
+
+
 def proj_norm_rope_cache(x: torch.Tensor, q_off: int, k_off: int, v_off: int, heads: int, kv_heads: int, dim: int,
                          vdim: int, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float,
                          rot: Optional[torch.Tensor], rotary_dim: int, pairing: str, slots: Optional[torch.Tensor],
