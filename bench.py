@@ -204,7 +204,7 @@ def serve(args, config, model_name: str, full_layers: int, page_size: int, peaks
     prompts = [seeded_tokens(config.vocab_size, n, 200 + i) for i, n in enumerate(lengths)]
     capacity = sum(-(-(n + decode_tokens) // page_size) for n in lengths) + 64
     engine = Engine.from_config(config, seed=0, dtype="bfloat16", page_size=page_size, num_pages=capacity,
-                                max_requests=requests, max_batch_tokens=PREFILL_TOKENS)
+                                max_requests=requests, max_batch_tokens=PREFILL_TOKENS, kv_cache=args.kv_cache)
     engine.generate([p[:300] for p in prompts[:4]], max_tokens=8, ignore_eos=True)       # warm-up: shapes, graphs
     engine.generate(prompts[:2], max_tokens=4, ignore_eos=True)
     sampler = ClockSampler()
@@ -740,6 +740,8 @@ def main() -> int:
                         help="tokens already in the cache before the timed portion of 2,048 (0: a fresh prompt)")
     parser.add_argument("--skip-e2e", action="store_true")
     parser.add_argument("--page-size", type=int, default=16, help="keys a cache page holds")
+    parser.add_argument("--kv-cache", choices=["auto", "fp4"], default="auto",
+                        help="what the Qwen3 shapes hold keys and values as: bfloat16 (auto), or 4 bits")
     parser.add_argument("--repeats", type=int, default=5,
                         help="how many times the K timed steps are run (the line carries the median, the "
                              "fastest and the slowest)")
@@ -751,6 +753,8 @@ def main() -> int:
                              "(prefill of 2,048 tokens, decode at batch 8)")
     parser.add_argument("--sizes", default=None, help="with --design: which of its size sets to run, comma separated")
     args = parser.parse_args()
+    if args.design and args.kv_cache != "auto":
+        parser.error("--kv-cache is for the Qwen3 shapes")
 
     if args.impl == "reference":
         print(json.dumps({"impl": "reference", "unavailable":
@@ -797,10 +801,10 @@ def main() -> int:
     config = Qwen3Config(**sizes)
     engine = Engine.from_config(config, seed=0, dtype="bfloat16", page_size=page_size,
                                 num_pages=-(-capacity // page_size), max_requests=max(64, sum(batches)),
-                                max_batch_tokens=max(PREFILL_TOKENS, args.prefill_depth))
+                                max_batch_tokens=max(PREFILL_TOKENS, args.prefill_depth), kv_cache=args.kv_cache)
     executor = engine.executor
     vocab = config.vocab_size
-    kv_bytes = config.kv_bytes_per_token(2)
+    kv_bytes = executor.cache.bytes_per_page() // page_size
     # every weight the step uses, once; of an embedding table that is not also the head only B rows
     weight_bytes = executor.model.weight_bytes()
     if not config.tie_word_embeddings:
@@ -930,7 +934,7 @@ def main() -> int:
             "head_dim": d, "intermediate": config.intermediate_size, "vocab": vocab,
             "rope_theta": config.rope_theta, "rms_norm_eps": config.rms_norm_eps,
             "tied": config.tie_word_embeddings, "global_batch": main_batch, "seq_len": context,
-            "max_context": config.max_position_embeddings, "page_size": page_size,
+            "max_context": config.max_position_embeddings, "page_size": page_size, "kv_cache": args.kv_cache,
             "parallelism": "single GPU", "l2": f"inputs larger than L2 ({weight_bytes / 1e9:.0f} GB of weights per step)",
         },
         "e2e": e2e, "gpu_launches": launches, "clocks": clocks,

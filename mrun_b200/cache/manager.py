@@ -4,7 +4,8 @@ the layers need, and slots for per-request state of fixed size.
 * A **group** is the set of schedule entries whose need has the same ``group_key`` (all keys, or
   a window of W keys).  A group has one page pool and, per request, one list of pages indexed by
   logical block (position // page_size).  Every owning entry of the group has key and value
-  tensors ``[pages, kv_heads, page_size, head_dim]`` of its own, indexed by the same page ids.
+  tensors ``[pages, kv_heads, page_size, head_dim]`` of its own, indexed by the same page ids; an entry held in
+  4 bits has one tensor of packed pages.
 * Appending is plan → do → commit, as the reference's ledger works
   (crates/mrun-engine/src/ledger.rs:5-9): :meth:`plan_append` takes every page the step needs
   or raises :class:`OutOfPages` with nothing changed; :meth:`commit` advances the lengths and,
@@ -24,6 +25,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 
+from ..kernels.ops import FP4_TOKENS, fp4_cache_shape, fp4_unit_bytes
 from . import native
 from .needs import FixedState, PagedKV, PagedLatent, PagedMaps, split_need
 from .pages import OutOfPages
@@ -112,11 +114,12 @@ class PagedGroup:
 class EntryCache:
     """The cache of one schedule entry, as its mixer sees it."""
 
-    def __init__(self, need, group_key, writable: bool, k=None, v=None, state=None, states=None):
+    def __init__(self, need, group_key, writable: bool, k=None, v=None, state=None, states=None, packed=None):
         self.need = need
         self.group_key = group_key
         self.writable = writable
         self.k, self.v, self.state = k, v, state
+        self.packed = packed        # the pages of a need with ``fp4``, in place of ``k`` and ``v``
         # every fixed-size state of the entry by its name ([max_requests, *shape] each); ``state``
         # is the first of them
         self.states = dict(states or {})
@@ -131,7 +134,9 @@ def token_bytes(needs: Sequence[object], shares: Sequence[Optional[int]], elemen
         if share is not None or need is None:
             continue
         paged, states = split_need(need)
-        if isinstance(paged, PagedKV):
+        if isinstance(paged, PagedKV) and paged.fp4:
+            per_token += paged.kv_heads * fp4_unit_bytes(paged.head_dim) // FP4_TOKENS
+        elif isinstance(paged, PagedKV):
             per_token += paged.kv_heads * (paged.head_dim + (paged.value_dim or paged.head_dim)) * element_size
         elif isinstance(paged, PagedLatent):
             per_token += paged.width * element_size
@@ -144,6 +149,13 @@ def token_bytes(needs: Sequence[object], shares: Sequence[Optional[int]], elemen
                 count *= extent
             per_slot += count * _STATE_BYTES.get(state.dtype, 4)
     return per_token, per_slot
+
+
+def read_back_bytes(needs: Sequence[object]) -> int:
+    """Bytes of scratch that a prompt portion takes for every token of its context: a layer's keys and values held in 4 bits
+    are read back in 16 bits, one layer at a time."""
+    paged = [split_need(need)[0] for need in needs]
+    return max((4 * p.kv_heads * p.head_dim for p in paged if isinstance(p, PagedKV) and p.fp4), default=0)
 
 
 _STATE_BYTES = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "float64": 8}
@@ -177,7 +189,7 @@ class CacheManager:
                 if owner is None:
                     raise ValueError(f"schedule entry {i} reads the cache of entry {share}, which keeps none")
                 self.entries.append(EntryCache(owner.need, owner.group_key, False, owner.k, owner.v, owner.state,
-                                               owner.states))
+                                               owner.states, owner.packed))
                 continue
             paged, fixed = split_need(need)
             if paged is None and not fixed:
@@ -206,10 +218,15 @@ class CacheManager:
                     group.table_device = torch.full((max_requests, self.max_blocks), FREED,
                                                     dtype=torch.int32, device=device)
             group.entries.append(i)
-            k = v = None
+            k = v = packed = None
+            if isinstance(paged, PagedKV) and paged.fp4 and paged.value_dim not in (None, paged.head_dim):
+                raise ValueError(f"schedule entry {i}: a 4-bit cache holds keys and values of one size, got {paged}")
             if device is not None:
                 import torch
-                if isinstance(paged, PagedLatent):       # one row a token: the key and the value
+                if isinstance(paged, PagedKV) and paged.fp4:
+                    shape = fp4_cache_shape(num_pages, paged.kv_heads, page_size, paged.head_dim)
+                    packed = torch.zeros(shape, dtype=torch.uint8, device=device)
+                elif isinstance(paged, PagedLatent):       # one row a token: the key and the value
                     k = v = torch.zeros((num_pages, 1, page_size, paged.width), dtype=dtype, device=device)
                 elif isinstance(paged, PagedMaps):
                     k = torch.zeros((paged.maps, num_pages, paged.kv_heads, page_size, paged.key_dim),
@@ -220,7 +237,7 @@ class CacheManager:
                     shape = (num_pages, paged.kv_heads, page_size)
                     k = torch.zeros(shape + (paged.head_dim,), dtype=dtype, device=device)
                     v = torch.zeros(shape + (paged.value_dim or paged.head_dim,), dtype=dtype, device=device)
-            self.entries.append(EntryCache(paged, key, True, k=k, v=v, state=first_state, states=states))
+            self.entries.append(EntryCache(paged, key, True, k=k, v=v, state=first_state, states=states, packed=packed))
 
         # the books: pools, block tables, lengths, plans (csrc/host/cache_core.cpp)
         self._lib = native.library()
@@ -267,6 +284,8 @@ class CacheManager:
     def bytes_per_page(self) -> int:
         total = 0
         for entry in self.entries:
+            if entry is not None and entry.writable and entry.packed is not None:
+                total += entry.packed[0].numel()
             if entry is None or not entry.writable or entry.k is None:
                 continue
             if isinstance(entry.need, PagedMaps):

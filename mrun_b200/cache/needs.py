@@ -15,12 +15,14 @@ from typing import Optional, Tuple
 @dataclass(frozen=True)
 class PagedKV:
     """Keys and values of every token (``window`` None) or of the last ``window`` tokens.
-    ``value_dim``: the values' feature size where it differs from the keys' (``head_dim``)."""
+    ``value_dim``: the values' feature size where it differs from the keys' (``head_dim``).  ``fp4``: held in 4 bits, the
+    keys and the values in one tensor of pages (``csrc/fp4_unit.cuh``)."""
 
     kv_heads: int
     head_dim: int
     window: Optional[int] = None
     value_dim: Optional[int] = None
+    fp4: bool = False
 
     def group_key(self) -> tuple:
         return ("paged", self.window)

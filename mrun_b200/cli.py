@@ -3,6 +3,7 @@ reference's token-ids-in example (crates/mrun-engine/examples/generate.rs:1-13).
 
     mrun run MODEL --prompt IDS [--max-tokens N] [--temperature T] [--top-p P] [--top-k K]
                    [--min-p P] [--seed S] [--stop IDS]... [--budget-gib GIB | --context TOKENS] [--info]
+                   [--kv-cache auto|fp4]
     mrun random MODEL_DIR --config CONFIG.json --seed S
 
 ``MODEL`` is a folder with config.json and safetensors.  ``--prompt`` takes token ids, inline or
@@ -99,6 +100,8 @@ def build_parser() -> argparse.ArgumentParser:
     run.add_argument("--info", action="store_true", help="print the memory breakdown after loading and exit")
     run.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     run.add_argument("--page-size", type=int, default=16)
+    run.add_argument("--kv-cache", choices=["auto", "fp4"], default="auto",
+                     help="what keys and values are held as: the compute dtype (auto), or 4 bits")
     run.add_argument("--max-batch-tokens", type=int, default=2048)
     run.add_argument("--ignore-eos", action="store_true")
     run.add_argument("--stop", action="append", default=[], metavar="IDS",
@@ -151,7 +154,7 @@ def command_run(args) -> int:
         memory = budget.plan(budget.read_device(), args.budget_gib)
         engine = Engine.from_folder(args.model, dtype=args.dtype, page_size=args.page_size,
                                     context=args.context, max_requests=1,
-                                    max_batch_tokens=args.max_batch_tokens, memory=memory)
+                                    max_batch_tokens=args.max_batch_tokens, memory=memory, kv_cache=args.kv_cache)
     except budget.BudgetError as error:
         print(f"error: {error}", file=sys.stderr)
         return 4

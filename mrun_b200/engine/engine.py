@@ -8,13 +8,13 @@ follows both: the same option names and meanings, the same finish reasons.
 from __future__ import annotations
 
 import time
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import List, Optional, Sequence, Union
 
 import numpy as np
 import torch
 
-from ..cache.manager import token_bytes
+from ..cache.manager import read_back_bytes, token_bytes
 from ..cache.pages import OutOfPages
 from ..kernels.ops import STATUS_WORDS, status_block
 from ..sampling.mask import TokenMask
@@ -88,16 +88,17 @@ class Engine:
     def from_folder(cls, model_dir: str, dtype: str = "bfloat16", page_size: int = 16,
                     num_pages: Optional[int] = None, context: Optional[int] = None,
                     max_requests: int = 64, max_batch_tokens: int = 2048, reserve: bool = True,
-                    device: str = "cuda:0", memory: Optional[MemoryBudget] = None, **kw) -> "Engine":
+                    device: str = "cuda:0", memory: Optional[MemoryBudget] = None, kv_cache: str = "auto", **kw) -> "Engine":
         """``num_pages`` or ``context`` size the cache directly.  With ``memory`` (a budget from
         :func:`mrun_b200.engine.budget.plan`) the cache is what the budget leaves beside the
-        weights and the step's scratch, or exactly ``context`` tokens if that fits."""
+        weights and the step's scratch, or exactly ``context`` tokens if that fits.  ``kv_cache="fp4"`` holds keys and
+        values in 4 bits (bfloat16, models of grouped-query attention with heads of 64 or 128 features, ``page_size`` a multiple of 16)."""
         sizing = None
         if memory is not None and num_pages is None:
             sizing = _sizing(memory, context, page_size, max_requests, max_batch_tokens)
         pages = _pages_for(num_pages, context, page_size)
         executor = executor_from_folder(model_dir, dtype=dtype, page_size=page_size, num_pages=pages,
-                                        max_requests=max_requests, device=device, sizing=sizing)
+                                        max_requests=max_requests, device=device, sizing=sizing, kv_cache=kv_cache)
         return cls(executor, max_batch_tokens=max_batch_tokens, reserve=reserve, **kw)
 
     @classmethod
@@ -105,14 +106,14 @@ class Engine:
                     norm_noise: float = 0.0, page_size: int = 16, num_pages: Optional[int] = None,
                     context: Optional[int] = None, max_requests: int = 64, max_batch_tokens: int = 2048,
                     reserve: bool = True, device: str = "cuda:0", memory: Optional[MemoryBudget] = None,
-                    **kw) -> "Engine":
+                    kv_cache: str = "auto", **kw) -> "Engine":
         sizing = None
         if memory is not None and num_pages is None:
             sizing = _sizing(memory, context, page_size, max_requests, max_batch_tokens)
         pages = _pages_for(num_pages, context, page_size)
         executor = executor_from_config(config, seed, dtype=dtype, std=std, norm_noise=norm_noise,
                                         page_size=page_size, num_pages=pages, max_requests=max_requests,
-                                        device=device, sizing=sizing)
+                                        device=device, sizing=sizing, kv_cache=kv_cache)
         return cls(executor, max_batch_tokens=max_batch_tokens, reserve=reserve, **kw)
 
     # ------------------------------------------------------------------ generation
@@ -344,6 +345,7 @@ class Engine:
         return {
             "architecture": ex.spec.architecture,
             "dtype": ex.precision.name,
+            "kv_cache": ex.runtime.kv_cache,
             "weights_bytes": ex.model.weight_bytes(),
             "page_size": ex.cache.page_size,
             "num_pages": ex.cache.num_pages,
@@ -387,7 +389,10 @@ def _sizing(memory: MemoryBudget, context: Optional[int], page_size: int, max_re
     def sizing(model):
         spec, precision = model.spec, model.runtime.precision
         element = 2 if precision.act == torch.bfloat16 else 4
-        per_token, per_slot = token_bytes(model.cache_needs(), model.cache_shares(), element)
+        needs = model.cache_needs()
+        held, per_slot = token_bytes(needs, model.cache_shares(), element)
+        back = read_back_bytes(needs)
+        per_token = held + back            # what every token of context takes, held and read back
         scratch = budget.scratch_estimate(spec.hidden_size, model.activation_elements(), spec.vocab_size,
                                           max_batch_tokens, max_requests, element) + model.product_scratch(max_batch_tokens)
         weights = model.weight_bytes()
@@ -398,6 +403,8 @@ def _sizing(memory: MemoryBudget, context: Optional[int], page_size: int, max_re
         else:
             done = budget.with_capacity(memory, weights, scratch, max(1, per_token), most,
                                         per_slot * max_requests)
+        if back:
+            done = replace(done, cache=done.capacity_tokens * held, scratch=done.scratch + done.capacity_tokens * back)
         return max(1, -(-done.capacity_tokens // page_size)), done
     return sizing
 

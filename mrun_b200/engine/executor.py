@@ -44,17 +44,18 @@ class LaunchCounter:
 class Executor:
     def __init__(self, spec: ModelSpec, tensors: Dict[str, torch.Tensor], dtype: str = "bfloat16",
                  page_size: int = 16, num_pages: int = 256, max_requests: int = 8,
-                 device: str = "cuda:0", sizing=None):
+                 device: str = "cuda:0", sizing=None, kv_cache: str = "auto"):
         """``sizing(model) -> (num_pages, memory)`` replaces ``num_pages`` once the weights are
         on the device: the memory budget needs their size and the parts' needs to say how many
-        pages fit; ``memory`` is kept for :meth:`Engine.info`."""
+        pages fit; ``memory`` is kept for :meth:`Engine.info`.  ``kv_cache``: "auto" holds keys and values in
+        the compute dtype, "fp4" in 4 bits (models whose mixers all offer it, in bfloat16)."""
         if not torch.cuda.is_available():
             raise RuntimeError("mrun_b200 runs on a CUDA device only: no GPU is visible and there "
                                "is no CPU path")
         self.device = torch.device(device)
         torch.cuda.set_device(self.device)
         self.precision = Precision.of(dtype)
-        self.runtime = Runtime(self.device, self.precision, page_size)
+        self.runtime = Runtime(self.device, self.precision, page_size, kv_cache)
         self.spec = spec
         self.model = Model(spec, tensors, self.runtime)
         self.memory = None

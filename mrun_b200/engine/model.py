@@ -13,9 +13,11 @@ import torch
 
 from ..config.spec import ModelSpec
 from ..kernels import ops
-from ..parts import ARRANGEMENTS, EMBEDDINGS, NORMS, TRANSFORMS, Runtime
+from ..parts import ARRANGEMENTS, EMBEDDINGS, MIXERS, NORMS, TRANSFORMS, Runtime
 from ..parts.base import local
 from .batch import StepContext
+
+KV_CACHES = ("auto", "fp4")        # what keys and values are held as: the compute dtype, or 4 bits
 
 
 class Model:
@@ -23,6 +25,12 @@ class Model:
         spec.validate()
         if spec.streams < 1 or (spec.streams > 1 and spec.embedding_transform is not None):
             raise ValueError("a model has at least one residual stream; an embedding transform takes one stream")
+        if runtime.kv_cache not in KV_CACHES:
+            raise ValueError(f"kv_cache must be one of {', '.join(KV_CACHES)}, got {runtime.kv_cache!r}")
+        if runtime.kv_cache == "fp4":
+            for i, layer in enumerate(spec.layers):
+                if not getattr(MIXERS.get(layer.mixer.kind), "holds_fp4", False):
+                    raise ValueError(f"layer {i}: the mixer {layer.mixer.kind!r} does not hold its cache in 4 bits")
         self.spec = spec
         self.runtime = runtime
         self.embedding = runtime.matrix(tensors[spec.embedding_name])

@@ -5,6 +5,8 @@ concatenation; the reference keeps three products, crates/mrun-engine/src/models
 per-head RMSNorm of q and k, then rotation, then k and v into the pages
 (crates/mrun-engine/src/models/common.rs:183,194-198); softmax attention of each token over the
 keys of its request up to itself; output projection (crates/mrun-engine/src/models/common.rs:137,206).
+With ``runtime.kv_cache`` "fp4" the keys and values are held in 4 bits (bfloat16 activations, heads of 64 or 128 features, pages
+of a multiple of 16 tokens).
 A projection's ``.bias`` is bound and added when the checkpoint has one
 (crates/mrun-engine/src/load.rs:281,302-305); Qwen3's have none.
 """
@@ -15,13 +17,14 @@ import torch
 from ..cache.needs import PagedKV
 from ..config.spec import AttentionSpec, TensorSpec
 from ..kernels import ops
-from ..kernels.attention import decode_fuses_input, paged_attention, supports_tensor_cores
+from ..kernels.attention import decode_fuses_input, paged_attention, paged_attention_fp4, supports_tensor_cores
 from .base import NORMS, POSITIONS, Runtime, register_mixer
 
 
 @register_mixer("attention")
 class Attention:
     accepts_normed_rows = True      # its first product takes ``ops.NormedRows`` as x
+    holds_fp4 = True                # the cache may be held in 4 bits
     can_defer_output = True         # ``forward(..., defer_output=True)`` may return ``ops.PendingLinear``
 
     @staticmethod
@@ -49,6 +52,11 @@ class Attention:
             raise ValueError(f"heads={spec.heads} is not a multiple of kv_heads={spec.kv_heads}")
         if spec.qk_norm is not None and spec.qk_norm.size != spec.head_dim:
             raise ValueError("the q/k norm works per head: its size must be head_dim")
+        self.fp4 = runtime.kv_cache == "fp4"
+        if self.fp4 and runtime.precision.act != torch.bfloat16:
+            raise ValueError(f"a 4-bit cache takes bfloat16 activations, not {runtime.precision.name}")
+        if self.fp4:
+            ops.fp4_cache_shape(0, spec.kv_heads, runtime.page_size, spec.head_dim)        # refuses what it cannot hold
         self.spec = spec
         self.runtime = runtime
         self.wqkv = runtime.matrix(torch.cat(
@@ -73,10 +81,10 @@ class Attention:
             self.position = POSITIONS.build(spec.position, {}, runtime)
         # the tiled kernel that very wide groups fall to needs a tile list made on the host
         ratio = spec.heads // spec.kv_heads
-        self.graph_safe = not (supports_tensor_cores(runtime.precision.act, spec.head_dim, ratio) and ratio > 16)
+        self.graph_safe = self.fp4 or not (supports_tensor_cores(runtime.precision.act, spec.head_dim, ratio) and ratio > 16)
 
     def cache_need(self):
-        return PagedKV(self.spec.kv_heads, self.spec.head_dim, self.spec.window)
+        return PagedKV(self.spec.kv_heads, self.spec.head_dim, self.spec.window, fp4=self.fp4)
 
     def activation_elements(self) -> int:
         """Elements per token of the temporaries alive at once (q, k, v and the heads' output)."""
@@ -90,7 +98,11 @@ class Attention:
         rotary_dim = self.position.rotary_dim if self.position is not None else 0
         slots = group.slot_mapping if cache.writable else None
         out = qkv.new_empty((x.shape[0], s.heads * s.head_dim))
-        if decode_fuses_input(ctx, x.dtype, s.heads, s.kv_heads, s.head_dim, self.runtime.page_size):
+        if self.fp4:
+            ops.qk_norm_rope_cache_fp4(qkv, s.heads, s.kv_heads, s.head_dim, self.q_weight, self.k_weight, self.eps, rot, rotary_dim,
+                                       slots, cache.packed)
+            paged_attention_fp4(qkv, qkv.shape[1], out, cache.packed, group, ctx, s.heads, s.head_dim, s.softmax_scale, s.window or 0)
+        elif decode_fuses_input(ctx, x.dtype, s.heads, s.kv_heads, s.head_dim, self.runtime.page_size):
             # a pure decode step: the attention kernel norms, rotates and stores q, k, v itself
             paged_attention(qkv, qkv.shape[1], out, cache, group, ctx, s.heads, s.softmax_scale, s.window or 0,
                             raw=(self.q_weight, self.k_weight, self.eps, rot, rotary_dim, slots))

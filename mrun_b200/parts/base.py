@@ -42,6 +42,7 @@ rows fold the residual sum and the norm into the products around them:
 last product unrun, ``kernels.ops.PendingLinear``); ``accepts_pending`` on a norm or arrangement
 (``delta`` may be such a product; a norm may answer with ``kernels.ops.NormedRows``);
 ``accepts_normed_rows`` on a mixer or feed-forward (``x`` may be ``NormedRows``).
+``holds_fp4`` on a mixer: with ``runtime.kv_cache`` "fp4" its cache need is one held in 4 bits.
 ``heads_forward(x, ctx, cache, out, scale)`` and ``w_o`` on a mixer (everything in front of its output
 projection, times ``scale``, into the rows ``out``) let two mixers side by side share one output product.
 """
@@ -73,6 +74,7 @@ class Runtime:
     device: torch.device
     precision: Precision
     page_size: int
+    kv_cache: str = "auto"    # "auto": keys and values in the compute dtype; "fp4": in 4 bits, by the mixers that offer it
 
     def matrix(self, tensor: torch.Tensor) -> torch.Tensor:
         """A checkpoint matrix in the compute dtype on the device."""

@@ -93,3 +93,66 @@ def test_attention_refuses():
     _Step.page_size = 16
     with pytest.raises(KernelError, match="CUDA only"):
         call()
+
+
+def test_the_books_count_what_pages_take():
+    from mrun_b200.cache import CacheManager, PagedKV, token_bytes
+    from mrun_b200.cache.manager import read_back_bytes
+    needs = [PagedKV(8, 128, fp4=True)] * 36
+    assert token_bytes(needs, [None] * 36, 2) == (36 * 8 * 144, 0) == token_bytes(needs, [None] * 36, 4)
+    assert token_bytes([PagedKV(4, 64, fp4=True), None, PagedKV(8, 128)], [None, 0, None], 2)[0] == 4 * 72 + 8 * 128 * 4
+    assert read_back_bytes(needs) == 8 * 128 * 4 and read_back_bytes([PagedKV(8, 128), None]) == 0
+    assert CacheManager(needs, [None] * 36, 16, 10, 2).bytes_per_page() == 0            # the books alone hold no pages
+    with pytest.raises(ValueError, match="one size"):
+        CacheManager([PagedKV(8, 128, value_dim=64, fp4=True)], [None], 16, 10, 2)
+
+
+def test_a_budget_leaves_room_to_read_a_layer_back():
+    from types import SimpleNamespace
+    from mrun_b200.cache import PagedKV
+    from mrun_b200.engine import budget
+    from mrun_b200.engine.engine import _sizing
+    from mrun_b200.engine.model import Model
+    m = Model.__new__(Model)
+    m.spec = SimpleNamespace(hidden_size=256, vocab_size=1000, max_positions=1 << 22)
+    m.runtime = SimpleNamespace(precision=SimpleNamespace(act=torch.bfloat16))
+    m.final_norm, m.embedding, m.head, m.embedder = None, torch.empty(8, 256), torch.empty(8, 256), None
+    m.order, m.blocks = [], []
+    m.cache_needs, m.cache_shares = (lambda: [PagedKV(8, 128, fp4=True)] * 4), (lambda: [None] * 4)
+    memory = budget.plan(budget.DeviceMemory(80 * budget.GIB, 80 * budget.GIB), 4)
+    pages, done = _sizing(memory, None, 16, 4, 512)(m)
+    held, back = 4 * 8 * 144, 4 * 8 * 128
+    fixed = done.scratch - done.capacity_tokens * back
+    assert done.cache == done.capacity_tokens * held and pages == -(-done.capacity_tokens // 16)
+    assert done.budget - held - back < done.weights + done.scratch + done.cache <= done.budget
+    assert fixed == budget.scratch_estimate(256, 0, 1000, 512, 4, 2) + m.product_scratch(512)
+    exactly = _sizing(memory, 5000, 16, 4, 512)(m)[1]
+    assert exactly.capacity_tokens == 5000 and exactly.budget == exactly.weights + exactly.scratch + exactly.cache
+
+
+def _spec(kind):
+    from types import SimpleNamespace
+    return SimpleNamespace(validate=lambda: None, streams=1, embedding_transform=None, layers=[SimpleNamespace(mixer=SimpleNamespace(kind=kind))])
+
+
+def test_models_that_do_not_hold_their_cache_in_4_bits_are_refused():
+    from mrun_b200.engine.model import Model
+    from mrun_b200.parts import Precision, Runtime
+    runtime = lambda kv_cache: Runtime(torch.device("cpu"), Precision.of("bfloat16"), 16, kv_cache)
+    with pytest.raises(ValueError, match="layer 0: the mixer 'latent_attention' does not hold"):
+        Model(_spec("latent_attention"), {}, runtime("fp4"))
+    with pytest.raises(ValueError, match="kv_cache must be one of auto, fp4, got 'fp8'"):
+        Model(_spec("attention"), {}, runtime("fp8"))
+
+
+def test_an_attention_layer_refuses_what_the_format_does_not_hold():
+    from mrun_b200.config.spec import AttentionSpec
+    from mrun_b200.parts import MIXERS, Precision, Runtime
+    spec = lambda dim: AttentionSpec(hidden=32, heads=4, kv_heads=2, head_dim=dim, softmax_scale=1.0, qk_norm=None, position=None)
+    build = lambda dim, page, dtype: MIXERS.build(spec(dim), {}, Runtime(torch.device("cpu"), Precision.of(dtype), page, "fp4"))
+    with pytest.raises(ValueError, match="bfloat16 activations"):
+        build(64, 16, "float32")
+    with pytest.raises(KernelError, match="multiple of 16"):
+        build(64, 8, "bfloat16")
+    with pytest.raises(KernelError, match="64 or 128"):
+        build(96, 16, "bfloat16")
