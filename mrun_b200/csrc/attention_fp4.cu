@@ -4,27 +4,26 @@
 //
 // What bounds it: a key and its value are 2.25 D / 2 bytes of DRAM, a quarter of their bfloat16 size, so the
 // work on them counts.  At 6.5 TB/s a multiprocessor gets a key and value of 128 features every 6 clocks, 42
-// codes a clock.  Turned into halves by cvt.e2m1x2 (two codes an instruction, full rate: 21 words of eight codes
-// a clock and multiprocessor measured; integer codes by mask and subtraction 9.6) and times their scale
-// (exact), they are operands of mma.m16n8k16, whose 16 rows are keys or features and whose 8 columns are the
-// query heads of a kv head:
-//   S^T [16 keys x 8 heads]     = K Q^T      A = the keys as they lie in the page, B = the queries (registers)
-//   O^T [32 features x 8 heads] += V^T P^T   A = the values as they lie in the page: a register holds two
-//                                            neighbouring features of one key, not two keys of one feature.
-// The second product gets its sum over keys all the same: its k index is (key, parity of the feature), and P is
-// given twice, once with zeros in the places of the odd parity (giving the even features) and once
-// with zeros in those of the even one.  That is twice the products (24 for 16 keys, a quarter of the tensor
-// pipe's time at the memory's rate) and no permutation of the values.
+// codes a clock.  cvt.e2m1x2 makes two halves of a byte in one instruction of the integer pipe (two a clock and
+// multiprocessor; integer codes by mask and subtraction take three times as many); times their scale (exact) they are
+// operands of mma.m16n8k16, whose 16 rows are keys or features and whose 8 columns are query heads of a kv head:
+//   S^T [16 keys x 8]     = K Q^T      A = the keys as they lie in the page, B = the queries (registers)
+//   O^T [32 features x 8] += V^T P^T   A = the values as they lie in the page: a register holds two
+//                                      neighbouring features of one key, not two keys of one feature.
+// The second product gets its sum over keys all the same: its k index is (key, parity of the feature), and a column
+// of P has zeros in the places of one parity, so that it gives the features of the other.  A group of up to four query
+// heads has both columns of a head in one product; a wider one takes two products, one a parity, still a fifth of the tensor
+// pipe's time at the memory's rate, and no permutation of the values.
 // P comes out of the first product by rows and goes into the second by columns: one movmatrix for 8 keys.
 // Queries are scaled by a power of two into a half's range (exact for 24 binary digits below the largest);
 // P carries a factor of 32, so that a half keeps its digits down to 2^-19 of the running maximum, which is raised
 // only when a score passes it by 8 (base 2).
 //
-// A block is four warps; each copies its own units (16 keys) with cp.async into a ring of its own, several
-// ahead, across pairs: no barrier but where a pair's pieces meet.  Every warp of a block works on the same
-// (token, kv head, group of heads) pair.  The tiles (4 units) of all pairs lie in one list, cut evenly among the
+// A block is four warps; each copies its own units (two at a time, 32 keys) with cp.async into a ring of its own while it
+// works on the two before, across pairs: no barrier but where a pair's pieces meet.  Every warp of a block works on the same
+// (token, kv head, group of heads) pair.  The tiles (8 units) of all pairs lie in one list, cut evenly among the
 // blocks that the device holds at once; a pair that lies in several blocks leaves its pieces in scratch, and
-// a second kernel adds them in block order.
+// a second kernel, on the device before the first has ended, adds them in block order.
 #include <cuda_fp16.h>
 
 #include "attention_paging.cuh"
@@ -37,10 +36,11 @@ using namespace mrun;
 using bf16 = __nv_bfloat16;
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int RING = 4;                 // units that a warp has under way or in work
-constexpr int UNITS_A_TILE = WARPS;
-constexpr int TILE_KEYS = UNITS_A_TILE * FP4_TOKENS;
-constexpr int MAX_TOKENS = 512;         // tokens of one launch (their prefix lies in shared memory beside the rings of four blocks)
+constexpr int UNITS = 2;                // units that a warp takes at a time
+constexpr int STAGES = 2;
+constexpr int UNITS_A_TILE = WARPS * UNITS;
+constexpr int MAX_TOKENS = 256;         // tokens of one launch (their plan lies in shared memory beside the rings of four blocks)
+constexpr int MERGE_THREADS = 128;
 constexpr float LIFT = 5.f;             // log2 of the factor that P carries
 constexpr float SLACK = 8.f;            // how far a score may pass the running maximum (base 2)
 
@@ -86,6 +86,22 @@ template <int I> __device__ __forceinline__ unsigned scale_twice(unsigned bytes)
     return __byte_perm(bytes, 0u, (I << 12) | (4 << 8) | (I << 4) | 4) >> 1;
 }
 
+// A score less the maximum it is taken against.  The product is rounded as the maximum's was: fused, the difference of a huge
+// score and its own rounding would stand in the exponent.
+__device__ __forceinline__ float against(float product, float scale, float nbase) { return __fadd_rn(__fmul_rn(product, scale), nbase); }
+
+// The weight of a part whose maximum is m beside one of maximum `top`.  A part without keys has m = -inf and l = 0; one whose
+// scores are all NaN has m = -inf and l = NaN, and keeps it.
+__device__ __forceinline__ float weight_of(float m, float l, float top) {
+    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2_fast(m - top);
+}
+
+__device__ __forceinline__ void store_row(bf16* dst, float4 acc, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    __nv_bfloat162 two[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv), __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(two);
+}
+
 // Tiles of a token that sees the keys from the first visible one to its own position.
 __device__ __forceinline__ int tiles_of(int pos, int window) {
     if (pos < 0) return 0;
@@ -124,22 +140,34 @@ __device__ __forceinline__ Piece next_piece(Cursor& at, int left, const int* pre
     }
 }
 
-template <int D, int NT>
-struct Shared {
+// HT: columns of eight that the heads of a pair take; 0: up to four heads, each with both of its columns in one.
+template <int D, int HT>
+struct Shape {
+    static constexpr int HEADS = HT == 0 ? 4 : 8 * HT, NT = HT == 0 ? 1 : HT;
+    static constexpr int MINE = HT == 0 ? 1 : 2 * HT;                            // heads whose scores a lane holds
     static constexpr int ROW = D + 4;                                            // a head's values, maximum, sum
-    static constexpr int RING_BYTES = WARPS * RING * Fp4Unit<D>::BYTES;
-    static constexpr int MERGE_BYTES = WARPS * 8 * NT * ROW * 4;
-    static size_t bytes(int tokens) { return RING_BYTES + MERGE_BYTES + (size_t)(tokens + 1) * 4; }
+    static constexpr int RING_BYTES = WARPS * STAGES * UNITS * Fp4Unit<D>::BYTES;
+    static constexpr int MERGE_BYTES = WARPS * HEADS * ROW * 4;
+    // ... and per token its prefix of tiles, position and block-table row
+    static size_t bytes(int tokens) { return RING_BYTES + MERGE_BYTES + (size_t)(3 * tokens + 1) * 4; }
 };
 
-// Sums tiles_of over the tokens into prefix[0 .. tokens]; all threads of the block, `scratch` of 33 ints.
-__device__ __forceinline__ void make_prefix(int* prefix, const int* __restrict__ positions, int tokens, int window, int* scratch) {
+// Sums tiles_of over the tokens into prefix[0 .. tokens], positions into held[0 .. tokens) and block-table rows into
+// held[tokens .. 2 tokens); all threads of the block.
+__device__ __forceinline__ void make_plan(int* prefix, int* held, const int* __restrict__ positions, const int* __restrict__ token_slot,
+                                          int tokens, int window, int* scratch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int carried = 0;
     if (threadIdx.x == 0) prefix[0] = 0;
     for (int first = 0; first < tokens; first += THREADS) {
         const int t = first + threadIdx.x;
-        int sum = t < tokens ? tiles_of(positions[t], window) : 0;
+        int pos = -1;
+        if (t < tokens) {
+            pos = positions[t];
+            held[t] = pos;
+            held[tokens + t] = token_slot[t];
+        }
+        int sum = tiles_of(pos, window);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int below = __shfl_up_sync(0xffffffffu, sum, o);
@@ -155,7 +183,6 @@ __device__ __forceinline__ void make_prefix(int* prefix, const int* __restrict__
         if (t < tokens) prefix[t + 1] = before + sum;
         __syncthreads();
     }
-    __syncthreads();
 }
 
 // Tiles that a block takes.
@@ -166,35 +193,43 @@ struct Step {
     const int* token_slot;
     const int* positions;
     const int* rows;             // the rows of q and out that the tokens are, or null: the first ones
-    int max_blocks, table_rows, tokens, heads, kv_heads, page_size, window;
+    int max_blocks, table_rows, tokens, heads, kv_heads, page_size, unit_shift, window;     // unit_shift: of the units of a page, or -1
     long pages, q_stride;
     float scale_log2;
+    float* part_o;               // [blocks, 2, HEADS, D]
+    float2* part_ml;             // [blocks, 2, HEADS]: maximum, sum
+    int* plan;                   // [tokens + 1]: the prefix of tiles
 };
 
-template <int D, int NT>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : 3)
-decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsigned char* __restrict__ cache, const Step step,
-                  float* __restrict__ part_o, float2* __restrict__ part_ml) {
+template <int D, int HT>
+__global__ void __launch_bounds__(THREADS, HT == 2 ? 3 : 4)
+decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsigned char* __restrict__ cache, const Step step) {
     using Unit = Fp4Unit<D>;
-    using Sh = Shared<D, NT>;
-    constexpr int HEADS = 8 * NT, WORDS_K = D / 32, WORDS_V = D / 64, TILES_M = D / 32;
+    using Sh = Shape<D, HT>;
+    constexpr int HEADS = Sh::HEADS, NT = Sh::NT, MINE = Sh::MINE, WORDS_K = D / 32, WORDS_V = D / 64, TILES_M = D / 32;
+    constexpr int COLUMNS = HT == 0 ? 1 : 2;           // products that give a 32-feature tile of a column of eight
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int scratch[WARPS];
     float* merge = reinterpret_cast<float*>(smem + Sh::RING_BYTES);              // [WARPS][HEADS][ROW]
     int* prefix = reinterpret_cast<int*>(smem + Sh::RING_BYTES + Sh::MERGE_BYTES);
+    int* held_pos = prefix + step.tokens + 1;
+    const int* held_row = held_pos + step.tokens;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    unsigned char* ring = smem + warp * RING * Unit::BYTES;
+    unsigned char* ring = smem + warp * STAGES * UNITS * Unit::BYTES;
     const int group = step.heads / step.kv_heads, head_groups = (group + HEADS - 1) / HEADS;
-    const int units_a_page = step.page_size / FP4_TOKENS;
+    const int units_a_page = step.page_size / FP4_TOKENS, pairs = step.kv_heads * head_groups;
 
-    make_prefix(prefix, step.positions, step.tokens, step.window, scratch);
+    dependents_may_start();                            // the second kernel's blocks come as these leave, and wait for the last
+    make_plan(prefix, held_pos, step.positions, step.token_slot, step.tokens, step.window, scratch);
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i <= step.tokens; i += THREADS) step.plan[i] = prefix[i];
     // padding rows come out as zeros
     for (int tok = blockIdx.x; tok < step.tokens; tok += gridDim.x)
-        if (step.positions[tok] < 0)
+        if (held_pos[tok] < 0)
             for (int i = threadIdx.x; i < step.heads * D / 2; i += THREADS)
                 reinterpret_cast<unsigned*>(out + (size_t)(step.rows ? step.rows[tok] : tok) * step.heads * D)[i] = 0u;
 
-    const long total = (long)prefix[step.tokens] * step.kv_heads * head_groups;
+    const long total = (long)prefix[step.tokens] * pairs;
     const int per = tiles_a_block(total, gridDim.x);
     const long begin = (long)blockIdx.x * per;
     if (begin >= total) return;
@@ -204,67 +239,80 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
         int low = 0, high = step.tokens - 1;
         while (low < high) {
             const int mid = (low + high) / 2;
-            if ((long)prefix[mid + 1] * step.kv_heads * head_groups <= begin) low = mid + 1;
+            if ((long)prefix[mid + 1] * pairs <= begin) low = mid + 1;
             else high = mid;
         }
         start.tok = low;
-        start.rest = (int)(begin - (long)prefix[low] * step.kv_heads * head_groups);
+        start.rest = (int)(begin - (long)prefix[low] * pairs);
     }
 
-    // ---- the copies: this warp's unit of every tile, RING - 1 ahead of the work
+    // ---- the copies: this warp's units of every tile, one tile ahead of the work.  The pages of a tile's units are asked for
+    // one tile before their copies, so that these do not wait for the block table.
     Cursor ahead = start;
     Piece ap = {};
-    int ap_tile = 0, issued = 0;
-    int a_pos = -1, a_first = 0;                       // of the token whose units are copied
+    int ap_tile = 0, located = 0, issued = 0;
+    int a_last = -1, a_unit = 0;                       // of the token whose units are copied: its last unit, this warp's next ones
     const int* a_table = nullptr;
-    unsigned held = 0;                                 // bit i: the unit in stage i is there
-    auto issue = [&]() {
-        const int s = issued % RING;
-        held &= ~(1u << s);
-        if (issued < count) {
-            if (ap_tile == ap.tiles) {
-                ap = next_piece(ahead, count - issued, prefix, step.kv_heads, head_groups);
-                ap_tile = 0;
-                a_pos = step.positions[ap.tok];
-                a_first = first_visible(a_pos, step.window) / FP4_TOKENS;
-                const int slot = step.token_slot[ap.tok];
-                a_table = slot >= 0 && slot < step.table_rows ? step.block_tables + (size_t)slot * step.max_blocks : nullptr;
-            }
-            const int unit = a_first + (ap.tile0 + ap_tile) * UNITS_A_TILE + warp;
-            const int block = unit / units_a_page;
-            if (unit <= a_pos / FP4_TOKENS && a_table && block < step.max_blocks) {
-                const int page = a_table[block];
-                if (page >= 0 && page < step.pages) {
-                    const unsigned char* src = cache + (((size_t)page * step.kv_heads + ap.kvh) * units_a_page + (unit - block * units_a_page)) * Unit::BYTES;
-                    const unsigned dst = smem_addr(ring + s * Unit::BYTES);
+    int page[UNITS], in_page[UNITS], kvh = 0;          // of the units that were located last
+    unsigned arriving = 0;                             // bit u: unit u of the stage that was filled last is there
+    auto locate = [&]() {
 #pragma unroll
-                    for (int c = 0; c < Unit::BYTES / 512; ++c) cp_async_16(dst + (c * 32 + lane) * 16, src + (c * 32 + lane) * 16);
-                    if (lane < Unit::BYTES % 512 / 16)
-                        cp_async_16(dst + (Unit::BYTES / 512 * 32 + lane) * 16, src + (Unit::BYTES / 512 * 32 + lane) * 16);
-                    held |= 1u << s;
-                }
+        for (int u = 0; u < UNITS; ++u) page[u] = -1;
+        if (located < count) {
+            if (ap_tile == ap.tiles) {
+                ap = next_piece(ahead, count - located, prefix, step.kv_heads, head_groups);
+                ap_tile = 0;
+                const int pos = held_pos[ap.tok], table_row = held_row[ap.tok];
+                a_last = pos / FP4_TOKENS;
+                a_unit = first_visible(pos, step.window) / FP4_TOKENS + ap.tile0 * UNITS_A_TILE + warp * UNITS;
+                a_table = step.block_tables + (size_t)table_row * step.max_blocks;
+                if (table_row < 0 || table_row >= step.table_rows) a_last = -1;
+                kvh = ap.kvh;
             }
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                const int unit = a_unit + u;
+                const int block = step.unit_shift >= 0 ? unit >> step.unit_shift : unit / units_a_page;
+                in_page[u] = unit - block * units_a_page;
+                if (unit <= a_last && block < step.max_blocks) page[u] = __ldg(a_table + block);
+            }
+            a_unit += UNITS_A_TILE;
             ++ap_tile;
+            ++located;
+        }
+    };
+    auto issue = [&]() {                               // copies the units located last and locates the next
+        const unsigned dst = smem_addr(ring + (issued % STAGES) * (UNITS * Unit::BYTES)) + lane * 16;
+        arriving = 0;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            if (page[u] < 0 || page[u] >= step.pages) continue;
+            const unsigned char* src = cache + (((size_t)page[u] * step.kv_heads + kvh) * units_a_page + in_page[u]) * Unit::BYTES + lane * 16;
+#pragma unroll
+            for (int c = 0; c < Unit::BYTES / 512; ++c) cp_async_16(dst + u * Unit::BYTES + c * 512, src + c * 512);
+            if (lane < Unit::BYTES % 512 / 16) cp_async_16(dst + u * Unit::BYTES + Unit::BYTES / 512 * 512, src + Unit::BYTES / 512 * 512);
+            arriving |= 1u << u;
         }
         cp_async_commit();
         ++issued;
+        locate();
     };
-#pragma unroll
-    for (int i = 0; i < RING - 1; ++i) issue();
+    locate();
+    issue();
 
     Cursor at = start;
     for (int done = 0, seg = 0; done < count; ++seg) {
         const Piece p = next_piece(at, count - done, prefix, step.kv_heads, head_groups);
-        const int pos = step.positions[p.tok], lo = first_visible(pos, step.window), first_unit = lo / FP4_TOKENS;
+        const int pos = held_pos[p.tok], lo = first_visible(pos, step.window), first_unit = lo / FP4_TOKENS;
         const size_t row = step.rows ? step.rows[p.tok] : p.tok;
         const int head0 = p.kvh * group + p.hg * HEADS, heads_here = min(HEADS, group - p.hg * HEADS);
 
-        // the queries: lane 4 g + t has features D/4 t .. of head g, as halves with the largest of the head in [128, 256)
+        // the queries: lane 4 g + t has features D/4 t .. of the head of column g, as halves with the largest of the head in [128, 256)
         unsigned qf[NT][D / 16][2];
-        float scale[NT][2];                                // of the scores of heads 2 t and 2 t + 1
+        float scale[MINE];                                 // of the scores of the lane's heads
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int h = nt * 8 + g;
+            const int h = HT == 0 ? g >> 1 : nt * 8 + g;
             const bf16* src = q + row * step.q_stride + (size_t)(head0 + h) * D + t * (D / 4);
             uint4 raw[D / 32];
             float largest = 0.f;
@@ -272,10 +320,10 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             for (int c = 0; c < D / 32; ++c) {
                 raw[c] = make_uint4(0, 0, 0, 0);
                 if (h < heads_here) raw[c] = *reinterpret_cast<const uint4*>(src + c * 8);
-                const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw[c]);
+                const __nv_bfloat162* two = reinterpret_cast<const __nv_bfloat162*>(&raw[c]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float2 f = __bfloat1622float2(pairs[e]);
+                    const float2 f = __bfloat1622float2(two[e]);
                     largest = fmaxf(largest, fmaxf(fabsf(f.x), fabsf(f.y)));
                 }
             }
@@ -287,43 +335,49 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             const float up = __uint_as_float((unsigned)(261 - ex) << 23), down = __uint_as_float((unsigned)(ex - 7) << 23);
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-                const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw[c]);
+                const __nv_bfloat162* two = reinterpret_cast<const __nv_bfloat162*>(&raw[c]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float2 f = __bfloat1622float2(pairs[e]);
+                    const float2 f = __bfloat1622float2(two[e]);
                     qf[nt][c * 2 + (e >> 1)][e & 1] = pack_h2(f.x * up, f.y * up);
                 }
             }
-            scale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t) * step.scale_log2;
-            scale[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4) * step.scale_log2;
+            scale[HT == 0 ? 0 : 2 * nt] = __shfl_sync(0xffffffffu, down, 8 * t) * step.scale_log2;
+            if constexpr (HT != 0) scale[2 * nt + 1] = __shfl_sync(0xffffffffu, down, 8 * t + 4) * step.scale_log2;
         }
 
-        float m[NT][2], l[NT][2], o[NT][TILES_M][2][4];
+        float m[MINE], nbase[MINE], l[MINE], o[NT][TILES_M][COLUMNS][4];     // nbase: LIFT less the maximum
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            m[nt][0] = m[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.f;
+        for (int h = 0; h < MINE; ++h) {
+            m[h] = -INFINITY;
+            nbase[h] = INFINITY;
+            l[h] = 0.f;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < TILES_M; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) o[nt][i][e][0] = o[nt][i][e][1] = o[nt][i][e][2] = o[nt][i][e][3] = 0.f;
-        }
+                for (int e = 0; e < COLUMNS; ++e) o[nt][i][e][0] = o[nt][i][e][1] = o[nt][i][e][2] = o[nt][i][e][3] = 0.f;
 
         for (int tile = p.tile0; tile < p.tile0 + p.tiles; ++tile, ++done) {
             __syncwarp();                                  // the stage that is filled next was read by all lanes
+            const unsigned here = arriving;                // which units of this stage are there
+            const unsigned char* stage = ring + (done % STAGES) * (UNITS * Unit::BYTES);
             issue();
-            const int s = done % RING;
-            cp_async_wait<RING - 1>();
+            cp_async_wait<1>();
             __syncwarp();
-            if (!((held >> s) & 1u)) continue;
-            const unsigned char* unit = ring + s * Unit::BYTES;
-            const int key0 = (first_unit + tile * UNITS_A_TILE + warp) * FP4_TOKENS;
+            if (here == 0) continue;
+            const int key0 = (first_unit + tile * UNITS_A_TILE + warp * UNITS) * FP4_TOKENS;
+            const bool whole = here == (1u << UNITS) - 1 && key0 >= lo && key0 + UNITS * FP4_TOKENS - 1 <= pos;
 
             // ---- scores
-            float c[NT][4];
+            float c[UNITS][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
-            {
+            for (int u = 0; u < UNITS; ++u) {
+                const unsigned char* unit = stage + u * Unit::BYTES;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) c[u][nt][0] = c[u][nt][1] = c[u][nt][2] = c[u][nt][3] = 0.f;
                 unsigned kw[2][WORDS_K];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -354,124 +408,145 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
-                            mma_f16(c[nt], a[0][2 * j], a[1][2 * j], a[0][2 * j + 1], a[1][2 * j + 1], qf[nt][2 * w + j][0], qf[nt][2 * w + j][1]);
+                            mma_f16(c[u][nt], a[0][2 * j], a[1][2 * j], a[0][2 * j + 1], a[1][2 * j + 1], qf[nt][2 * w + j][0], qf[nt][2 * w + j][1]);
                 }
             }
-            const bool whole = key0 >= lo && key0 + FP4_TOKENS - 1 <= pos;
+            // Score of the lane's head h with key g or g + 8 (r) of unit u: c[u][h / 2][h % 2 + 2 r].
+            auto hidden = [&](int u, int r) {
+                const int key = key0 + u * FP4_TOKENS + r * 8 + g;
+                return key > pos || key < lo || !((here >> u) & 1u);
+            };
+            float x[MINE][UNITS][2];                       // score + nbase, what P is the power of
             bool raise = false;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int h = 0; h < MINE; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = c[nt][e] * scale[nt][e & 1];
-                    if (!whole) {
-                        const int key = key0 + g + (e >> 1) * 8;
-                        if (key > pos || key < lo) v = -INFINITY;
-                    }
-                    c[nt][e] = v;
-                    raise = raise || v > m[nt][e & 1] + SLACK;
-                }
-            if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float mx = fmaxf(c[nt][h], c[nt][h + 2]);
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        mx = fmaxf(mx, m[nt][h]);
-                        const float corr = m[nt][h] == -INFINITY ? 0.f : exp2_fast(m[nt][h] - mx);
-                        m[nt][h] = mx;
-                        l[nt][h] *= corr;
-#pragma unroll
-                        for (int i = 0; i < TILES_M; ++i)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                o[nt][i][e][h] *= corr;
-                                o[nt][i][e][h + 2] *= corr;
-                            }
-                    }
-            }
-            unsigned pt[NT][2];                            // lane 4 g + t: keys 2 t and 2 t + 1 (then + 8) of head g
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float base[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) base[h] = m[nt][h] == -INFINITY ? 0.f : m[nt][h] - LIFT;
-                float pr[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) pr[e] = exp2_fast(c[nt][e] - base[e & 1]);
-                l[nt][0] += pr[0] + pr[2];
-                l[nt][1] += pr[1] + pr[3];
-                pt[nt][0] = transposed(pack_h2(pr[0], pr[1]));
-                pt[nt][1] = transposed(pack_h2(pr[2], pr[3]));
-            }
-
-            // ---- values
-            unsigned vs = *reinterpret_cast<const unsigned*>(unit + Unit::V_SCALES + (D == 128 ? lane : (g >> 1) * 4 + t) * 4);
-            if (!whole) {
-                // a key that is not seen may lie in memory that nothing has written: 0 times its value must be 0
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int key = key0 + (b >> 1) * 8 + 2 * t + (b & 1);
-                    if (key > pos || key < lo) vs &= ~(0xFFu << (8 * b));
-                }
-            }
-            const unsigned sv[4] = {scale_twice<0>(vs), scale_twice<1>(vs), scale_twice<2>(vs), scale_twice<3>(vs)};
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                unsigned vw[2][WORDS_V];                   // of tokens 2 t and 2 t + 1 (+ 8 half)
-                const unsigned char* src = unit + Unit::V_CODES + half * (4 * D) + lane * 2 * Unit::PIECE;
-                if constexpr (D == 128) *reinterpret_cast<uint4*>(vw) = *reinterpret_cast<const uint4*>(src);
-                else *reinterpret_cast<uint2*>(vw) = *reinterpret_cast<const uint2*>(src);
-                unsigned be[NT][2], bo[NT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    be[nt][0] = pt[nt][half] & 0xffffu; be[nt][1] = pt[nt][half] >> 16;
-                    bo[nt][0] = pt[nt][half] << 16;     bo[nt][1] = pt[nt][half] & 0xffff0000u;
-                }
-#pragma unroll
-                for (int w = 0; w < WORDS_V; ++w) {
-                    unsigned a[2][4];
+                for (int u = 0; u < UNITS; ++u)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        halves_of(vw[r][w], a[r]);
+                        x[h][u][r] = against(c[u][h >> 1][(h & 1) + 2 * r], scale[h], nbase[h]);
+                        if (!whole && hidden(u, r)) x[h][u][r] = -INFINITY;
+                        raise = raise || x[h][u][r] > LIFT + SLACK;
+                    }
+            if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) a[r][i] = mul_h2(a[r][i], sv[half * 2 + r]);
+                for (int h = 0; h < MINE; ++h) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            if (whole || !hidden(u, r)) mx = fmaxf(mx, __fmul_rn(c[u][h >> 1][(h & 1) + 2 * r], scale[h]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    mx = fmaxf(mx, m[h]);
+                    const float corr = m[h] == -INFINITY ? 0.f : exp2_fast(m[h] - mx);
+                    m[h] = mx;
+                    nbase[h] = LIFT - mx;
+                    l[h] *= corr;
+#pragma unroll
+                    for (int i = 0; i < TILES_M; ++i)
+#pragma unroll
+                        for (int e = 0; e < COLUMNS; ++e)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (HT == 0 || (k & 1) == (h & 1)) o[h >> 1][i][e][k] *= corr;
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            x[h][u][r] = against(c[u][h >> 1][(h & 1) + 2 * r], scale[h], nbase[h]);
+                            if (!whole && hidden(u, r)) x[h][u][r] = -INFINITY;
+                        }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < MINE; ++h)
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        x[h][u][r] = exp2_fast(x[h][u][r]);
+                        l[h] += x[h][u][r];
+                    }
+
+            // ---- values
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                const unsigned char* unit = stage + u * Unit::BYTES;
+                unsigned vs = *reinterpret_cast<const unsigned*>(unit + Unit::V_SCALES + (D == 128 ? lane : (g >> 1) * 4 + t) * 4);
+                if (!whole) {
+                    // a key that is not seen may lie in memory that nothing has written: 0 times its value must be 0
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const int key = key0 + u * FP4_TOKENS + (b >> 1) * 8 + 2 * t + (b & 1);
+                        if (key > pos || key < lo || !((here >> u) & 1u)) vs &= ~(0xFFu << (8 * b));
+                    }
+                }
+                const unsigned sv[4] = {scale_twice<0>(vs), scale_twice<1>(vs), scale_twice<2>(vs), scale_twice<3>(vs)};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    unsigned vw[2][WORDS_V];               // of tokens 2 t and 2 t + 1 (+ 8 half)
+                    const unsigned char* src = unit + Unit::V_CODES + half * (4 * D) + lane * 2 * Unit::PIECE;
+                    if constexpr (D == 128) *reinterpret_cast<uint4*>(vw) = *reinterpret_cast<const uint4*>(src);
+                    else *reinterpret_cast<uint2*>(vw) = *reinterpret_cast<const uint2*>(src);
+                    unsigned b[NT][COLUMNS][2];            // P of tokens 2 t and 2 t + 1 for the head of column g
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float p0 = x[HT == 0 ? 0 : 2 * nt][u][half], p1 = x[HT == 0 ? 0 : 2 * nt + 1][u][half];
+                        const unsigned pt = transposed(pack_h2(p0, p1));
+                        if constexpr (HT == 0) {           // column g is of head g / 2 and of the features of parity g % 2
+                            b[nt][0][0] = __byte_perm(pt, 0u, g & 1 ? 0x1044u : 0x4410u);
+                            b[nt][0][1] = __byte_perm(pt, 0u, g & 1 ? 0x3244u : 0x4432u);
+                        } else {
+                            b[nt][0][0] = pt & 0xffffu; b[nt][0][1] = pt >> 16;
+                            b[nt][COLUMNS - 1][0] = pt << 16; b[nt][COLUMNS - 1][1] = pt & 0xffff0000u;
+                        }
                     }
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int w = 0; w < WORDS_V; ++w) {
+                        unsigned a[2][4];
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma_f16(o[nt][2 * w + j][0], a[0][2 * j], a[0][2 * j + 1], a[1][2 * j], a[1][2 * j + 1], be[nt][0], be[nt][1]);
-                            mma_f16(o[nt][2 * w + j][1], a[0][2 * j], a[0][2 * j + 1], a[1][2 * j], a[1][2 * j + 1], bo[nt][0], bo[nt][1]);
+                        for (int r = 0; r < 2; ++r) {
+                            halves_of(vw[r][w], a[r]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) a[r][i] = mul_h2(a[r][i], sv[half * 2 + r]);
                         }
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < COLUMNS; ++e)
+                                    mma_f16(o[nt][2 * w + j][e], a[0][2 * j], a[0][2 * j + 1], a[1][2 * j], a[1][2 * j + 1], b[nt][e][0], b[nt][e][1]);
+                    }
                 }
             }
         }
 
         // ---- the four warps' results meet
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int h = 0; h < MINE; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+            const int head = HT == 0 ? t : (h >> 1) * 8 + 2 * t + (h & 1);
+            float* dst = merge + (warp * HEADS + head) * Sh::ROW;
+            if (head < heads_here) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], 4);
-                l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], 8);
-                l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], 16);
-                const int head = nt * 8 + 2 * t + h;
-                float* dst = merge + (warp * HEADS + head) * Sh::ROW;
-                if (head < heads_here) {
-#pragma unroll
-                    for (int i = 0; i < TILES_M; ++i)      // features D/8 g + 4 i ..
-                        *reinterpret_cast<float4*>(dst + g * (D / 8) + 4 * i) =
-                            make_float4(o[nt][i][0][h], o[nt][i][1][h], o[nt][i][0][h + 2], o[nt][i][1][h + 2]);
-                    if (g == 0) {
-                        dst[D] = m[nt][h];
-                        dst[D + 1] = l[nt][h];
-                    }
+                for (int i = 0; i < TILES_M; ++i) {        // features D/8 g + 4 i ..
+                    const float (&oo)[COLUMNS][4] = o[h >> 1][i];
+                    *reinterpret_cast<float4*>(dst + g * (D / 8) + 4 * i) =
+                        HT == 0 ? make_float4(oo[0][0], oo[0][1], oo[0][2], oo[0][3])
+                                : make_float4(oo[0][h & 1], oo[COLUMNS - 1][h & 1], oo[0][(h & 1) + 2], oo[COLUMNS - 1][(h & 1) + 2]);
+                }
+                if (g == 0) {
+                    dst[D] = m[h];
+                    dst[D + 1] = l[h];
                 }
             }
+        }
         __syncthreads();
         const size_t my = (size_t)blockIdx.x * 2 + (seg == 0 ? 0 : 1);
         for (int i = threadIdx.x; i < heads_here * (D / 4); i += THREADS) {
@@ -484,18 +559,16 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 const float* src = merge + (w * HEADS + head) * Sh::ROW;
-                const float f = src[D] == -INFINITY ? (src[D + 1] == 0.f ? 0.f : 1.f) : exp2f(src[D] - mm);
+                const float f = weight_of(src[D], src[D + 1], mm);
                 const float4 v = *reinterpret_cast<const float4*>(src + d);
                 acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
                 ll += src[D + 1] * f;
             }
             if (p.complete) {
-                const float inv = ll == 0.f ? 0.f : 1.f / ll;
-                __nv_bfloat162 pair[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv), __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
-                *reinterpret_cast<uint2*>(out + row * step.heads * D + (size_t)(head0 + head) * D + d) = *reinterpret_cast<uint2*>(pair);
+                store_row(out + row * step.heads * D + (size_t)(head0 + head) * D + d, acc, ll);
             } else {
-                *reinterpret_cast<float4*>(part_o + (my * HEADS + head) * D + d) = acc;
-                if (d == 0) part_ml[my * HEADS + head] = make_float2(mm, ll);
+                *reinterpret_cast<float4*>(step.part_o + (my * HEADS + head) * D + d) = acc;
+                if (d == 0) step.part_ml[my * HEADS + head] = make_float2(mm, ll);
             }
         }
         __syncthreads();
@@ -503,94 +576,137 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     cp_async_wait<0>();
 }
 
-// Adds the pieces of the pairs that lie in several blocks, in block order.  A block takes a pair.
-template <int D, int NT>
-__global__ void __launch_bounds__(THREADS)
-merge_fp4_kernel(bf16* __restrict__ out, const Step step, const float* __restrict__ part_o, const float2* __restrict__ part_ml, int blocks) {
-    constexpr int HEADS = 8 * NT;
-    __shared__ int scratch[WARPS];
-    extern __shared__ int prefix[];
+// Adds the pieces of the pairs that lie in several blocks: grid (tokens * pairs, heads of a pair), a block a head.  A slice of
+// the threads takes every SLICES-th piece, four values a thread; then the slices are added in their order.
+template <int D, int HT>
+__global__ void __launch_bounds__(MERGE_THREADS)
+merge_fp4_kernel(bf16* __restrict__ out, const Step step, int blocks) {
+    constexpr int HEADS = Shape<D, HT>::HEADS, LANES = D / 4, SLICES = MERGE_THREADS / LANES;
+    __shared__ float4 sums[SLICES][LANES];
+    __shared__ float2 tops[SLICES];
+    const int group = step.heads / step.kv_heads, head_groups = (group + HEADS - 1) / HEADS, pairs = step.kv_heads * head_groups;
+    const int tok = blockIdx.x / pairs, pair = blockIdx.x - tok * pairs, kvh = pair / head_groups, hg = pair - kvh * head_groups;
+    const int head = blockIdx.y;
+    if (head >= group - hg * HEADS) return;
     wait_for_kernel_before();
-    make_prefix(prefix, step.positions, step.tokens, step.window, scratch);
-    const int group = step.heads / step.kv_heads, head_groups = (group + HEADS - 1) / HEADS;
-    const int pairs = step.kv_heads * head_groups;
-    const int tok = blockIdx.x / pairs, pair = blockIdx.x - tok * pairs;
-    const long total = (long)prefix[step.tokens] * pairs;
-    const int per = tiles_a_block(total, blocks), tiles = prefix[tok + 1] - prefix[tok];
+    const int before = __ldcg(step.plan + tok), tiles = __ldcg(step.plan + tok + 1) - before;
+    const long total = (long)__ldcg(step.plan + step.tokens) * pairs;
     if (tiles == 0) return;
-    const long start = (long)prefix[tok] * pairs + (long)pair * tiles;
+    const int per = tiles_a_block(total, blocks);
+    const long start = (long)before * pairs + (long)pair * tiles;
     const int first = (int)(start / per), last = (int)((start + tiles - 1) / per);
     if (first == last) return;
-    const int kvh = pair / head_groups, hg = pair - kvh * head_groups;
-    const int heads_here = min(HEADS, group - hg * HEADS);
-    const size_t row = step.rows ? step.rows[tok] : tok;
     // a block's piece of this pair is its first one where its range begins inside the pair
-    auto slot = [&](int b) { return (size_t)b * 2 + ((long)b * per >= start ? 0 : 1); };
-    for (int i = threadIdx.x; i < heads_here * (D / 4); i += THREADS) {
-        const int head = i / (D / 4), d = (i - head * (D / 4)) * 4;
-        float mm = -INFINITY;
-        for (int b = first; b <= last; ++b) mm = fmaxf(mm, part_ml[slot(b) * HEADS + head].x);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float ll = 0.f;
-        for (int b = first; b <= last; ++b) {
-            const float2 ml = part_ml[slot(b) * HEADS + head];
-            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - mm);
-            const float4 v = *reinterpret_cast<const float4*>(part_o + (slot(b) * HEADS + head) * D + d);
-            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-            ll += ml.y * f;
+    auto slot = [&](int b) { return ((size_t)b * 2 + ((long)b * per >= start ? 0 : 1)) * HEADS + head; };
+    const int slice = threadIdx.x / LANES, d = threadIdx.x % LANES;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int b0 = first + slice; b0 <= last; b0 += 4 * SLICES) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {                      // all asked for before any is used
+            ml[k] = make_float2(-INFINITY, 0.f);
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int b = b0 + k * SLICES;
+            if (b <= last) {
+                ml[k] = __ldcg(step.part_ml + slot(b));
+                v[k] = __ldcg(reinterpret_cast<const float4*>(step.part_o + slot(b) * D) + d);
+            }
         }
-        const float inv = ll == 0.f ? 0.f : 1.f / ll;
-        __nv_bfloat162 two[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv), __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
-        *reinterpret_cast<uint2*>(out + row * step.heads * D + (size_t)(kvh * group + hg * HEADS + head) * D + d) = *reinterpret_cast<uint2*>(two);
+        float mm = m;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mm = fmaxf(mm, ml[k].x);
+        const float old = weight_of(m, l, mm);
+        acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+        l *= old;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float f = weight_of(ml[k].x, ml[k].y, mm);
+            acc.x += v[k].x * f; acc.y += v[k].y * f; acc.z += v[k].z * f; acc.w += v[k].w * f;
+            l += ml[k].y * f;
+        }
+        m = mm;
     }
+    sums[slice][d] = acc;
+    if (d == 0) tops[slice] = make_float2(m, l);
+    __syncthreads();
+    if (slice) return;
+    float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int i = 0; i < SLICES; ++i) mm = fmaxf(mm, tops[i].x);
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < SLICES; ++i) {
+        const float f = weight_of(tops[i].x, tops[i].y, mm);
+        const float4 v = sums[i][d];
+        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+        ll += tops[i].y * f;
+    }
+    const size_t row = step.rows ? step.rows[tok] : tok;
+    store_row(out + row * step.heads * D + (size_t)(kvh * group + hg * HEADS + head) * D + d * 4, acc, ll);
 }
 
-template <int D, int NT>
-cudaError_t launch_decode(const bf16* q, bf16* out, const unsigned char* cache, const Step& step, float* part_o, float* part_ml, int blocks,
-                          cudaStream_t stream) {
-    const size_t smem = Shared<D, NT>::bytes(step.tokens);
-    cudaError_t err = cudaFuncSetAttribute(decode_fp4_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shared<D, NT>::bytes(MAX_TOKENS));
+template <int D, int HT>
+cudaError_t launch_decode(const bf16* q, bf16* out, const unsigned char* cache, const Step& step, int blocks, cudaStream_t stream) {
+    using Sh = Shape<D, HT>;
+    cudaError_t err = cudaFuncSetAttribute(decode_fp4_kernel<D, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::bytes(MAX_TOKENS));
     if (err != cudaSuccess) return err;
-    err = launch_kernel(decode_fp4_kernel<D, NT>, dim3(blocks), dim3(THREADS), smem, stream, q, out, cache, step, part_o, (float2*)part_ml);
+    err = launch_kernel(decode_fp4_kernel<D, HT>, dim3(blocks), dim3(THREADS), Sh::bytes(step.tokens), stream, q, out, cache, step);
     if (err != cudaSuccess) return err;
-    const int group = step.heads / step.kv_heads, head_groups = (group + 8 * NT - 1) / (8 * NT);
-    return launch_kernel_overlapped(merge_fp4_kernel<D, NT>, dim3(step.tokens * step.kv_heads * head_groups), dim3(THREADS),
-                                    (size_t)(step.tokens + 1) * 4, stream, out, step, part_o, (const float2*)part_ml, blocks);
+    const int group = step.heads / step.kv_heads, head_groups = (group + Sh::HEADS - 1) / Sh::HEADS;
+    return launch_kernel_overlapped(merge_fp4_kernel<D, HT>, dim3(step.tokens * step.kv_heads * head_groups, group < Sh::HEADS ? group : Sh::HEADS),
+                                    dim3(MERGE_THREADS), 0, stream, out, step, blocks);
 }
 
-template <int D, int NT> int occupancy() {
+template <int D, int HT> int occupancy() {
     int n = 0;
-    cudaFuncSetAttribute(decode_fp4_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shared<D, NT>::bytes(MAX_TOKENS));
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_fp4_kernel<D, NT>, THREADS, Shared<D, NT>::bytes(MAX_TOKENS)) != cudaSuccess) return 0;
+    const size_t smem = Shape<D, HT>::bytes(MAX_TOKENS);
+    if (cudaFuncSetAttribute(decode_fp4_kernel<D, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_fp4_kernel<D, HT>, THREADS, smem) != cudaSuccess) return 0;
     return n;
 }
+
+// Heads that a block takes of a kv head's group.
+int heads_a_block(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
 
 }  // namespace
 
 // Blocks of the decode kernel that a multiprocessor holds at once; 0: the device refuses.
 MRUN_API int mrun_attn_fp4_occupancy(int head_dim, int group) {
-    return head_dim == 64 ? (group <= 8 ? occupancy<64, 1>() : occupancy<64, 2>()) : (group <= 8 ? occupancy<128, 1>() : occupancy<128, 2>());
+    const int heads = heads_a_block(group);
+    return head_dim == 64 ? (heads == 4 ? occupancy<64, 0>() : heads == 8 ? occupancy<64, 1>() : occupancy<64, 2>())
+                          : (heads == 4 ? occupancy<128, 0>() : heads == 8 ? occupancy<128, 1>() : occupancy<128, 2>());
 }
 
-// part_o: float [blocks, 2, heads a block, head_dim]; part_ml: float [blocks, 2, heads a block, 2].
+// Bytes of scratch that a launch of `blocks` blocks over `tokens` tokens takes.
+MRUN_API int mrun_attn_fp4_scratch(int blocks, int tokens, int head_dim, int group) {
+    return blocks * 2 * heads_a_block(group) * (head_dim * 4 + 8) + (tokens + 1) * 4;
+}
+
+// One token a row: `tokens` rows of q and out, or those that `rows` names.  scratch: see mrun_attn_fp4_scratch, on 16 bytes.
 MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const void* cache, const int* block_tables, int table_rows,
                                   int max_blocks, const int* token_slot, const int* positions, const int* rows, int tokens, int heads,
-                                  int kv_heads, int head_dim, int page_size, long pages, float scale, int window, float* part_o,
-                                  float* part_ml, int blocks, cudaStream_t stream) {
+                                  int kv_heads, int head_dim, int page_size, long pages, float scale, int window, void* scratch,
+                                  int blocks, cudaStream_t stream) {
     const char* name = "paged_attention_fp4";
     MRUN_REQUIRE(tokens >= 0 && tokens <= MAX_TOKENS, "%s: %d tokens, a launch takes up to %d", name, tokens, MAX_TOKENS);
     MRUN_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && blocks > 0 && pages >= 0 && max_blocks >= 0 && table_rows >= 0,
                  "%s: bad sizes", name);
     MRUN_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim=%d: the 4-bit cache takes heads of 64 or 128 features", name, head_dim);
     MRUN_REQUIRE(page_size > 0 && page_size % FP4_TOKENS == 0, "%s: page_size=%d is not a multiple of 16", name, page_size);
-    MRUN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)part_o) & 15) == 0 && q_stride % 8 == 0,
+    MRUN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)scratch) & 15) == 0 && q_stride % 8 == 0,
                  "%s: rows and pages start on 16 bytes", name);
     if (tokens == 0) return 0;
-    Step step = {block_tables, token_slot, positions, rows, max_blocks, table_rows, tokens, heads, kv_heads, page_size, window,
-                 pages, q_stride, scale * 1.4426950408889634f};
-    auto launch = head_dim == 64 ? (heads / kv_heads <= 8 ? launch_decode<64, 1> : launch_decode<64, 2>)
-                                 : (heads / kv_heads <= 8 ? launch_decode<128, 1> : launch_decode<128, 2>);
-    MRUN_CHECK_CUDA(launch((const bf16*)q, (bf16*)out, (const unsigned char*)cache, step, part_o, part_ml, blocks, stream), name);
+    const int block_heads = heads_a_block(heads / kv_heads);
+    float* part_o = (float*)scratch;
+    float2* part_ml = (float2*)(part_o + (size_t)blocks * 2 * block_heads * head_dim);
+    const Step step = {block_tables, token_slot, positions, rows, max_blocks, table_rows, tokens, heads, kv_heads, page_size,
+                       page_shift_of(page_size / FP4_TOKENS), window, pages, q_stride, scale * 1.4426950408889634f, part_o, part_ml,
+                       (int*)(part_ml + (size_t)blocks * 2 * block_heads)};
+    auto launch = head_dim == 64 ? (block_heads == 4 ? launch_decode<64, 0> : block_heads == 8 ? launch_decode<64, 1> : launch_decode<64, 2>)
+                                 : (block_heads == 4 ? launch_decode<128, 0> : block_heads == 8 ? launch_decode<128, 1> : launch_decode<128, 2>);
+    MRUN_CHECK_CUDA(launch((const bf16*)q, (bf16*)out, (const unsigned char*)cache, step, blocks, stream), name);
     MRUN_CHECK_LAUNCH(name);
     return 0;
 }

@@ -506,7 +506,7 @@ class _View:
 
 def _fp4_blocks(library, device: torch.device, head_dim: int, ratio: int) -> tuple:
     """(blocks of the decode kernel that the device holds, heads that a block takes)."""
-    rows = 8 if ratio <= 8 else 16
+    rows = 4 if ratio <= 4 else 8 if ratio <= 8 else 16
     found = _fp4_slots.get((device, head_dim, rows))
     if found is None:
         per_sm = library.function("mrun_attn_fp4_occupancy")(head_dim, ratio)
@@ -516,7 +516,8 @@ def _fp4_blocks(library, device: torch.device, head_dim: int, ratio: int) -> tup
     return found, rows
 
 
-FP4_MAX_TOKENS = 512       # tokens of one launch of the decode kernel
+FP4_MAX_TOKENS = 256       # tokens of one launch of the decode kernel
+FP4_TILE_KEYS = 128        # keys that its blocks are dealt together
 
 
 def _fp4_tokens(q, q_stride: int, out, cache, group, heads: int, head_dim: int, scale: float, window: int, token_slot, positions,
@@ -526,20 +527,20 @@ def _fp4_tokens(q, q_stride: int, out, cache, group, heads: int, head_dim: int, 
     ratio = heads // kv_heads
     library = _lib.fp4()
     slots, block_heads = _fp4_blocks(library, q.device, head_dim, ratio)
-    pairs_a_token = kv_heads * -(-ratio // block_heads)
+    longest = max_kv_len if window == 0 else min(max_kv_len, abs(window))
+    # no more blocks than tiles (a window that does not begin with a tile's first key touches one more)
+    tiles_a_token = kv_heads * -(-ratio // block_heads) * (-(-longest // FP4_TILE_KEYS) + (window != 0))
+    scratch_bytes = library.function("mrun_attn_fp4_scratch")
     for first in range(0, tokens, FP4_MAX_TOKENS):
         n = min(FP4_MAX_TOKENS, tokens - first)
-        # no more blocks than tiles of 64 keys (an unaligned window touches one more)
-        most = n * pairs_a_token * (-(-min(max_kv_len, window if window > 0 else max_kv_len) // 64) + 1)
-        blocks = max(1, min(slots, most))
-        part_o = torch.empty((blocks, 2, block_heads, head_dim), dtype=torch.float32, device=q.device)
-        part_ml = torch.empty((blocks, 2, block_heads, 2), dtype=torch.float32, device=q.device)
+        blocks = max(1, min(slots, n * tiles_a_token))
+        scratch = torch.empty(scratch_bytes(blocks, n, head_dim, ratio), dtype=torch.uint8, device=q.device)
         here = slice(first, first + n)
         library.call("mrun_attn_fp4_decode", _address(q if rows is not None else q[here]), q_stride,
                      _address(out if rows is not None else out[here]), _address(cache), _address(group.block_tables),
                      group.block_tables.shape[0], group.block_tables.shape[1], _address(token_slot[here]), _address(positions[here]),
                      _address(rows[here] if rows is not None else None), n, heads, kv_heads, head_dim, units * ops.FP4_TOKENS, pages,
-                     scale, window, _address(part_o), _address(part_ml), blocks, _queue())
+                     scale, window, _address(scratch), blocks, _queue())
 
 
 def _fp4_portions(ctx, window: int, short: int):
