@@ -24,6 +24,7 @@
 // (token, kv head, group of heads) pair.  The tiles (8 units) of all pairs lie in one list, cut evenly among the
 // blocks that the device holds at once; a pair that lies in several blocks leaves its pieces in scratch, and
 // a second kernel, on the device before the first has ended, adds them in block order.
+#include <cfloat>
 #include <cuda_fp16.h>
 
 #include "attention_paging.cuh"
@@ -45,8 +46,9 @@ constexpr float LIFT = 5.f;             // log2 of the factor that P carries
 constexpr float SLACK = 8.f;            // how far a score may pass the running maximum (base 2)
 
 __device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp_async_16(unsigned dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+// 16 bytes, or with bytes = 0 zeros, the source not read
+__device__ __forceinline__ void cp_async_16(unsigned dst, const void* src, unsigned bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
@@ -194,7 +196,9 @@ struct Step {
     const int* positions;
     const int* rows;             // the rows of q and out that the tokens are, or null: the first ones
     int max_blocks, table_rows, tokens, heads, kv_heads, page_size, unit_shift, window;     // unit_shift: of the units of a page, or -1
-    long pages, q_stride;
+    int pages;
+    unsigned page_bytes;         // of all kv heads
+    long q_stride;
     float scale_log2;
     float* part_o;               // [blocks, 2, HEADS, D]
     float2* part_ml;             // [blocks, 2, HEADS]: maximum, sum
@@ -253,7 +257,8 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     int ap_tile = 0, located = 0, issued = 0;
     int a_last = -1, a_unit = 0;                       // of the token whose units are copied: its last unit, this warp's next ones
     const int* a_table = nullptr;
-    int page[UNITS], in_page[UNITS], kvh = 0;          // of the units that were located last
+    const unsigned char* a_head = cache;               // the kv head's part of page 0
+    int page[UNITS], in_page[UNITS];                   // of the units that were located last
     unsigned arriving = 0;                             // bit u: unit u of the stage that was filled last is there
     auto locate = [&]() {
 #pragma unroll
@@ -263,35 +268,36 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                 ap = next_piece(ahead, count - located, prefix, step.kv_heads, head_groups);
                 ap_tile = 0;
                 const int pos = held_pos[ap.tok], table_row = held_row[ap.tok];
-                a_last = pos / FP4_TOKENS;
+                a_last = min(pos / FP4_TOKENS, step.max_blocks * units_a_page - 1);
                 a_unit = first_visible(pos, step.window) / FP4_TOKENS + ap.tile0 * UNITS_A_TILE + warp * UNITS;
                 a_table = step.block_tables + (size_t)table_row * step.max_blocks;
                 if (table_row < 0 || table_row >= step.table_rows) a_last = -1;
-                kvh = ap.kvh;
+                a_head = cache + (size_t)ap.kvh * units_a_page * Unit::BYTES + lane * 16;
             }
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) {
                 const int unit = a_unit + u;
                 const int block = step.unit_shift >= 0 ? unit >> step.unit_shift : unit / units_a_page;
-                in_page[u] = unit - block * units_a_page;
-                if (unit <= a_last && block < step.max_blocks) page[u] = __ldg(a_table + block);
+                in_page[u] = (unit - block * units_a_page) * Unit::BYTES;
+                if (unit <= a_last) page[u] = __ldg(a_table + block);
             }
             a_unit += UNITS_A_TILE;
             ++ap_tile;
             ++located;
         }
     };
-    auto issue = [&]() {                               // copies the units located last and locates the next
+    auto issue = [&]() {                               // copies the units located last (one that is not there as zeros) and locates the next
         const unsigned dst = smem_addr(ring + (issued % STAGES) * (UNITS * Unit::BYTES)) + lane * 16;
         arriving = 0;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            if (page[u] < 0 || page[u] >= step.pages) continue;
-            const unsigned char* src = cache + (((size_t)page[u] * step.kv_heads + kvh) * units_a_page + in_page[u]) * Unit::BYTES + lane * 16;
+            const bool there = (unsigned)page[u] < (unsigned)step.pages;
+            const unsigned char* src = there ? a_head + (size_t)page[u] * step.page_bytes + in_page[u] : cache;
+            const unsigned bytes = there ? 16u : 0u;
 #pragma unroll
-            for (int c = 0; c < Unit::BYTES / 512; ++c) cp_async_16(dst + u * Unit::BYTES + c * 512, src + c * 512);
-            if (lane < Unit::BYTES % 512 / 16) cp_async_16(dst + u * Unit::BYTES + Unit::BYTES / 512 * 512, src + Unit::BYTES / 512 * 512);
-            arriving |= 1u << u;
+            for (int c = 0; c < Unit::BYTES / 512; ++c) cp_async_16(dst + u * Unit::BYTES + c * 512, src + c * 512, bytes);
+            if (lane < Unit::BYTES % 512 / 16) cp_async_16(dst + u * Unit::BYTES + Unit::BYTES / 512 * 512, src + Unit::BYTES / 512 * 512, bytes);
+            arriving |= (there ? 1u : 0u) << u;
         }
         cp_async_commit();
         ++issued;
@@ -342,15 +348,16 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                     qf[nt][c * 2 + (e >> 1)][e & 1] = pack_h2(f.x * up, f.y * up);
                 }
             }
-            scale[HT == 0 ? 0 : 2 * nt] = __shfl_sync(0xffffffffu, down, 8 * t) * step.scale_log2;
-            if constexpr (HT != 0) scale[2 * nt + 1] = __shfl_sync(0xffffffffu, down, 8 * t + 4) * step.scale_log2;
+            // never 0, which would make NaN of a hidden key's score (a head that small has scores of 0 either way)
+            scale[HT == 0 ? 0 : 2 * nt] = fmaxf(__shfl_sync(0xffffffffu, down, 8 * t) * step.scale_log2, FLT_MIN);
+            if constexpr (HT != 0) scale[2 * nt + 1] = fmaxf(__shfl_sync(0xffffffffu, down, 8 * t + 4) * step.scale_log2, FLT_MIN);
         }
 
         float m[MINE], nbase[MINE], l[MINE], o[NT][TILES_M][COLUMNS][4];     // nbase: LIFT less the maximum
 #pragma unroll
         for (int h = 0; h < MINE; ++h) {
             m[h] = -INFINITY;
-            nbase[h] = INFINITY;
+            nbase[h] = 1e38f;                              // any score raises it; one of -inf stays -inf
             l[h] = 0.f;
         }
 #pragma unroll
@@ -412,10 +419,27 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                 }
             }
             // Score of the lane's head h with key g or g + 8 (r) of unit u: c[u][h / 2][h % 2 + 2 r].
-            auto hidden = [&](int u, int r) {
-                const int key = key0 + u * FP4_TOKENS + r * 8 + g;
-                return key > pos || key < lo || !((here >> u) & 1u);
-            };
+            unsigned seen[UNITS];                          // of the value scales, which a lane holds of keys 2 t, 2 t + 1, 2 t + 8 and 2 t + 9
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) seen[u] = 0xffffffffu;
+            if (!whole) {
+                // A key that is not seen may lie in memory that nothing has written: its score is -inf, and its value's scale 0.
+                auto hidden = [&](int u, int r) {
+                    const int key = key0 + u * FP4_TOKENS + r;
+                    return key > pos || key < lo || !((here >> u) & 1u);
+                };
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (hidden(u, g + (e >> 1) * 8)) c[u][nt][e] = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        if (hidden(u, (b >> 1) * 8 + 2 * t + (b & 1))) seen[u] &= ~(0xFFu << (8 * b));
+                }
+            }
             float x[MINE][UNITS][2];                       // score + nbase, what P is the power of
             bool raise = false;
 #pragma unroll
@@ -425,7 +449,6 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         x[h][u][r] = against(c[u][h >> 1][(h & 1) + 2 * r], scale[h], nbase[h]);
-                        if (!whole && hidden(u, r)) x[h][u][r] = -INFINITY;
                         raise = raise || x[h][u][r] > LIFT + SLACK;
                     }
             if (__any_sync(0xffffffffu, raise)) {
@@ -436,14 +459,14 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                     for (int u = 0; u < UNITS; ++u)
 #pragma unroll
                         for (int r = 0; r < 2; ++r)
-                            if (whole || !hidden(u, r)) mx = fmaxf(mx, __fmul_rn(c[u][h >> 1][(h & 1) + 2 * r], scale[h]));
+                            mx = fmaxf(mx, __fmul_rn(c[u][h >> 1][(h & 1) + 2 * r], scale[h]));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     mx = fmaxf(mx, m[h]);
                     const float corr = m[h] == -INFINITY ? 0.f : exp2_fast(m[h] - mx);
                     m[h] = mx;
-                    nbase[h] = LIFT - mx;
+                    if (mx > -INFINITY) nbase[h] = LIFT - mx;
                     l[h] *= corr;
 #pragma unroll
                     for (int i = 0; i < TILES_M; ++i)
@@ -455,10 +478,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
                     for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            x[h][u][r] = against(c[u][h >> 1][(h & 1) + 2 * r], scale[h], nbase[h]);
-                            if (!whole && hidden(u, r)) x[h][u][r] = -INFINITY;
-                        }
+                        for (int r = 0; r < 2; ++r) x[h][u][r] = against(c[u][h >> 1][(h & 1) + 2 * r], scale[h], nbase[h]);
                 }
             }
 #pragma unroll
@@ -476,14 +496,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             for (int u = 0; u < UNITS; ++u) {
                 const unsigned char* unit = stage + u * Unit::BYTES;
                 unsigned vs = *reinterpret_cast<const unsigned*>(unit + Unit::V_SCALES + (D == 128 ? lane : (g >> 1) * 4 + t) * 4);
-                if (!whole) {
-                    // a key that is not seen may lie in memory that nothing has written: 0 times its value must be 0
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const int key = key0 + u * FP4_TOKENS + (b >> 1) * 8 + 2 * t + (b & 1);
-                        if (key > pos || key < lo || !((here >> u) & 1u)) vs &= ~(0xFFu << (8 * b));
-                    }
-                }
+                vs &= seen[u];
                 const unsigned sv[4] = {scale_twice<0>(vs), scale_twice<1>(vs), scale_twice<2>(vs), scale_twice<3>(vs)};
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -697,12 +710,16 @@ MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const
     MRUN_REQUIRE(page_size > 0 && page_size % FP4_TOKENS == 0, "%s: page_size=%d is not a multiple of 16", name, page_size);
     MRUN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)scratch) & 15) == 0 && q_stride % 8 == 0,
                  "%s: rows and pages start on 16 bytes", name);
+    MRUN_REQUIRE(pages < (1L << 31) && (long)page_size / FP4_TOKENS * kv_heads * 18 * head_dim < (1L << 31) && (long)max_blocks * (page_size / FP4_TOKENS) < (1L << 31),
+                 "%s: pages=%ld of %d tokens and %d kv heads", name, pages, page_size, kv_heads);
+    MRUN_REQUIRE(scale > 0.f && scale < FLT_MAX, "%s: scale=%g is not a positive number", name, (double)scale);
     if (tokens == 0) return 0;
     const int block_heads = heads_a_block(heads / kv_heads);
     float* part_o = (float*)scratch;
     float2* part_ml = (float2*)(part_o + (size_t)blocks * 2 * block_heads * head_dim);
     const Step step = {block_tables, token_slot, positions, rows, max_blocks, table_rows, tokens, heads, kv_heads, page_size,
-                       page_shift_of(page_size / FP4_TOKENS), window, pages, q_stride, scale * 1.4426950408889634f, part_o, part_ml,
+                       page_shift_of(page_size / FP4_TOKENS), window, (int)pages,
+                       (unsigned)(page_size / FP4_TOKENS * kv_heads * 18 * head_dim), q_stride, scale * 1.4426950408889634f, part_o, part_ml,
                        (int*)(part_ml + (size_t)blocks * 2 * block_heads)};
     auto launch = head_dim == 64 ? (block_heads == 4 ? launch_decode<64, 0> : block_heads == 8 ? launch_decode<64, 1> : launch_decode<64, 2>)
                                  : (block_heads == 4 ? launch_decode<128, 0> : block_heads == 8 ? launch_decode<128, 1> : launch_decode<128, 2>);
