@@ -104,11 +104,11 @@ __device__ __forceinline__ void store_row(bf16* dst, float4 acc, float l) {
     *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(two);
 }
 
-// Tiles of a token that sees the keys from the first visible one to its own position.
-__device__ __forceinline__ int tiles_of(int pos, int window) {
+// Tiles of a token that sees the keys from the first visible one to its own position, as far as its block table goes.
+__device__ __forceinline__ int tiles_of(int pos, int window, int table_units) {
     if (pos < 0) return 0;
-    const int units = pos / FP4_TOKENS - first_visible(pos, window) / FP4_TOKENS + 1;
-    return (units + UNITS_A_TILE - 1) / UNITS_A_TILE;
+    const int units = min(pos / FP4_TOKENS, table_units - 1) - first_visible(pos, window) / FP4_TOKENS + 1;
+    return units <= 0 ? 0 : (units + UNITS_A_TILE - 1) / UNITS_A_TILE;
 }
 
 // One (token, kv head, group of heads) pair's part of a block's range.
@@ -129,7 +129,7 @@ __device__ __forceinline__ Piece next_piece(Cursor& at, int left, const int* pre
             Piece p;
             p.tok = at.tok;
             const int pair = at.rest / tiles;
-            p.kvh = pair / head_groups;
+            p.kvh = head_groups == 1 ? pair : pair / head_groups;
             p.hg = pair - p.kvh * head_groups;
             p.tile0 = at.rest - pair * tiles;
             p.tiles = min(left, tiles - p.tile0);
@@ -142,11 +142,11 @@ __device__ __forceinline__ Piece next_piece(Cursor& at, int left, const int* pre
     }
 }
 
-// HT: columns of eight that the heads of a pair take; 0: up to four heads, each with both of its columns in one.
-template <int D, int HT>
+// FOUR: up to four query heads, each with both of its columns in one product; else up to eight.
+template <int D, bool FOUR>
 struct Shape {
-    static constexpr int HEADS = HT == 0 ? 4 : 8 * HT, NT = HT == 0 ? 1 : HT;
-    static constexpr int MINE = HT == 0 ? 1 : 2 * HT;                            // heads whose scores a lane holds
+    static constexpr int HEADS = FOUR ? 4 : 8;
+    static constexpr int MINE = FOUR ? 1 : 2;                                    // heads whose scores a lane holds
     static constexpr int ROW = D + 4;                                            // a head's values, maximum, sum
     static constexpr int RING_BYTES = WARPS * STAGES * UNITS * Fp4Unit<D>::BYTES;
     static constexpr int MERGE_BYTES = WARPS * HEADS * ROW * 4;
@@ -157,27 +157,33 @@ struct Shape {
 // Sums tiles_of over the tokens into prefix[0 .. tokens], positions into held[0 .. tokens) and block-table rows into
 // held[tokens .. 2 tokens); all threads of the block.
 __device__ __forceinline__ void make_plan(int* prefix, int* held, const int* __restrict__ positions, const int* __restrict__ token_slot,
-                                          int tokens, int window, int* scratch) {
+                                          int tokens, int window, int table_units, int* scratch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int carried = 0;
     if (threadIdx.x == 0) prefix[0] = 0;
     for (int first = 0; first < tokens; first += THREADS) {
         const int t = first + threadIdx.x;
-        int pos = -1;
+        int pos = -1, table_row = -1;
         if (t < tokens) {
             pos = positions[t];
+            table_row = token_slot[t];
             held[t] = pos;
-            held[tokens + t] = token_slot[t];
+            held[tokens + t] = table_row;
         }
-        int sum = tiles_of(pos, window);
+        int sum = tiles_of(pos, window, table_units);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int below = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += below;
         }
+        if (first + THREADS >= tokens && tokens - first <= 32) {       // few tokens left: the first warp has them all
+            if (t < tokens) prefix[t + 1] = carried + sum;
+            break;
+        }
         if (lane == 31) scratch[warp] = sum;
         __syncthreads();
         int before = carried;
+#pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             if (w < warp) before += scratch[w];
             carried += scratch[w];
@@ -185,10 +191,11 @@ __device__ __forceinline__ void make_plan(int* prefix, int* held, const int* __r
         if (t < tokens) prefix[t + 1] = before + sum;
         __syncthreads();
     }
+    __syncthreads();
 }
 
 // Tiles that a block takes.
-__device__ __forceinline__ int tiles_a_block(long total, int blocks) { return (int)((total + blocks - 1) / blocks); }
+__device__ __forceinline__ int tiles_a_block(int total, int blocks) { return (total + blocks - 1) / blocks; }
 
 struct Step {
     const int* block_tables;
@@ -205,13 +212,13 @@ struct Step {
     int* plan;                   // [tokens + 1]: the prefix of tiles
 };
 
-template <int D, int HT>
-__global__ void __launch_bounds__(THREADS, HT == 2 ? 3 : 4)
+template <int D, bool FOUR>
+__global__ void __launch_bounds__(THREADS, 4)
 decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsigned char* __restrict__ cache, const Step step) {
     using Unit = Fp4Unit<D>;
-    using Sh = Shape<D, HT>;
-    constexpr int HEADS = Sh::HEADS, NT = Sh::NT, MINE = Sh::MINE, WORDS_K = D / 32, WORDS_V = D / 64, TILES_M = D / 32;
-    constexpr int COLUMNS = HT == 0 ? 1 : 2;           // products that give a 32-feature tile of a column of eight
+    using Sh = Shape<D, FOUR>;
+    constexpr int HEADS = Sh::HEADS, MINE = Sh::MINE, WORDS_K = D / 32, WORDS_V = D / 64, TILES_M = D / 32;
+    constexpr int COLUMNS = FOUR ? 1 : 2;              // products that give 32 features of the heads
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int scratch[WARPS];
     float* merge = reinterpret_cast<float*>(smem + Sh::RING_BYTES);              // [WARPS][HEADS][ROW]
@@ -221,33 +228,31 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     unsigned char* ring = smem + warp * STAGES * UNITS * Unit::BYTES;
     const int group = step.heads / step.kv_heads, head_groups = (group + HEADS - 1) / HEADS;
-    const int units_a_page = step.page_size / FP4_TOKENS, pairs = step.kv_heads * head_groups;
+    const int units_a_page = step.page_size / FP4_TOKENS, table_units = step.max_blocks * units_a_page, pairs = step.kv_heads * head_groups;
 
     dependents_may_start();                            // the second kernel's blocks come as these leave, and wait for the last
-    make_plan(prefix, held_pos, step.positions, step.token_slot, step.tokens, step.window, scratch);
+    make_plan(prefix, held_pos, step.positions, step.token_slot, step.tokens, step.window, table_units, scratch);
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i <= step.tokens; i += THREADS) step.plan[i] = prefix[i];
-    // padding rows come out as zeros
+    // rows without a tile (padding) come out as zeros
     for (int tok = blockIdx.x; tok < step.tokens; tok += gridDim.x)
-        if (held_pos[tok] < 0)
+        if (prefix[tok] == prefix[tok + 1])
             for (int i = threadIdx.x; i < step.heads * D / 2; i += THREADS)
                 reinterpret_cast<unsigned*>(out + (size_t)(step.rows ? step.rows[tok] : tok) * step.heads * D)[i] = 0u;
 
-    const long total = (long)prefix[step.tokens] * pairs;
-    const int per = tiles_a_block(total, gridDim.x);
-    const long begin = (long)blockIdx.x * per;
+    const int total = prefix[step.tokens] * pairs, per = tiles_a_block(total, gridDim.x), begin = blockIdx.x * per;
     if (begin >= total) return;
-    const int count = (int)min((long)per, total - begin);
+    const int count = min(per, total - begin);
     Cursor start;
     {   // the token whose tiles hold the block's first one
         int low = 0, high = step.tokens - 1;
         while (low < high) {
             const int mid = (low + high) / 2;
-            if ((long)prefix[mid + 1] * pairs <= begin) low = mid + 1;
+            if (prefix[mid + 1] * pairs <= begin) low = mid + 1;
             else high = mid;
         }
         start.tok = low;
-        start.rest = (int)(begin - (long)prefix[low] * pairs);
+        start.rest = begin - prefix[low] * pairs;
     }
 
     // ---- the copies: this warp's units of every tile, one tile ahead of the work.  The pages of a tile's units are asked for
@@ -268,7 +273,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                 ap = next_piece(ahead, count - located, prefix, step.kv_heads, head_groups);
                 ap_tile = 0;
                 const int pos = held_pos[ap.tok], table_row = held_row[ap.tok];
-                a_last = min(pos / FP4_TOKENS, step.max_blocks * units_a_page - 1);
+                a_last = min(pos / FP4_TOKENS, table_units - 1);
                 a_unit = first_visible(pos, step.window) / FP4_TOKENS + ap.tile0 * UNITS_A_TILE + warp * UNITS;
                 a_table = step.block_tables + (size_t)table_row * step.max_blocks;
                 if (table_row < 0 || table_row >= step.table_rows) a_last = -1;
@@ -303,29 +308,35 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
         ++issued;
         locate();
     };
+    // The queries of a piece: lane 4 g + t has features D/4 t .. of the head of column g.
+    uint4 raw[D / 32];
+    auto ask_queries = [&](const Piece& p) {
+        const int h = FOUR ? g >> 1 : g;
+        const size_t row = step.rows ? step.rows[p.tok] : p.tok;
+        const bf16* src = q + row * step.q_stride + (size_t)(p.kvh * group + p.hg * HEADS + h) * D + t * (D / 4);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            raw[c] = make_uint4(0, 0, 0, 0);
+            if (h < group - p.hg * HEADS) raw[c] = *reinterpret_cast<const uint4*>(src + c * 8);
+        }
+    };
+    Cursor at = start;
+    Piece p = next_piece(at, count, prefix, step.kv_heads, head_groups);
     locate();
+    ask_queries(p);
     issue();
 
-    Cursor at = start;
     for (int done = 0, seg = 0; done < count; ++seg) {
-        const Piece p = next_piece(at, count - done, prefix, step.kv_heads, head_groups);
         const int pos = held_pos[p.tok], lo = first_visible(pos, step.window), first_unit = lo / FP4_TOKENS;
         const size_t row = step.rows ? step.rows[p.tok] : p.tok;
         const int head0 = p.kvh * group + p.hg * HEADS, heads_here = min(HEADS, group - p.hg * HEADS);
 
-        // the queries: lane 4 g + t has features D/4 t .. of the head of column g, as halves with the largest of the head in [128, 256)
-        unsigned qf[NT][D / 16][2];
+        unsigned qf[D / 16][2];                            // as halves with the largest of the head in [128, 256)
         float scale[MINE];                                 // of the scores of the lane's heads
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int h = HT == 0 ? g >> 1 : nt * 8 + g;
-            const bf16* src = q + row * step.q_stride + (size_t)(head0 + h) * D + t * (D / 4);
-            uint4 raw[D / 32];
+        {
             float largest = 0.f;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-                raw[c] = make_uint4(0, 0, 0, 0);
-                if (h < heads_here) raw[c] = *reinterpret_cast<const uint4*>(src + c * 8);
                 const __nv_bfloat162* two = reinterpret_cast<const __nv_bfloat162*>(&raw[c]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -345,15 +356,15 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float2 f = __bfloat1622float2(two[e]);
-                    qf[nt][c * 2 + (e >> 1)][e & 1] = pack_h2(f.x * up, f.y * up);
+                    qf[c * 2 + (e >> 1)][e & 1] = pack_h2(f.x * up, f.y * up);
                 }
             }
             // never 0, which would make NaN of a hidden key's score (a head that small has scores of 0 either way)
-            scale[HT == 0 ? 0 : 2 * nt] = fmaxf(__shfl_sync(0xffffffffu, down, 8 * t) * step.scale_log2, FLT_MIN);
-            if constexpr (HT != 0) scale[2 * nt + 1] = fmaxf(__shfl_sync(0xffffffffu, down, 8 * t + 4) * step.scale_log2, FLT_MIN);
+#pragma unroll
+            for (int h = 0; h < MINE; ++h) scale[h] = fmaxf(__shfl_sync(0xffffffffu, down, 8 * t + 4 * h) * step.scale_log2, FLT_MIN);
         }
 
-        float m[MINE], nbase[MINE], l[MINE], o[NT][TILES_M][COLUMNS][4];     // nbase: LIFT less the maximum
+        float m[MINE], nbase[MINE], l[MINE], o[TILES_M][COLUMNS][4];         // nbase: LIFT less the maximum
 #pragma unroll
         for (int h = 0; h < MINE; ++h) {
             m[h] = -INFINITY;
@@ -361,11 +372,9 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             l[h] = 0.f;
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < TILES_M; ++i)
 #pragma unroll
-            for (int i = 0; i < TILES_M; ++i)
-#pragma unroll
-                for (int e = 0; e < COLUMNS; ++e) o[nt][i][e][0] = o[nt][i][e][1] = o[nt][i][e][2] = o[nt][i][e][3] = 0.f;
+            for (int e = 0; e < COLUMNS; ++e) o[i][e][0] = o[i][e][1] = o[i][e][2] = o[i][e][3] = 0.f;
 
         for (int tile = p.tile0; tile < p.tile0 + p.tiles; ++tile, ++done) {
             __syncwarp();                                  // the stage that is filled next was read by all lanes
@@ -379,12 +388,11 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             const bool whole = here == (1u << UNITS) - 1 && key0 >= lo && key0 + UNITS * FP4_TOKENS - 1 <= pos;
 
             // ---- scores
-            float c[UNITS][NT][4];
+            float c[UNITS][4];
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) {
                 const unsigned char* unit = stage + u * Unit::BYTES;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) c[u][nt][0] = c[u][nt][1] = c[u][nt][2] = c[u][nt][3] = 0.f;
+                c[u][0] = c[u][1] = c[u][2] = c[u][3] = 0.f;
                 unsigned kw[2][WORDS_K];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -413,12 +421,10 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            mma_f16(c[u][nt], a[0][2 * j], a[1][2 * j], a[0][2 * j + 1], a[1][2 * j + 1], qf[nt][2 * w + j][0], qf[nt][2 * w + j][1]);
+                        mma_f16(c[u], a[0][2 * j], a[1][2 * j], a[0][2 * j + 1], a[1][2 * j + 1], qf[2 * w + j][0], qf[2 * w + j][1]);
                 }
             }
-            // Score of the lane's head h with key g or g + 8 (r) of unit u: c[u][h / 2][h % 2 + 2 r].
+            // Score of the lane's head h with key g or g + 8 (r) of unit u: c[u][h + 2 r].
             unsigned seen[UNITS];                          // of the value scales, which a lane holds of keys 2 t, 2 t + 1, 2 t + 8 and 2 t + 9
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) seen[u] = 0xffffffffu;
@@ -431,10 +437,8 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
                 for (int u = 0; u < UNITS; ++u) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (hidden(u, g + (e >> 1) * 8)) c[u][nt][e] = -INFINITY;
+                    for (int e = 0; e < 4; ++e)
+                        if (hidden(u, g + (e >> 1) * 8)) c[u][e] = -INFINITY;
 #pragma unroll
                     for (int b = 0; b < 4; ++b)
                         if (hidden(u, (b >> 1) * 8 + 2 * t + (b & 1))) seen[u] &= ~(0xFFu << (8 * b));
@@ -448,7 +452,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                 for (int u = 0; u < UNITS; ++u)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        x[h][u][r] = against(c[u][h >> 1][(h & 1) + 2 * r], scale[h], nbase[h]);
+                        x[h][u][r] = against(c[u][h + 2 * r], scale[h], nbase[h]);
                         raise = raise || x[h][u][r] > LIFT + SLACK;
                     }
             if (__any_sync(0xffffffffu, raise)) {
@@ -458,8 +462,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
                     for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r)
-                            mx = fmaxf(mx, __fmul_rn(c[u][h >> 1][(h & 1) + 2 * r], scale[h]));
+                        for (int r = 0; r < 2; ++r) mx = fmaxf(mx, __fmul_rn(c[u][h + 2 * r], scale[h]));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -474,11 +477,11 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                         for (int e = 0; e < COLUMNS; ++e)
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                if (HT == 0 || (k & 1) == (h & 1)) o[h >> 1][i][e][k] *= corr;
+                                if (FOUR || (k & 1) == h) o[i][e][k] *= corr;
 #pragma unroll
                     for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) x[h][u][r] = against(c[u][h >> 1][(h & 1) + 2 * r], scale[h], nbase[h]);
+                        for (int r = 0; r < 2; ++r) x[h][u][r] = against(c[u][h + 2 * r], scale[h], nbase[h]);
                 }
             }
 #pragma unroll
@@ -495,8 +498,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) {
                 const unsigned char* unit = stage + u * Unit::BYTES;
-                unsigned vs = *reinterpret_cast<const unsigned*>(unit + Unit::V_SCALES + (D == 128 ? lane : (g >> 1) * 4 + t) * 4);
-                vs &= seen[u];
+                const unsigned vs = *reinterpret_cast<const unsigned*>(unit + Unit::V_SCALES + (D == 128 ? lane : (g >> 1) * 4 + t) * 4) & seen[u];
                 const unsigned sv[4] = {scale_twice<0>(vs), scale_twice<1>(vs), scale_twice<2>(vs), scale_twice<3>(vs)};
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -504,18 +506,14 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                     const unsigned char* src = unit + Unit::V_CODES + half * (4 * D) + lane * 2 * Unit::PIECE;
                     if constexpr (D == 128) *reinterpret_cast<uint4*>(vw) = *reinterpret_cast<const uint4*>(src);
                     else *reinterpret_cast<uint2*>(vw) = *reinterpret_cast<const uint2*>(src);
-                    unsigned b[NT][COLUMNS][2];            // P of tokens 2 t and 2 t + 1 for the head of column g
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const float p0 = x[HT == 0 ? 0 : 2 * nt][u][half], p1 = x[HT == 0 ? 0 : 2 * nt + 1][u][half];
-                        const unsigned pt = transposed(pack_h2(p0, p1));
-                        if constexpr (HT == 0) {           // column g is of head g / 2 and of the features of parity g % 2
-                            b[nt][0][0] = __byte_perm(pt, 0u, g & 1 ? 0x1044u : 0x4410u);
-                            b[nt][0][1] = __byte_perm(pt, 0u, g & 1 ? 0x3244u : 0x4432u);
-                        } else {
-                            b[nt][0][0] = pt & 0xffffu; b[nt][0][1] = pt >> 16;
-                            b[nt][COLUMNS - 1][0] = pt << 16; b[nt][COLUMNS - 1][1] = pt & 0xffff0000u;
-                        }
+                    unsigned b[COLUMNS][2];                // P of tokens 2 t and 2 t + 1 for the head of column g
+                    const unsigned pt = transposed(pack_h2(x[0][u][half], x[MINE - 1][u][half]));
+                    if constexpr (FOUR) {                  // column g is of head g / 2 and of the features of parity g % 2
+                        b[0][0] = __byte_perm(pt, 0u, g & 1 ? 0x1044u : 0x4410u);
+                        b[0][1] = __byte_perm(pt, 0u, g & 1 ? 0x3244u : 0x4432u);
+                    } else {
+                        b[0][0] = pt & 0xffffu; b[0][1] = pt >> 16;
+                        b[COLUMNS - 1][0] = pt << 16; b[COLUMNS - 1][1] = pt & 0xffff0000u;
                     }
 #pragma unroll
                     for (int w = 0; w < WORDS_V; ++w) {
@@ -529,31 +527,29 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
                         for (int j = 0; j < 2; ++j)
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int e = 0; e < COLUMNS; ++e)
-                                    mma_f16(o[nt][2 * w + j][e], a[0][2 * j], a[0][2 * j + 1], a[1][2 * j], a[1][2 * j + 1], b[nt][e][0], b[nt][e][1]);
+                            for (int e = 0; e < COLUMNS; ++e)
+                                mma_f16(o[2 * w + j][e], a[0][2 * j], a[0][2 * j + 1], a[1][2 * j], a[1][2 * j + 1], b[e][0], b[e][1]);
                     }
                 }
             }
         }
 
-        // ---- the four warps' results meet
+        // ---- the four warps' results meet; the next piece's queries are on their way meanwhile
+        const Piece next = done < count ? next_piece(at, count - done, prefix, step.kv_heads, head_groups) : p;
+        ask_queries(next);
 #pragma unroll
         for (int h = 0; h < MINE; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
-            const int head = HT == 0 ? t : (h >> 1) * 8 + 2 * t + (h & 1);
+            const int head = FOUR ? t : 2 * t + h;
             float* dst = merge + (warp * HEADS + head) * Sh::ROW;
             if (head < heads_here) {
 #pragma unroll
-                for (int i = 0; i < TILES_M; ++i) {        // features D/8 g + 4 i ..
-                    const float (&oo)[COLUMNS][4] = o[h >> 1][i];
+                for (int i = 0; i < TILES_M; ++i)          // features D/8 g + 4 i ..
                     *reinterpret_cast<float4*>(dst + g * (D / 8) + 4 * i) =
-                        HT == 0 ? make_float4(oo[0][0], oo[0][1], oo[0][2], oo[0][3])
-                                : make_float4(oo[0][h & 1], oo[COLUMNS - 1][h & 1], oo[0][(h & 1) + 2], oo[COLUMNS - 1][(h & 1) + 2]);
-                }
+                        FOUR ? make_float4(o[i][0][0], o[i][0][1], o[i][0][2], o[i][0][3])
+                             : make_float4(o[i][0][h], o[i][COLUMNS - 1][h], o[i][0][h + 2], o[i][COLUMNS - 1][h + 2]);
                 if (g == 0) {
                     dst[D] = m[h];
                     dst[D + 1] = l[h];
@@ -585,111 +581,122 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             }
         }
         __syncthreads();
+        p = next;
     }
     cp_async_wait<0>();
 }
 
-// Adds the pieces of the pairs that lie in several blocks: grid (tokens * pairs, heads of a pair), a block a head.  A slice of
-// the threads takes every SLICES-th piece, four values a thread; then the slices are added in their order.
-template <int D, int HT>
+// Adds the pieces of the pairs that lie in several blocks.  Four values of a head a thread; the groups of D / 4 threads of a block take a head each
+// (grid: pairs, heads / groups), or with `deep`, where pairs are few and their pieces many, every so-manieth piece of
+// one head (grid: pairs, heads), added in the groups' order at the end.
+template <int D, bool FOUR>
 __global__ void __launch_bounds__(MERGE_THREADS)
-merge_fp4_kernel(bf16* __restrict__ out, const Step step, int blocks) {
-    constexpr int HEADS = Shape<D, HT>::HEADS, LANES = D / 4, SLICES = MERGE_THREADS / LANES;
-    __shared__ float4 sums[SLICES][LANES];
-    __shared__ float2 tops[SLICES];
+merge_fp4_kernel(bf16* __restrict__ out, const Step step, int blocks, int deep) {
+    constexpr int HEADS = Shape<D, FOUR>::HEADS, LANES = D / 4, GROUPS = MERGE_THREADS / LANES;
+    __shared__ float4 sums[GROUPS][LANES];
+    __shared__ float2 tops[GROUPS];
     const int group = step.heads / step.kv_heads, head_groups = (group + HEADS - 1) / HEADS, pairs = step.kv_heads * head_groups;
     const int tok = blockIdx.x / pairs, pair = blockIdx.x - tok * pairs, kvh = pair / head_groups, hg = pair - kvh * head_groups;
-    const int head = blockIdx.y;
-    if (head >= group - hg * HEADS) return;
+    const int part = threadIdx.x / LANES, d = threadIdx.x % LANES;
+    const int head = deep ? blockIdx.y : blockIdx.y * GROUPS + part, slice = deep ? part : 0, slices = deep ? GROUPS : 1;
     wait_for_kernel_before();
     const int before = __ldcg(step.plan + tok), tiles = __ldcg(step.plan + tok + 1) - before;
-    const long total = (long)__ldcg(step.plan + step.tokens) * pairs;
+    const int total = __ldcg(step.plan + step.tokens) * pairs;
     if (tiles == 0) return;
-    const int per = tiles_a_block(total, blocks);
-    const long start = (long)before * pairs + (long)pair * tiles;
-    const int first = (int)(start / per), last = (int)((start + tiles - 1) / per);
+    const int per = tiles_a_block(total, blocks), start = before * pairs + pair * tiles;
+    const int first = start / per, last = (start + tiles - 1) / per;
     if (first == last) return;
     // a block's piece of this pair is its first one where its range begins inside the pair
-    auto slot = [&](int b) { return ((size_t)b * 2 + ((long)b * per >= start ? 0 : 1)) * HEADS + head; };
-    const int slice = threadIdx.x / LANES, d = threadIdx.x % LANES;
+    auto slot = [&](int b) { return ((size_t)b * 2 + (b * per >= start ? 0 : 1)) * HEADS + head; };
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int b0 = first + slice; b0 <= last; b0 += 4 * SLICES) {
-        float2 ml[4];
-        float4 v[4];
+    if (head < group - hg * HEADS && head < HEADS)
+        for (int b0 = first + slice; b0 <= last; b0 += 4 * slices) {
+            float2 ml[4];
+            float4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {                      // all asked for before any is used
-            ml[k] = make_float2(-INFINITY, 0.f);
-            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            const int b = b0 + k * SLICES;
-            if (b <= last) {
-                ml[k] = __ldcg(step.part_ml + slot(b));
-                v[k] = __ldcg(reinterpret_cast<const float4*>(step.part_o + slot(b) * D) + d);
+            for (int k = 0; k < 4; ++k) {                  // all asked for before any is used
+                ml[k] = make_float2(-INFINITY, 0.f);
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                const int b = b0 + k * slices;
+                if (b <= last) {
+                    ml[k] = __ldcg(step.part_ml + slot(b));
+                    v[k] = __ldcg(reinterpret_cast<const float4*>(step.part_o + slot(b) * D) + d);
+                }
             }
-        }
-        float mm = m;
+            float mm = m;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mm = fmaxf(mm, ml[k].x);
-        const float old = weight_of(m, l, mm);
-        acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
-        l *= old;
+            for (int k = 0; k < 4; ++k) mm = fmaxf(mm, ml[k].x);
+            const float old = weight_of(m, l, mm);
+            acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+            l *= old;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float f = weight_of(ml[k].x, ml[k].y, mm);
-            acc.x += v[k].x * f; acc.y += v[k].y * f; acc.z += v[k].z * f; acc.w += v[k].w * f;
-            l += ml[k].y * f;
+            for (int k = 0; k < 4; ++k) {
+                const float f = weight_of(ml[k].x, ml[k].y, mm);
+                acc.x += v[k].x * f; acc.y += v[k].y * f; acc.z += v[k].z * f; acc.w += v[k].w * f;
+                l += ml[k].y * f;
+            }
+            m = mm;
         }
-        m = mm;
+    const size_t row = step.rows ? step.rows[tok] : tok;
+    bf16* dst = out + row * step.heads * D + (size_t)(kvh * group + hg * HEADS + head) * D + d * 4;
+    if (!deep) {
+        if (head < group - hg * HEADS && head < HEADS) store_row(dst, acc, l);
+        return;
     }
-    sums[slice][d] = acc;
-    if (d == 0) tops[slice] = make_float2(m, l);
+    sums[part][d] = acc;
+    if (d == 0) tops[part] = make_float2(m, l);
     __syncthreads();
-    if (slice) return;
-    float mm = -INFINITY, ll = 0.f;
+    if (part || head >= group - hg * HEADS) return;
+    m = -INFINITY;
+    l = 0.f;
 #pragma unroll
-    for (int i = 0; i < SLICES; ++i) mm = fmaxf(mm, tops[i].x);
+    for (int i = 0; i < GROUPS; ++i) m = fmaxf(m, tops[i].x);
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < SLICES; ++i) {
-        const float f = weight_of(tops[i].x, tops[i].y, mm);
+    for (int i = 0; i < GROUPS; ++i) {
+        const float f = weight_of(tops[i].x, tops[i].y, m);
         const float4 v = sums[i][d];
         acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-        ll += tops[i].y * f;
+        l += tops[i].y * f;
     }
-    const size_t row = step.rows ? step.rows[tok] : tok;
-    store_row(out + row * step.heads * D + (size_t)(kvh * group + hg * HEADS + head) * D + d * 4, acc, ll);
+    store_row(dst, acc, l);
 }
 
-template <int D, int HT>
+template <int D, bool FOUR>
 cudaError_t launch_decode(const bf16* q, bf16* out, const unsigned char* cache, const Step& step, int blocks, cudaStream_t stream) {
-    using Sh = Shape<D, HT>;
-    cudaError_t err = cudaFuncSetAttribute(decode_fp4_kernel<D, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::bytes(MAX_TOKENS));
+    using Sh = Shape<D, FOUR>;
+    cudaError_t err = cudaFuncSetAttribute(decode_fp4_kernel<D, FOUR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::bytes(MAX_TOKENS));
     if (err != cudaSuccess) return err;
-    err = launch_kernel(decode_fp4_kernel<D, HT>, dim3(blocks), dim3(THREADS), Sh::bytes(step.tokens), stream, q, out, cache, step);
+    err = launch_kernel(decode_fp4_kernel<D, FOUR>, dim3(blocks), dim3(THREADS), Sh::bytes(step.tokens), stream, q, out, cache, step);
     if (err != cudaSuccess) return err;
+    constexpr int GROUPS = MERGE_THREADS / (D / 4);
     const int group = step.heads / step.kv_heads, head_groups = (group + Sh::HEADS - 1) / Sh::HEADS;
-    return launch_kernel_overlapped(merge_fp4_kernel<D, HT>, dim3(step.tokens * step.kv_heads * head_groups, group < Sh::HEADS ? group : Sh::HEADS),
-                                    dim3(MERGE_THREADS), 0, stream, out, step, blocks);
+    const int pairs = step.tokens * step.kv_heads * head_groups, heads = group < Sh::HEADS ? group : Sh::HEADS;
+    const int deep = 4 * pairs < blocks;               // more than four pieces a pair
+    return launch_kernel_overlapped(merge_fp4_kernel<D, FOUR>, dim3(pairs, deep ? heads : (heads + GROUPS - 1) / GROUPS), dim3(MERGE_THREADS), 0,
+                                    stream, out, step, blocks, deep);
 }
 
-template <int D, int HT> int occupancy() {
+template <int D, bool FOUR> int occupancy() {
     int n = 0;
-    const size_t smem = Shape<D, HT>::bytes(MAX_TOKENS);
-    if (cudaFuncSetAttribute(decode_fp4_kernel<D, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_fp4_kernel<D, HT>, THREADS, smem) != cudaSuccess) return 0;
+    const size_t smem = Shape<D, FOUR>::bytes(MAX_TOKENS);
+    if (cudaFuncSetAttribute(decode_fp4_kernel<D, FOUR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_fp4_kernel<D, FOUR>, THREADS, smem) != cudaSuccess) return 0;
     return n;
 }
 
-// Heads that a block takes of a kv head's group.
-int heads_a_block(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
+// Heads that a block takes of a kv head's group.  Groups of more than eight are cut: sixteen heads in one block (their
+// outputs and queries take 96 registers a thread, three blocks a multiprocessor) were slower than reading the pages
+// from the L2 cache for each eight (B200, 16 requests of up to 16,384 keys, 32 heads over 2: see the figures in the design document).
+int heads_a_block(int group) { return group <= 4 ? 4 : 8; }
 
 }  // namespace
 
 // Blocks of the decode kernel that a multiprocessor holds at once; 0: the device refuses.
 MRUN_API int mrun_attn_fp4_occupancy(int head_dim, int group) {
-    const int heads = heads_a_block(group);
-    return head_dim == 64 ? (heads == 4 ? occupancy<64, 0>() : heads == 8 ? occupancy<64, 1>() : occupancy<64, 2>())
-                          : (heads == 4 ? occupancy<128, 0>() : heads == 8 ? occupancy<128, 1>() : occupancy<128, 2>());
+    return head_dim == 64 ? (group <= 4 ? occupancy<64, true>() : occupancy<64, false>())
+                          : (group <= 4 ? occupancy<128, true>() : occupancy<128, false>());
 }
 
 // Bytes of scratch that a launch of `blocks` blocks over `tokens` tokens takes.
@@ -710,19 +717,21 @@ MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const
     MRUN_REQUIRE(page_size > 0 && page_size % FP4_TOKENS == 0, "%s: page_size=%d is not a multiple of 16", name, page_size);
     MRUN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)scratch) & 15) == 0 && q_stride % 8 == 0,
                  "%s: rows and pages start on 16 bytes", name);
-    MRUN_REQUIRE(pages < (1L << 31) && (long)page_size / FP4_TOKENS * kv_heads * 18 * head_dim < (1L << 31) && (long)max_blocks * (page_size / FP4_TOKENS) < (1L << 31),
-                 "%s: pages=%ld of %d tokens and %d kv heads", name, pages, page_size, kv_heads);
+    const long page_units = page_size / FP4_TOKENS, table_tiles = max_blocks * page_units / UNITS_A_TILE + 1;
+    MRUN_REQUIRE(pages < (1L << 31) && page_units * kv_heads * 18 * head_dim < (1L << 31), "%s: pages=%ld of %d tokens and %d kv heads", name,
+                 pages, page_size, kv_heads);
+    MRUN_REQUIRE(max_blocks * page_units < (1L << 31) && table_tiles * tokens * heads < (1L << 31),
+                 "%s: %d tokens of %d heads over block tables of %d pages of %d tokens", name, tokens, heads, max_blocks, page_size);
     MRUN_REQUIRE(scale > 0.f && scale < FLT_MAX, "%s: scale=%g is not a positive number", name, (double)scale);
     if (tokens == 0) return 0;
-    const int block_heads = heads_a_block(heads / kv_heads);
+    const int group = heads / kv_heads, block_heads = heads_a_block(group);
     float* part_o = (float*)scratch;
     float2* part_ml = (float2*)(part_o + (size_t)blocks * 2 * block_heads * head_dim);
     const Step step = {block_tables, token_slot, positions, rows, max_blocks, table_rows, tokens, heads, kv_heads, page_size,
-                       page_shift_of(page_size / FP4_TOKENS), window, (int)pages,
-                       (unsigned)(page_size / FP4_TOKENS * kv_heads * 18 * head_dim), q_stride, scale * 1.4426950408889634f, part_o, part_ml,
-                       (int*)(part_ml + (size_t)blocks * 2 * block_heads)};
-    auto launch = head_dim == 64 ? (block_heads == 4 ? launch_decode<64, 0> : block_heads == 8 ? launch_decode<64, 1> : launch_decode<64, 2>)
-                                 : (block_heads == 4 ? launch_decode<128, 0> : block_heads == 8 ? launch_decode<128, 1> : launch_decode<128, 2>);
+                       page_shift_of((int)page_units), window, (int)pages, (unsigned)(page_units * kv_heads * 18 * head_dim), q_stride,
+                       scale * 1.4426950408889634f, part_o, part_ml, (int*)(part_ml + (size_t)blocks * 2 * block_heads)};
+    auto launch = head_dim == 64 ? (group <= 4 ? launch_decode<64, true> : launch_decode<64, false>)
+                                 : (group <= 4 ? launch_decode<128, true> : launch_decode<128, false>);
     MRUN_CHECK_CUDA(launch((const bf16*)q, (bf16*)out, (const unsigned char*)cache, step, blocks, stream), name);
     MRUN_CHECK_LAUNCH(name);
     return 0;

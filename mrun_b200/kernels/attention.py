@@ -506,7 +506,7 @@ class _View:
 
 def _fp4_blocks(library, device: torch.device, head_dim: int, ratio: int) -> tuple:
     """(blocks of the decode kernel that the device holds, heads that a block takes)."""
-    rows = 4 if ratio <= 4 else 8 if ratio <= 8 else 16
+    rows = 4 if ratio <= 4 else 8
     found = _fp4_slots.get((device, head_dim, rows))
     if found is None:
         per_sm = library.function("mrun_attn_fp4_occupancy")(head_dim, ratio)
