@@ -24,6 +24,7 @@
 // (token, kv head, group of heads) pair.  The tiles (8 units) of all pairs lie in one list, cut evenly among the
 // blocks that the device holds at once; a pair that lies in several blocks leaves its pieces in scratch, and
 // a second kernel, on the device before the first has ended, adds them in block order.
+#include <atomic>
 #include <cfloat>
 #include <cuda_fp16.h>
 
@@ -154,10 +155,18 @@ struct Shape {
     static size_t bytes(int tokens) { return RING_BYTES + MERGE_BYTES + (size_t)(3 * tokens + 1) * 4; }
 };
 
+// Which rows of the step a launch's tokens are: the first ones, or (listed) these, given by value so that no copy
+// to the device goes before the launch.
+struct Rows {
+    int listed;
+    int row[MAX_TOKENS];
+    __device__ __forceinline__ int of(int tok) const { return listed ? row[tok] : tok; }
+};
+
 // Sums tiles_of over the tokens into prefix[0 .. tokens], positions into held[0 .. tokens) and block-table rows into
 // held[tokens .. 2 tokens); all threads of the block.
 __device__ __forceinline__ void make_plan(int* prefix, int* held, const int* __restrict__ positions, const int* __restrict__ token_slot,
-                                          int tokens, int window, int table_units, int* scratch) {
+                                          const Rows& rows, int tokens, int window, int table_units, int* scratch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int carried = 0;
     if (threadIdx.x == 0) prefix[0] = 0;
@@ -165,8 +174,9 @@ __device__ __forceinline__ void make_plan(int* prefix, int* held, const int* __r
         const int t = first + threadIdx.x;
         int pos = -1, table_row = -1;
         if (t < tokens) {
-            pos = positions[t];
-            table_row = token_slot[t];
+            const int row = rows.of(t);
+            pos = positions[row];
+            table_row = token_slot[row];
             held[t] = pos;
             held[tokens + t] = table_row;
         }
@@ -201,7 +211,6 @@ struct Step {
     const int* block_tables;
     const int* token_slot;
     const int* positions;
-    const int* rows;             // the rows of q and out that the tokens are, or null: the first ones
     int max_blocks, table_rows, tokens, heads, kv_heads, page_size, unit_shift, window;     // unit_shift: of the units of a page, or -1
     int pages;
     unsigned page_bytes;         // of all kv heads
@@ -214,7 +223,8 @@ struct Step {
 
 template <int D, bool FOUR>
 __global__ void __launch_bounds__(THREADS, 4)
-decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsigned char* __restrict__ cache, const Step step) {
+decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsigned char* __restrict__ cache, const Step step,
+                  const __grid_constant__ Rows rows) {
     using Unit = Fp4Unit<D>;
     using Sh = Shape<D, FOUR>;
     constexpr int HEADS = Sh::HEADS, MINE = Sh::MINE, WORDS_K = D / 32, WORDS_V = D / 64, TILES_M = D / 32;
@@ -231,14 +241,14 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     const int units_a_page = step.page_size / FP4_TOKENS, table_units = step.max_blocks * units_a_page, pairs = step.kv_heads * head_groups;
 
     dependents_may_start();                            // the second kernel's blocks come as these leave, and wait for the last
-    make_plan(prefix, held_pos, step.positions, step.token_slot, step.tokens, step.window, table_units, scratch);
+    make_plan(prefix, held_pos, step.positions, step.token_slot, rows, step.tokens, step.window, table_units, scratch);
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i <= step.tokens; i += THREADS) step.plan[i] = prefix[i];
     // rows without a tile (padding) come out as zeros
     for (int tok = blockIdx.x; tok < step.tokens; tok += gridDim.x)
         if (prefix[tok] == prefix[tok + 1])
             for (int i = threadIdx.x; i < step.heads * D / 2; i += THREADS)
-                reinterpret_cast<unsigned*>(out + (size_t)(step.rows ? step.rows[tok] : tok) * step.heads * D)[i] = 0u;
+                reinterpret_cast<unsigned*>(out + (size_t)rows.of(tok) * step.heads * D)[i] = 0u;
 
     const int total = prefix[step.tokens] * pairs, per = tiles_a_block(total, gridDim.x), begin = blockIdx.x * per;
     if (begin >= total) return;
@@ -312,7 +322,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     uint4 raw[D / 32];
     auto ask_queries = [&](const Piece& p) {
         const int h = FOUR ? g >> 1 : g;
-        const size_t row = step.rows ? step.rows[p.tok] : p.tok;
+        const size_t row = rows.of(p.tok);
         const bf16* src = q + row * step.q_stride + (size_t)(p.kvh * group + p.hg * HEADS + h) * D + t * (D / 4);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -328,7 +338,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 
     for (int done = 0, seg = 0; done < count; ++seg) {
         const int pos = held_pos[p.tok], lo = first_visible(pos, step.window), first_unit = lo / FP4_TOKENS;
-        const size_t row = step.rows ? step.rows[p.tok] : p.tok;
+        const size_t row = rows.of(p.tok);
         const int head0 = p.kvh * group + p.hg * HEADS, heads_here = min(HEADS, group - p.hg * HEADS);
 
         unsigned qf[D / 16][2];                            // as halves with the largest of the head in [128, 256)
@@ -591,7 +601,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 // one head (grid: pairs, heads), added in the groups' order at the end.
 template <int D, bool FOUR>
 __global__ void __launch_bounds__(MERGE_THREADS)
-merge_fp4_kernel(bf16* __restrict__ out, const Step step, int blocks, int deep) {
+merge_fp4_kernel(bf16* __restrict__ out, const Step step, const __grid_constant__ Rows rows, int blocks, int deep) {
     constexpr int HEADS = Shape<D, FOUR>::HEADS, LANES = D / 4, GROUPS = MERGE_THREADS / LANES;
     __shared__ float4 sums[GROUPS][LANES];
     __shared__ float2 tops[GROUPS];
@@ -638,8 +648,7 @@ merge_fp4_kernel(bf16* __restrict__ out, const Step step, int blocks, int deep) 
             }
             m = mm;
         }
-    const size_t row = step.rows ? step.rows[tok] : tok;
-    bf16* dst = out + row * step.heads * D + (size_t)(kvh * group + hg * HEADS + head) * D + d * 4;
+    bf16* dst = out + (size_t)rows.of(tok) * step.heads * D + (size_t)(kvh * group + hg * HEADS + head) * D + d * 4;
     if (!deep) {
         if (head < group - hg * HEADS && head < HEADS) store_row(dst, acc, l);
         return;
@@ -663,25 +672,39 @@ merge_fp4_kernel(bf16* __restrict__ out, const Step step, int blocks, int deep) 
     store_row(dst, acc, l);
 }
 
-template <int D, bool FOUR>
-cudaError_t launch_decode(const bf16* q, bf16* out, const unsigned char* cache, const Step& step, int blocks, cudaStream_t stream) {
-    using Sh = Shape<D, FOUR>;
-    cudaError_t err = cudaFuncSetAttribute(decode_fp4_kernel<D, FOUR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::bytes(MAX_TOKENS));
+// Lets the decode kernel have its shared memory on the current device, once a device.
+template <int D, bool FOUR> cudaError_t allow_shared() {
+    static std::atomic<unsigned long long> allowed{0};
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
     if (err != cudaSuccess) return err;
-    err = launch_kernel(decode_fp4_kernel<D, FOUR>, dim3(blocks), dim3(THREADS), Sh::bytes(step.tokens), stream, q, out, cache, step);
+    const unsigned long long bit = 1ull << (device & 63);
+    if (device < 64 && (allowed.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    err = cudaFuncSetAttribute(decode_fp4_kernel<D, FOUR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<D, FOUR>::bytes(MAX_TOKENS));
+    if (err == cudaSuccess && device < 64) allowed.fetch_or(bit, std::memory_order_relaxed);
+    return err;
+}
+
+template <int D, bool FOUR>
+cudaError_t launch_decode(const bf16* q, bf16* out, const unsigned char* cache, const Step& step, const Rows& rows, int blocks,
+                          cudaStream_t stream) {
+    using Sh = Shape<D, FOUR>;
+    cudaError_t err = allow_shared<D, FOUR>();
+    if (err != cudaSuccess) return err;
+    err = launch_kernel(decode_fp4_kernel<D, FOUR>, dim3(blocks), dim3(THREADS), Sh::bytes(step.tokens), stream, q, out, cache, step, rows);
     if (err != cudaSuccess) return err;
     constexpr int GROUPS = MERGE_THREADS / (D / 4);
     const int group = step.heads / step.kv_heads, head_groups = (group + Sh::HEADS - 1) / Sh::HEADS;
     const int pairs = step.tokens * step.kv_heads * head_groups, heads = group < Sh::HEADS ? group : Sh::HEADS;
     const int deep = 4 * pairs < blocks;               // more than four pieces a pair
     return launch_kernel_overlapped(merge_fp4_kernel<D, FOUR>, dim3(pairs, deep ? heads : (heads + GROUPS - 1) / GROUPS), dim3(MERGE_THREADS), 0,
-                                    stream, out, step, blocks, deep);
+                                    stream, out, step, rows, blocks, deep);
 }
 
 template <int D, bool FOUR> int occupancy() {
     int n = 0;
     const size_t smem = Shape<D, FOUR>::bytes(MAX_TOKENS);
-    if (cudaFuncSetAttribute(decode_fp4_kernel<D, FOUR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+    if (allow_shared<D, FOUR>() != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_fp4_kernel<D, FOUR>, THREADS, smem) != cudaSuccess) return 0;
     return n;
 }
@@ -699,12 +722,9 @@ MRUN_API int mrun_attn_fp4_occupancy(int head_dim, int group) {
                           : (group <= 4 ? occupancy<128, true>() : occupancy<128, false>());
 }
 
-// Bytes of scratch that a launch of `blocks` blocks over `tokens` tokens takes.
-MRUN_API int mrun_attn_fp4_scratch(int blocks, int tokens, int head_dim, int group) {
-    return blocks * 2 * heads_a_block(group) * (head_dim * 4 + 8) + (tokens + 1) * 4;
-}
 
-// One token a row: `tokens` rows of q and out, or those that `rows` names.  scratch: see mrun_attn_fp4_scratch, on 16 bytes.
+// One token a row of q, out, positions and token_slot: the first `tokens` rows, or those that `rows` (host memory) names.  scratch:
+// 4-byte words: blocks * 2 * (4 or 8 heads) * (head_dim + 2) + tokens + 1, on 16 bytes.
 MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const void* cache, const int* block_tables, int table_rows,
                                   int max_blocks, const int* token_slot, const int* positions, const int* rows, int tokens, int heads,
                                   int kv_heads, int head_dim, int page_size, long pages, float scale, int window, void* scratch,
@@ -727,12 +747,16 @@ MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const
     const int group = heads / kv_heads, block_heads = heads_a_block(group);
     float* part_o = (float*)scratch;
     float2* part_ml = (float2*)(part_o + (size_t)blocks * 2 * block_heads * head_dim);
-    const Step step = {block_tables, token_slot, positions, rows, max_blocks, table_rows, tokens, heads, kv_heads, page_size,
+    Rows selected;
+    selected.listed = rows != nullptr;
+    if (rows)
+        for (int i = 0; i < MAX_TOKENS; ++i) selected.row[i] = i < tokens ? rows[i] : 0;
+    const Step step = {block_tables, token_slot, positions, max_blocks, table_rows, tokens, heads, kv_heads, page_size,
                        page_shift_of((int)page_units), window, (int)pages, (unsigned)(page_units * kv_heads * 18 * head_dim), q_stride,
                        scale * 1.4426950408889634f, part_o, part_ml, (int*)(part_ml + (size_t)blocks * 2 * block_heads)};
     auto launch = head_dim == 64 ? (group <= 4 ? launch_decode<64, true> : launch_decode<64, false>)
                                  : (group <= 4 ? launch_decode<128, true> : launch_decode<128, false>);
-    MRUN_CHECK_CUDA(launch((const bf16*)q, (bf16*)out, (const unsigned char*)cache, step, blocks, stream), name);
+    MRUN_CHECK_CUDA(launch((const bf16*)q, (bf16*)out, (const unsigned char*)cache, step, selected, blocks, stream), name);
     MRUN_CHECK_LAUNCH(name);
     return 0;
 }

@@ -215,8 +215,10 @@ qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, lon
 // Reading back into rows [page, kv head, row, :] of bfloat16 keys and values (exact: a value has at most 6
 // significant bits).  A block takes 16 rows of one kv head, a thread eight features of a key and of a value.
 //   ids      output page i is cache page ids[i]
-//   ranges   output page i holds tokens ranges[i].y .. of the request in block-table row ranges[i].x, its first
-//            ranges[i].z rows; the rest are zeros
+//   spans    the output pages hold the tokens of spans of requests, one span's pages after the other's: tokens `first` .. `end` (a
+//            span begins with an output page's first row) of the request in block-table row `row`; rows behind `end`
+//            are zeros.  The blocks of the first kv head also write the spans' own block tables ([spans, table_width], -1 in front of
+//            `first`) and, for the rows row0 .. row0 + rows of the step, which span they belong to.
 // A page outside the cache gives zeros.
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned half2_of_codes(unsigned byte) {
@@ -225,26 +227,52 @@ __device__ __forceinline__ unsigned half2_of_codes(unsigned byte) {
     return out;
 }
 
+constexpr int MAX_SPANS = 64;               // of one launch: they are given by value, so that no copy to the device goes before it
+struct Span {
+    int row, first, end, page0, row0, rows;  // page0: its first output page
+};
+struct Spans {
+    int n, index0;                          // index0: of the first of them among the call's
+    Span span[MAX_SPANS];
+    int* table;                             // null: neither is written
+    int table_width;
+    int* span_of_row;
+};
+
 template <int D>
 __global__ void __launch_bounds__(2 * D)
-fp4_rows_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ ids, const int4* __restrict__ ranges,
+fp4_rows_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ ids, const __grid_constant__ Spans spans,
                 const int* __restrict__ block_tables, int table_rows, int max_blocks, bf16* __restrict__ k_out, bf16* __restrict__ v_out,
                 int kv_heads, int page_size, int out_page, long pages) {
     using Unit = Fp4Unit<D>;
     constexpr int LANES = D / 8;
     const int units_out = out_page / FP4_TOKENS, units_in = page_size / FP4_TOKENS;
-    const int i = blockIdx.x / units_out, unit_out = blockIdx.x - i * units_out, kv_head = blockIdx.y;
+    int i = blockIdx.x / units_out;
+    const int unit_out = blockIdx.x - i * units_out, kv_head = blockIdx.y;
     const int part = threadIdx.x % LANES, r = threadIdx.x / LANES;
     long page = -1;
     int unit_in = unit_out, rows = FP4_TOKENS;
     if (ids) {
         page = ids[i];
     } else {
-        const int4 range = ranges[i];
-        const int unit = range.y / FP4_TOKENS + unit_out, block = unit / units_in;      // a range begins with a unit
+        i += spans.span[0].page0;
+        int s = 0;
+        while (s + 1 < spans.n && spans.span[s + 1].page0 <= i) ++s;
+        const Span& span = spans.span[s];
+        const int in_span = i - span.page0, unit = span.first / FP4_TOKENS + in_span * units_out + unit_out, block = unit / units_in;
         unit_in = unit - block * units_in;
-        rows = range.z - unit_out * FP4_TOKENS;
-        if (rows > 0 && range.x >= 0 && range.x < table_rows && block < max_blocks) page = block_tables[(size_t)range.x * max_blocks + block];
+        rows = span.end - unit * FP4_TOKENS;
+        if (rows > 0 && span.row >= 0 && span.row < table_rows && block < max_blocks) page = block_tables[(size_t)span.row * max_blocks + block];
+        if (spans.table && kv_head == 0 && unit_out == 0) {
+            int* table = spans.table + (size_t)(spans.index0 + s) * spans.table_width;
+            const int before = span.first / out_page;
+            if (threadIdx.x == 0) table[before + in_span] = i;
+            if (in_span == 0) {
+                for (int b = threadIdx.x; b < before; b += 2 * D) table[b] = -1;
+                for (int b = before + (span.end - span.first + out_page - 1) / out_page + threadIdx.x; b < spans.table_width; b += 2 * D) table[b] = -1;
+                for (int r0 = threadIdx.x; r0 < span.rows; r0 += 2 * D) spans.span_of_row[span.row0 + r0] = spans.index0 + s;
+            }
+        }
     }
     uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     if (page >= 0 && page < pages && r < rows) {
@@ -278,6 +306,23 @@ cudaError_t launch_store(const void* qkv, void* q_out, long q_stride, const floa
                          rotary_dim / 2, slots, (unsigned char*)cache, tokens, heads, kv_heads, page_size, pages);
 }
 
+int launch_rows(const void* cache, const int* ids, const Spans& spans, const int* block_tables, int table_rows, int max_blocks, void* k_out,
+                void* v_out, int n, int kv_heads, int head_dim, int page_size, int out_page, long pages, const char* name, cudaStream_t stream) {
+    MRUN_REQUIRE(n >= 0 && kv_heads > 0 && kv_heads < 65536 && pages >= 0, "%s: bad sizes", name);
+    MRUN_REQUIRE((((uintptr_t)cache | (uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "%s: pages start on 16 bytes", name);
+    if (n == 0) return 0;
+    const long blocks = (long)n * (out_page / FP4_TOKENS);
+    MRUN_REQUIRE(blocks < (1L << 31), "%s: %d pages are more than a launch takes", name, n);
+    const dim3 grid((unsigned)blocks, (unsigned)kv_heads);
+    const auto launch = [&](auto kernel) {
+        return launch_kernel(kernel, grid, dim3(2 * head_dim), 0, stream, (const unsigned char*)cache, ids, spans, block_tables, table_rows,
+                             max_blocks, (bf16*)k_out, (bf16*)v_out, kv_heads, page_size, out_page, pages);
+    };
+    MRUN_CHECK_CUDA(head_dim == 64 ? launch(fp4_rows_kernel<64>) : launch(fp4_rows_kernel<128>), name);
+    MRUN_CHECK_LAUNCH(name);
+    return 0;
+}
+
 }  // namespace
 
 #define MRUN_REQUIRE_FP4(head_dim, page_size, name)                                                                   \
@@ -308,25 +353,45 @@ MRUN_API int mrun_qk_norm_rope_cache_fp4(const void* qkv, void* q_out, long q_st
     return 0;
 }
 
-// Either `ids` or `ranges` (with the block tables), int [n] or [n, 4]; out_page: rows of an output page.
-MRUN_API int mrun_fp4_rows(const void* cache, const int* ids, const void* ranges, const int* block_tables, int table_rows, int max_blocks,
-                           void* k_out, void* v_out, int n, int kv_heads, int head_dim, int page_size, int out_page, long pages,
-                           cudaStream_t stream) {
-    const char* name = "fp4_rows";
-    MRUN_REQUIRE(n >= 0 && kv_heads > 0 && kv_heads < 65536 && pages >= 0, "%s: bad sizes", name);
+// Output page i is cache page ids[i].
+MRUN_API int mrun_fp4_pages(const void* cache, const int* ids, void* k_out, void* v_out, int n, int kv_heads, int head_dim,
+                            int page_size, long pages, cudaStream_t stream) {
+    const char* name = "fp4_pages";
     MRUN_REQUIRE_FP4(head_dim, page_size, name);
-    MRUN_REQUIRE(out_page > 0 && out_page % FP4_TOKENS == 0 && (ranges || out_page == page_size), "%s: out_page=%d", name, out_page);
-    MRUN_REQUIRE((ids != nullptr) != (ranges != nullptr) && (!ranges || block_tables), "%s: pages or ranges of block tables", name);
-    MRUN_REQUIRE((((uintptr_t)cache | (uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)ranges) & 15) == 0, "%s: pages start on 16 bytes", name);
-    if (n == 0) return 0;
-    const long blocks = (long)n * (out_page / FP4_TOKENS);
-    MRUN_REQUIRE(blocks < (1L << 31), "%s: %d pages are more than a launch takes", name, n);
-    const dim3 grid((unsigned)blocks, (unsigned)kv_heads);
-    const auto launch = [&](auto kernel) {
-        return launch_kernel(kernel, grid, dim3(2 * head_dim), 0, stream, (const unsigned char*)cache, ids, (const int4*)ranges, block_tables,
-                             table_rows, max_blocks, (bf16*)k_out, (bf16*)v_out, kv_heads, page_size, out_page, pages);
-    };
-    MRUN_CHECK_CUDA(head_dim == 64 ? launch(fp4_rows_kernel<64>) : launch(fp4_rows_kernel<128>), name);
-    MRUN_CHECK_LAUNCH(name);
+    return launch_rows(cache, ids, Spans{}, nullptr, 0, 0, k_out, v_out, n, kv_heads, head_dim, page_size, page_size, pages, name, stream);
+}
+
+// `spans` (host memory): int [n, 6], see Span, in ascending order of their pages and without a gap between them; out_page: rows of an output page.
+MRUN_API int mrun_fp4_spans(const void* cache, const int* spans, int n, const int* block_tables, int table_rows, int max_blocks,
+                            void* k_out, void* v_out, int* table, int table_width, int* span_of_row, int kv_heads, int head_dim,
+                            int page_size, int out_page, long pages, cudaStream_t stream) {
+    const char* name = "fp4_spans";
+    MRUN_REQUIRE_FP4(head_dim, page_size, name);
+    MRUN_REQUIRE(out_page > 0 && out_page % FP4_TOKENS == 0, "%s: out_page=%d", name, out_page);
+    MRUN_REQUIRE(n >= 0 && spans && block_tables && (table == nullptr) == (span_of_row == nullptr), "%s: %d spans", name, n);
+    int next = 0;
+    for (int s = 0; s < n; ++s) {
+        const int* v = spans + 6 * s;
+        MRUN_REQUIRE(v[1] >= 0 && v[1] % out_page == 0 && v[2] > v[1] && v[3] == next && v[5] >= 0, "%s: span %d is [%d, %d) at page %d", name, s,
+                     v[1], v[2], v[3]);
+        next += (v[2] - v[1] + out_page - 1) / out_page;
+        MRUN_REQUIRE(table == nullptr || v[1] / out_page + (v[2] - v[1] + out_page - 1) / out_page <= table_width, "%s: table_width=%d", name, table_width);
+    }
+    for (int first = 0; first < n; first += MAX_SPANS) {
+        Spans part = {};
+        part.n = n - first < MAX_SPANS ? n - first : MAX_SPANS;
+        part.index0 = first;
+        part.table = table;
+        part.table_width = table_width;
+        part.span_of_row = span_of_row;
+        for (int s = 0; s < part.n; ++s) {
+            const int* v = spans + 6 * (first + s);
+            part.span[s] = Span{v[0], v[1], v[2], v[3], v[4], v[5]};
+        }
+        const int end = first + part.n < n ? spans[6 * (first + part.n) + 3] : next;
+        if (int rc = launch_rows(cache, nullptr, part, block_tables, table_rows, max_blocks, k_out, v_out, end - part.span[0].page0, kv_heads,
+                                 head_dim, page_size, out_page, pages, name, stream))
+            return rc;
+    }
     return 0;
 }

@@ -499,6 +499,15 @@ class _Pages:
 
 
 @dataclass
+class SegmentView:
+    """A segment as the prompt kernels' tile lists take it; ``slot``: its row of the block tables."""
+    slot: int
+    q_start: int
+    q_len: int
+    pos_start: int
+
+
+@dataclass
 class _View:
     block_tables: torch.Tensor
     max_blocks: int
@@ -520,69 +529,58 @@ FP4_MAX_TOKENS = 256       # tokens of one launch of the decode kernel
 FP4_TILE_KEYS = 128        # keys that its blocks are dealt together
 
 
-def _fp4_tokens(q, q_stride: int, out, cache, group, heads: int, head_dim: int, scale: float, window: int, token_slot, positions,
-                rows, tokens: int, max_kv_len: int) -> None:
-    """Single tokens: those of the step, or the rows ``rows`` of it."""
+def _fp4_tokens(q, q_stride: int, out, cache, group, ctx, heads: int, head_dim: int, scale: float, window: int, rows=None) -> None:
+    """Single tokens: all rows of the step, or those that ``rows`` lists."""
     pages, kv_heads, units, _ = cache.shape
     ratio = heads // kv_heads
     library = _lib.fp4()
     slots, block_heads = _fp4_blocks(library, q.device, head_dim, ratio)
-    longest = max_kv_len if window == 0 else min(max_kv_len, abs(window))
+    longest = ctx.max_kv_len if window == 0 else min(ctx.max_kv_len, abs(window))
     # no more blocks than tiles (a window that does not begin with a tile's first key touches one more)
     tiles_a_token = kv_heads * -(-ratio // block_heads) * (-(-longest // FP4_TILE_KEYS) + (window != 0))
-    scratch_bytes = library.function("mrun_attn_fp4_scratch")
+    tables = group.block_tables
+    tokens = ctx.num_tokens if rows is None else len(rows)
     for first in range(0, tokens, FP4_MAX_TOKENS):
         n = min(FP4_MAX_TOKENS, tokens - first)
         blocks = max(1, min(slots, n * tiles_a_token))
-        scratch = torch.empty(scratch_bytes(blocks, n, head_dim, ratio), dtype=torch.uint8, device=q.device)
-        here = slice(first, first + n)
-        library.call("mrun_attn_fp4_decode", _address(q if rows is not None else q[here]), q_stride,
-                     _address(out if rows is not None else out[here]), _address(cache), _address(group.block_tables),
-                     group.block_tables.shape[0], group.block_tables.shape[1], _address(token_slot[here]), _address(positions[here]),
-                     _address(rows[here] if rows is not None else None), n, heads, kv_heads, head_dim, units * ops.FP4_TOKENS, pages,
-                     scale, window, _address(scratch), blocks, _queue())
+        # the pieces of two pairs a block (sums, maximum and sum a head), and the prefix of tiles
+        scratch = torch.empty(blocks * 2 * block_heads * (head_dim + 2) + n + 1, dtype=torch.float32, device=q.device)
+        if rows is None:
+            listed, at = None, first
+        else:
+            listed, at = (ctypes.c_int * n)(*rows[first:first + n]), 0
+        library.call("mrun_attn_fp4_decode", q.data_ptr() + 2 * at * q_stride, q_stride, out.data_ptr() + 2 * at * heads * head_dim,
+                     cache.data_ptr(), tables.data_ptr(), tables.shape[0], tables.shape[1], ctx.token_slot.data_ptr() + 4 * at,
+                     ctx.positions.data_ptr() + 4 * at, None if listed is None else ctypes.addressof(listed), n, heads, kv_heads, head_dim,
+                     units * ops.FP4_TOKENS, pages, scale, window, scratch.data_ptr(), blocks, _queue())
 
 
 def _fp4_portions(ctx, window: int, short: int):
-    """What a step's prompt portions need, made once per step: ``(rows, positions, slots)`` of the tokens of its short segments and
-    their number, and for the others the ranges of tokens to read back, a step context over them and their block tables."""
+    """What a step's prompt portions need, made once per step: the rows of its short segments, and for the longer ones the spans of tokens
+    to read back, their pages, and a step context and block tables over these, which the first layer's call fills."""
     key = ("fp4_portions", window, short)
     found = ctx.shared.get(key)
     if found is not None:
         return found
-    few, many = [], []
+    rows, spans, longer, pages, width = [], [], [], 0, 0
     for seg in ctx.segments:
-        (few if seg.q_len <= short else many).append(seg)
-    rows = [seg.q_start + i for seg in few for i in range(seg.q_len)]
-    positions = [seg.pos_start + i for seg in few for i in range(seg.q_len)]
-    slots = [seg.slot for seg in few for _ in range(seg.q_len)]
-    ranges, tables = [], []
-    for seg in many:
+        if seg.q_len <= short:
+            rows.extend(range(seg.q_start, seg.q_start + seg.q_len))
+            continue
         end = seg.pos_start + seg.q_len
-        first = _first_visible(seg.pos_start, window) // FP4_SCRATCH_ROWS
-        table = [-1] * first
-        for block in range(first, -(-end // FP4_SCRATCH_ROWS)):
-            table.append(len(ranges))
-            ranges.append((seg.slot, block * FP4_SCRATCH_ROWS, min(FP4_SCRATCH_ROWS, end - block * FP4_SCRATCH_ROWS), 0))
-        tables.append(table)
-    width = max((len(table) for table in tables), default=0)
-    token_row = np.full(ctx.num_tokens, -1, dtype=np.int32)
-    for i, seg in enumerate(many):
-        token_row[seg.q_start:seg.q_start + seg.q_len] = i
-    parts = [np.asarray(ranges, dtype=np.int32).reshape(-1), np.asarray(rows, dtype=np.int32), np.asarray(positions, dtype=np.int32),
-             np.asarray(slots, dtype=np.int32), token_row,
-             np.asarray([table + [-1] * (width - len(table)) for table in tables], dtype=np.int32).reshape(-1)]
-    sent = ctx.upload(np.concatenate(parts))
-    at = np.cumsum([0] + [part.size for part in parts]).tolist()
-    take = lambda i: sent[at[i]:at[i + 1]]
-    singles = (take(1), take(2), take(3), len(rows))
-    longer = None
-    if many:
-        segments = [dataclasses.replace(seg, slot=i) for i, seg in enumerate(many)]
-        inner = dataclasses.replace(ctx, segments=segments, num_segments=len(segments), token_slot=take(4), shared={},
-                                    max_q_len=max(seg.q_len for seg in many), page_size=FP4_SCRATCH_ROWS)
-        longer = (take(0).view(-1, 4), inner, _View(take(5).view(len(many), width), width))
-    found = ctx.shared[key] = (singles, longer)
+        first = _first_visible(seg.pos_start, window) // FP4_SCRATCH_ROWS * FP4_SCRATCH_ROWS
+        longer.append(SegmentView(len(spans), seg.q_start, seg.q_len, seg.pos_start))
+        spans.append((seg.slot, first, end, pages, seg.q_start, seg.q_len))
+        pages += -(-(end - first) // FP4_SCRATCH_ROWS)
+        width = max(width, -(-end // FP4_SCRATCH_ROWS))
+    if not spans:
+        found = ctx.shared[key] = (rows, None)
+        return found
+    own = torch.empty(ctx.num_tokens + len(spans) * width, dtype=torch.int32, device=ctx.positions.device)
+    span_of_row, table = own[:ctx.num_tokens], own[ctx.num_tokens:].view(len(spans), width)
+    inner = dataclasses.replace(ctx, segments=longer, num_segments=len(longer), token_slot=span_of_row, shared={},
+                                max_q_len=max(seg.q_len for seg in longer), page_size=FP4_SCRATCH_ROWS, real_tokens=ctx.num_tokens)
+    found = ctx.shared[key] = (rows, (spans, pages, table, span_of_row, inner, _View(table, width)))
     return found
 
 
@@ -618,17 +616,19 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
     for name, t in (("block_tables", group.block_tables), ("positions", ctx.positions), ("token_slot", ctx.token_slot)):
         ops._check(t, name, torch.int32)
     if ctx.all_decode:
-        _fp4_tokens(q, q_stride, out, cache, group, heads, head_dim, scale, window, ctx.token_slot, ctx.positions, None, tokens, ctx.max_kv_len)
+        _fp4_tokens(q, q_stride, out, cache, group, ctx, heads, head_dim, scale, window)
         return out
     if tokens > ctx.real_tokens:
         out[ctx.real_tokens:].zero_()
     # the prompt kernels over tensor cores take up to 64 query heads a kv head
     short = FP4_SHORT if heads // kv_heads <= 64 else tokens
-    (rows, positions, slots, n), longer = _fp4_portions(ctx, window, short)
-    if n:
-        _fp4_tokens(q, q_stride, out, cache, group, heads, head_dim, scale, window, slots, positions, rows, n, ctx.max_kv_len)
+    filled = ("fp4_portions", window, short) in ctx.shared
+    rows, longer = _fp4_portions(ctx, window, short)
+    if rows:
+        _fp4_tokens(q, q_stride, out, cache, group, ctx, heads, head_dim, scale, window, rows)
     if longer is not None:
-        ranges, inner, view = longer
-        k, v = ops.fp4_ranges(cache, head_dim, group.block_tables, ranges, FP4_SCRATCH_ROWS)
+        spans, n, table, span_of_row, inner, view = longer
+        k, v = ops.fp4_spans(cache, head_dim, group.block_tables, spans, n, FP4_SCRATCH_ROWS, None if filled else table,
+                             None if filled else span_of_row)
         paged_attention(q, q_stride, out, _Pages(k, v), view, inner, heads, scale, window)
     return out

@@ -315,12 +315,13 @@ def qk_norm_rope_cache_fp4(qkv: torch.Tensor, heads: int, kv_heads: int, head_di
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("rot", rot)):
         if t is not None:
             _check(t, name, torch.float32)
-    q, stride = qkv[:, :heads * head_dim], qkv.shape[1]
-    if q_out is not None:
+    if q_out is None:
+        q, stride = qkv[:, :heads * head_dim], qkv.shape[1]
+    else:
         _check(q_out, "q_out", torch.bfloat16, dense=False)
         q, stride = q_out, _strided_rows(q_out, "q_out")
-    _lib.fp4().call("mrun_qk_norm_rope_cache_fp4", _address(qkv), _address(q), stride, _address(q_weight), _address(k_weight), eps,
-                    _address(rot), rotary_dim if rot is not None else 0, _address(slots), _address(cache if slots is not None else None),
+    _lib.fp4().call("mrun_qk_norm_rope_cache_fp4", qkv.data_ptr(), q.data_ptr(), stride, _address(q_weight), _address(k_weight), eps,
+                    _address(rot), rotary_dim if rot is not None else 0, _address(slots), cache.data_ptr() if slots is not None else None,
                     tokens, heads, kv_heads, head_dim, page_size, pages, _queue())
     return q
 
@@ -332,25 +333,36 @@ def fp4_pages(cache: torch.Tensor, head_dim: int, pages: torch.Tensor):
         raise KernelError(f"fp4_pages: pages is {tuple(pages.shape)}, expected a list")
     held, kv_heads, page_size = check_fp4_cache(cache, head_dim)
     _check(cache, "cache", torch.uint8); _check(pages, "pages", torch.int32)
-    k = torch.empty((pages.numel(), kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=cache.device)
-    v = torch.empty_like(k)
-    _lib.fp4().call("mrun_fp4_rows", _address(cache), _address(pages), _address(None), _address(None), 0, 0, _address(k), _address(v),
-                    pages.numel(), kv_heads, head_dim, page_size, page_size, held, _queue())
+    n = pages.shape[0]
+    k, v = torch.empty((2, n, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=cache.device).unbind(0)
+    _lib.fp4().call("mrun_fp4_pages", cache.data_ptr(), pages.data_ptr(), k.data_ptr(), v.data_ptr(), n, kv_heads, head_dim, page_size, held,
+                    _queue())
     return k, v
 
 
-def fp4_ranges(cache: torch.Tensor, head_dim: int, block_tables: torch.Tensor, ranges: torch.Tensor, rows: int):
-    """(keys, values): bfloat16 [n, kv heads, rows, head_dim] each.  Entry i holds tokens ``ranges[i][1]`` .. (a multiple of 16) of the
-    request in row ``ranges[i][0]`` of the block tables: its first ``ranges[i][2]`` rows, then zeros (int32 [n, 4], the last
-    unused).  ``rows``: a multiple of 16."""
-    if ranges.dim() != 2 or ranges.shape[1] != 4 or block_tables.dim() != 2:
-        raise KernelError(f"fp4_ranges: ranges {tuple(ranges.shape)}, block_tables {tuple(block_tables.shape)}")
+def fp4_spans(cache: torch.Tensor, head_dim: int, block_tables: torch.Tensor, spans, pages: int, rows: int, table: Optional[torch.Tensor] = None,
+              span_of_row: Optional[torch.Tensor] = None):
+    """(keys, values): bfloat16 [pages, kv heads, rows, head_dim] each, the contexts of several requests one after the other.  ``spans``: a
+    tuple (block-table row, first token, end, first output page, first row of the step, rows of the step) for each; a span begins with a
+    page's first row, and rows behind its end are zeros.  ``table`` (int32 [spans, blocks]) gets the spans' own block tables over the
+    output, ``span_of_row`` (int32 [rows of the step]) the span of their rows of the step."""
+    if block_tables.dim() != 2:
+        raise KernelError(f"fp4_spans: block_tables {tuple(block_tables.shape)}")
     held, kv_heads, page_size = check_fp4_cache(cache, head_dim)
-    _check(cache, "cache", torch.uint8); _check(ranges, "ranges", torch.int32); _check(block_tables, "block_tables", torch.int32)
-    k = torch.empty((ranges.shape[0], kv_heads, rows, head_dim), dtype=torch.bfloat16, device=cache.device)
-    v = torch.empty_like(k)
-    _lib.fp4().call("mrun_fp4_rows", _address(cache), _address(None), _address(ranges), _address(block_tables), block_tables.shape[0],
-                    block_tables.shape[1], _address(k), _address(v), ranges.shape[0], kv_heads, head_dim, page_size, rows, held, _queue())
+    _check(cache, "cache", torch.uint8); _check(block_tables, "block_tables", torch.int32)
+    if (table is None) != (span_of_row is None) or (table is not None and (table.dim() != 2 or table.shape[0] != len(spans))):
+        raise KernelError(f"fp4_spans: table {None if table is None else tuple(table.shape)} for {len(spans)} spans")
+    for name, t in (("table", table), ("span_of_row", span_of_row)):
+        if t is not None:
+            _check(t, name, torch.int32)
+    for span in spans:
+        if span[2] - span[1] + span[3] * rows > pages * rows or (table is not None and span[4] + span[5] > span_of_row.numel()):
+            raise KernelError(f"fp4_spans: span {span} does not fit {pages} pages of {rows} rows")
+    k, v = torch.empty((2, pages, kv_heads, rows, head_dim), dtype=torch.bfloat16, device=cache.device).unbind(0)
+    flat = (ctypes.c_int * (6 * len(spans)))(*[value for span in spans for value in span])
+    _lib.fp4().call("mrun_fp4_spans", cache.data_ptr(), ctypes.addressof(flat), len(spans), block_tables.data_ptr(), block_tables.shape[0],
+                    block_tables.shape[1], k.data_ptr(), v.data_ptr(), _address(table), 0 if table is None else table.shape[1],
+                    _address(span_of_row), kv_heads, head_dim, page_size, rows, held, _queue())
     return k, v
 
 
