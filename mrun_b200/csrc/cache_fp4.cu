@@ -16,13 +16,17 @@ using bf16 = __nv_bfloat16;
 //
 // A key is quantised from its unrounded value, and which side of a border between two codes a value
 // falls on decides a whole step of the code.  So that the codes are those of the formula and do not depend on
-// the order of a sum, a key's norm and rotation are computed in 64 bits (B200 has 64 such lanes a
-// multiprocessor beside 128 of 32 bits; a key is an eighth to a third of a row).  A value is a bfloat16 and its quotient by a
-// scale of 4 bits is told from every border (at most 3 bits) in 32 bits.
+// the order of a sum, a key is computed in 32 bits with a bound of its error, quantised at both ends of the bound, and where
+// the two differ (one head in two hundred) computed again in 64 bits.  In 64 bits throughout the kernel took 32 us for
+// 2,048 tokens of 32 + 8 + 8 heads of 128.
+// A value is a bfloat16: its quotient by a scale of 4 bits is a border (at most 3 bits) exactly or 2^-9 away from it.
+//
+// A block takes 256 threads' worth of the heads of one token, D / 8 lanes a head, eight features a lane: the token's cosines and sines
+// are read once into the first-level cache.
 // ------------------------------------------------------------------------------------------
-constexpr int HEADS_PER_GROUP = 4;      // heads of a token that a group of lanes takes, one after the other
+constexpr int STORE_THREADS = 256;
 
-// The byte of the scale nearest to `wanted` (>= 0), ties to the even byte.  `wanted` has a bit set below
+// The byte of the scale nearest to `wanted` (0 .. 10,240), ties to the even byte.  `wanted` has a bit set below
 // its 24 wherever something was cut off, so that this is the only rounding.
 __device__ __forceinline__ unsigned scale_byte(float wanted) {
     const unsigned bits = __float_as_uint(wanted);
@@ -47,18 +51,25 @@ __device__ __forceinline__ float cut_sticky(double v) {
     return (double)f == v ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
 
-// The codes (8 features a lane, four bytes) and the scale of the 16 features that two neighbouring lanes hold.
-__device__ __forceinline__ unsigned quantise(const double (&x)[8], unsigned mask, unsigned& scale) {
-    double largest = 0.0;
-    bool finite = true;
+// The largest magnitude of the 16 features that two neighbouring lanes hold; `finite`: none is a NaN or an infinity.
+template <typename F> __device__ __forceinline__ F largest_of(const F (&x)[8], unsigned mask, bool& finite) {
+    F largest = 0;
+    finite = true;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const double a = fabs(x[e]);
-        finite = finite && a < INFINITY;
-        largest = fmax(largest, a);
+        const F a = x[e] < 0 ? -x[e] : x[e];
+        finite = finite && a < (F)INFINITY;
+        largest = a > largest ? a : largest;
     }
-    largest = fmax(largest, __shfl_xor_sync(mask, largest, 1));
+    const F other = __shfl_xor_sync(mask, largest, 1);
     finite = __shfl_xor_sync(mask, (int)finite, 1) && finite;
+    return other > largest ? other : largest;
+}
+
+// The codes (8 features a lane, four bytes) and the scale of the 16 features that two neighbouring lanes hold: of any doubles,
+__device__ __forceinline__ unsigned quantise(const double (&x)[8], unsigned mask, unsigned& scale) {
+    bool finite;
+    const double largest = largest_of(x, mask, finite);
     scale = finite ? scale_byte(cut_sticky(fmin(largest / 6.0, 10240.0))) : (unsigned)FP4_NAN_SCALE;
     if (!finite) return 0u;
     const double s = scale_value(scale);
@@ -77,143 +88,233 @@ __device__ __forceinline__ unsigned quantise(const double (&x)[8], unsigned mask
     }
     return out;
 }
+
+// of floats that hold bfloat16 values,
 __device__ __forceinline__ unsigned quantise(const float (&x)[8], unsigned mask, unsigned& scale) {
-    float largest = 0.f;
-    bool finite = true;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float a = fabsf(x[e]);
-        finite = finite && a < INFINITY;
-        largest = fmaxf(largest, a);
-    }
-    largest = fmaxf(largest, __shfl_xor_sync(mask, largest, 1));
-    finite = __shfl_xor_sync(mask, (int)finite, 1) && finite;
+    bool finite;
+    const float largest = largest_of(x, mask, finite);
     scale = finite ? scale_byte(fminf(__fdiv_rn(largest, 6.f), 10240.f)) : (unsigned)FP4_NAN_SCALE;
     const float s = scale_value(scale);
     if (!(s > 0.f)) return 0u;
+    const float inverse = __fdiv_rn(1.f, s);
     unsigned out = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) out |= codes_of(__fdiv_rn(x[e], s), __fdiv_rn(x[e + 1], s)) << (4 * e);
+    for (int e = 0; e < 8; e += 2) {
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            // the quotient to 12 bits: one that is a border exactly comes out as it
+            const float y = __fmul_rn(fminf(fmaxf(x[e + i], -1e6f), 1e6f), inverse), wide = __fmul_rn(y, 4097.f);
+            f[i] = __fsub_rn(wide, __fsub_rn(wide, y));
+        }
+        out |= codes_of(f[0], f[1]) << (4 * e);
+    }
     return out;
 }
 
-// Norm and rotation of one head, eight features a lane, in 32 or 64 bits.  `other_lane`: the lane that holds the
-// rotation's partners; STAGED: they are fetched one by one through `stage`, a row of D of its own.
-template <typename F, int D, bool STAGED>
-__device__ __forceinline__ void norm_rotate(F (&v)[8], const float* __restrict__ weight, float eps, const float2* __restrict__ cs,
-                                            int half, int part, unsigned mask, F* stage) {
-    constexpr int LANES = D / 8;
-    if (weight) {
-        F ss = 0;
+// and of floats that are within `off` of the values meant.  `sure`: neither the scale nor a code depends on where within.
+__device__ __forceinline__ unsigned quantise(const float (&x)[8], float off, unsigned mask, unsigned& scale, bool& sure) {
+    bool finite;
+    const float largest = largest_of(x, mask, finite);
+    scale = scale_byte(fminf((largest + off) * (1.f / 6.f) * 1.000001f, 10240.f));
+    sure = finite && off < INFINITY && scale == scale_byte(fminf(fmaxf(largest - off, 0.f) * (1.f / 6.f) * 0.999999f, 10240.f));
+    const float s = scale_value(scale), inverse = s > 0.f ? 1.f / s : 0.f, away = off * inverse * 1.000001f;
+    unsigned low = 0, high = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const F inv = sizeof(F) == 4 ? (F)rsqrtf((float)ss / (float)D + eps) : (F)rsqrt((double)ss / (double)D + (double)eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * (F)weight[part * 8 + e];
+    for (int e = 0; e < 8; e += 2) {
+        // three roundings of the quotient and its ends: 2^-22 of it
+        const float y0 = x[e] * inverse, y1 = x[e + 1] * inverse;
+        const float a0 = fmaf(fabsf(y0), 4.8e-7f, away), a1 = fmaf(fabsf(y1), 4.8e-7f, away);
+        low |= codes_of(y0 - a0, y1 - a1) << (4 * e);
+        high |= codes_of(y0 + a0, y1 + a1) << (4 * e);
     }
-    if (half == 0) return;
-    if constexpr (STAGED) {
-        __syncwarp(mask);
+    sure = sure && low == high;
+    return low;
+}
+
+// Eight floats of `src`, on 16 bytes.
+__device__ __forceinline__ void load8(float (&v)[8], const float* __restrict__ src) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+// What a lane needs of the norm and the rotation of its eight features.  Pairs (j, j + half): with a half of a multiple of eight a
+// lane's partners are the eight features of another lane, and it holds their cosines and sines (these with their sign).
+struct Turn {
+    int partner;            // the lane of the group, itself where nothing turns
+    bool turns;
+    float c[8], s[8];
+};
+
+template <typename F, int D> __device__ __forceinline__ F sum_of_squares(const F (&v)[8], unsigned mask) {
+    F ss = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) stage[part * 8 + e] = v[e];
-        __syncwarp(mask);
+    for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int j = part * 8 + e;
-            if (j < half) v[e] = v[e] * (F)cs[j].x - stage[j + half] * (F)cs[j].y;
-            else if (j < 2 * half) v[e] = v[e] * (F)cs[j - half].x + stage[j - half] * (F)cs[j - half].y;
-        }
-    } else {
-        // rotary_dim is a multiple of 16: a lane's partners are another lane's eight features
-        const int away = half / 8;
-        const bool low = part < away, turns = part < 2 * away;
-        const int partner = turns ? (low ? part + away : part - away) : part;
-        const int base = (int)(threadIdx.x & 31) - part;
+    for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+    return ss;
+}
+
+template <typename F, int D>
+__device__ __forceinline__ void norm(F (&v)[8], const float (&weight)[8], float eps, unsigned mask) {
+    const F ss = sum_of_squares<F, D>(v, mask);
+    const F inv = sizeof(F) == 4 ? (F)rsqrtf((float)ss / (float)D + eps) : (F)rsqrt((double)ss / (double)D + (double)eps);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const F other = __shfl_sync(mask, v[e], base + partner);
-            if (turns) {
-                const float2 c = cs[(low ? part : partner) * 8 + e];
-                v[e] = low ? v[e] * (F)c.x - other * (F)c.y : v[e] * (F)c.x + other * (F)c.y;
-            }
-        }
+    for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * (F)weight[e];
+}
+
+// Returns the largest |first| + |second| of what is added.
+template <typename F>
+__device__ __forceinline__ F rotate(F (&v)[8], const Turn& turn, unsigned mask, int part) {
+    const int base = (int)(threadIdx.x & 31) - part;
+    F widest = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const F other = __shfl_sync(mask, v[e], base + turn.partner);
+        const F both = (v[e] < 0 ? -v[e] : v[e]) + (other < 0 ? -other : other);
+        widest = both > widest ? both : widest;
+        if (turn.turns) v[e] = v[e] * (F)turn.c[e] + other * (F)turn.s[e];
+    }
+    return widest;
+}
+
+// The rotation with the partners fetched one by one through `stage`, a row of D of the group's own.
+template <typename F>
+__device__ __forceinline__ void rotate_staged(F (&v)[8], const float2* __restrict__ cs, int half, unsigned mask, int part, F* stage) {
+    __syncwarp(mask);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) stage[part * 8 + e] = v[e];
+    __syncwarp(mask);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int j = part * 8 + e;
+        if (j < half) v[e] = v[e] * (F)cs[j].x - stage[j + half] * (F)cs[j].y;
+        else if (j < 2 * half) v[e] = v[e] * (F)cs[j - half].x + stage[j - half] * (F)cs[j - half].y;
     }
 }
 
+// STAGED: rotary sizes that are no multiple of 16, and weights or tables off 16 bytes; keys in 64 bits throughout.
 template <int D, bool STAGED>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(STORE_THREADS)
 qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, long q_stride,
                               const float* __restrict__ q_weight, const float* __restrict__ k_weight, float eps,
                               const float2* __restrict__ rot, int half, const int* __restrict__ slots,
-                              unsigned char* __restrict__ cache, int tokens, int heads, int kv_heads, int page_size, long pages) {
+                              unsigned char* __restrict__ cache, int heads, int kv_heads, int page_size, long pages, int blocks_per_token) {
     using Unit = Fp4Unit<D>;
-    constexpr int LANES = D / 8;
-    __shared__ double stage_all[STAGED ? 256 / LANES * D : 1];
+    constexpr int LANES = D / 8, GROUPS = STORE_THREADS / LANES;
+    __shared__ double stage_all[STAGED ? GROUPS * D : 1];
     const int per_token = heads + 2 * kv_heads;
-    const int groups_per_token = (per_token + HEADS_PER_GROUP - 1) / HEADS_PER_GROUP;
-    const long group = ((long)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
-    const int part = threadIdx.x % LANES;
-    if (group >= (long)tokens * groups_per_token) return;          // all lanes of a group together
-    const int t = (int)(group / groups_per_token);
-    const int head0 = (int)(group - (long)t * groups_per_token) * HEADS_PER_GROUP;
-    const int head1 = min(per_token, head0 + HEADS_PER_GROUP);
+    const int t = blockIdx.x / blocks_per_token, chunk = blockIdx.x - t * blocks_per_token;
+    const int group = threadIdx.x / LANES, part = threadIdx.x % LANES, head = chunk * GROUPS + group;
+    if (head >= per_token) return;                                 // all lanes of a group together
     const unsigned lane = threadIdx.x & 31;
     const unsigned mask = ((1u << LANES) - 1u) << (lane & ~(unsigned)(LANES - 1));
-    double* stage = stage_all + (STAGED ? threadIdx.x / LANES * D : 0);
-    const float2* cs = rot + (size_t)t * half;
+    const bool is_q = head < heads, is_k = !is_q && head < heads + kv_heads;
 
+    const uint4 raw = *reinterpret_cast<const uint4*>(qkv + ((size_t)t * per_token + head) * D + part * 8);
     // a slot outside the cache (a padding row's -1) writes nothing
-    const int slot = slots ? slots[t] : -1;
-    const int page = slot >= 0 ? slot / page_size : -1;
-    const bool writes = page >= 0 && page < pages;
-    const int off = slot - page * page_size, r = off & (FP4_TOKENS - 1);
-    const int units = page_size / FP4_TOKENS;
-
-    for (int head = head0; head < head1; ++head) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(qkv + ((size_t)t * per_token + head) * D + part * 8);
-        float x[8];
-        {
-            const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    const int slot = is_q || slots == nullptr ? -1 : slots[t];
+    const float* weights = is_q ? q_weight : k_weight;
+    const bool normed = weights != nullptr && (is_q || is_k), turned = half > 0 && (is_q || is_k);
+    float weight[8];
+    if (normed) {
+        if constexpr (STAGED) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = __bfloat1622float2(pairs[e]);
-                x[2 * e] = f.x; x[2 * e + 1] = f.y;
+            for (int e = 0; e < 8; ++e) weight[e] = weights[part * 8 + e];
+        } else {
+            load8(weight, weights + part * 8);
+        }
+    }
+    const float2* cs = rot + (size_t)t * half;
+    Turn turn;
+    if (!STAGED && turned) {
+        const int away = half / 8;
+        const bool low = part < away;
+        turn.turns = part < 2 * away;
+        turn.partner = turn.turns ? (low ? part + away : part - away) : part;
+        if (turn.turns) {
+            float two[2][8];
+            const float* src = reinterpret_cast<const float*>(cs + (low ? part : turn.partner) * 8);
+            load8(two[0], src);
+            load8(two[1], src + 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                turn.c[e] = two[e / 4][e % 4 * 2];
+                turn.s[e] = low ? -two[e / 4][e % 4 * 2 + 1] : two[e / 4][e % 4 * 2 + 1];
             }
         }
-        if (head < heads) {
-            norm_rotate<float, D, STAGED>(x, q_weight, eps, cs, half, part, mask, reinterpret_cast<float*>(stage));
-            uint4 packed;
-            __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(&packed);
+    }
+    double* stage = stage_all + (STAGED ? group * D : 0);
+    float x[8];
+    {
+        const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) out[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
-            *reinterpret_cast<uint4*>(q_out + (size_t)t * q_stride + (size_t)head * D + part * 8) = packed;
-            continue;
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = __bfloat1622float2(pairs[e]);
+            x[2 * e] = f.x; x[2 * e + 1] = f.y;
         }
-        if (!writes) continue;
-        const bool is_k = head < heads + kv_heads;
-        const int kv_head = is_k ? head - heads : head - heads - kv_heads;
-        unsigned char* unit = cache + (((size_t)page * kv_heads + kv_head) * units + off / FP4_TOKENS) * Unit::BYTES;
-        unsigned scale, codes;
-        if (is_k) {
+    }
+    if (is_q) {
+        if (normed) norm<float, D>(x, weight, eps, mask);
+        if (turned) {
+            if constexpr (STAGED) rotate_staged(x, cs, half, mask, part, reinterpret_cast<float*>(stage));
+            else rotate(x, turn, mask, part);
+        }
+        uint4 packed;
+        __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        *reinterpret_cast<uint4*>(q_out + (size_t)t * q_stride + (size_t)head * D + part * 8) = packed;
+        return;
+    }
+    const int page = slot >= 0 ? slot / page_size : -1;
+    if (page < 0 || page >= pages) return;
+    const int off = slot - page * page_size, r = off & (FP4_TOKENS - 1);
+    const int kv_head = is_k ? head - heads : head - heads - kv_heads;
+    unsigned char* unit = cache + (((size_t)page * kv_heads + kv_head) * (page_size / FP4_TOKENS) + off / FP4_TOKENS) * Unit::BYTES;
+    unsigned scale, codes;
+    if (is_k && (normed || turned)) {
+        bool sure = false;
+        if constexpr (!STAGED) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[e];
+            if (normed) norm<float, D>(y, weight, eps, mask);
+            float widest = 0.f;
+            if (turned) {
+                widest = rotate(y, turn, mask, part);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) widest = fmaxf(widest, fabsf(y[e]));
+            }
+            widest = fmaxf(widest, __shfl_xor_sync(mask, widest, 1));
+            // The sum of squares is off by 12 roundings at most and half of that under the root, the root by 2^-22, the two products and the
+            // two of the rotation by one each: less than 2^-20 of |first| + |second|.
+            codes = quantise(y, widest * 1.9073486328125e-06f, mask, scale, sure);
+            sure = __all_sync(mask, sure);
+        }
+        if (!sure) {
             double y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = x[e];
-            norm_rotate<double, D, STAGED>(y, k_weight, eps, cs, half, part, mask, stage);
+            if (normed) norm<double, D>(y, weight, eps, mask);
+            if (turned) {
+                if constexpr (STAGED) rotate_staged(y, cs, half, mask, part, stage);
+                else rotate(y, turn, mask, part);
+            }
             codes = quantise(y, mask, scale);
-        } else {
-            codes = quantise(x, mask, scale);
         }
-        // eight features are four bytes of one piece: D = 128 has pieces of eight bytes, D = 64 of four
-        *reinterpret_cast<unsigned*>(unit + (is_k ? Unit::k_code(r, part * 4) : Unit::v_code(r, part * 4))) = codes;
-        if ((part & 1) == 0) unit[is_k ? Unit::k_scale(r, part / 2) : Unit::v_scale(r, part / 2)] = (unsigned char)scale;
+    } else {
+        codes = quantise(x, mask, scale);
     }
+    // eight features are four bytes of one piece: D = 128 has pieces of eight bytes, D = 64 of four
+    *reinterpret_cast<unsigned*>(unit + (is_k ? Unit::k_code(r, part * 4) : Unit::v_code(r, part * 4))) = codes;
+    if ((part & 1) == 0) unit[is_k ? Unit::k_scale(r, part / 2) : Unit::v_scale(r, part / 2)] = (unsigned char)scale;
 }
 
 // ------------------------------------------------------------------------------------------
 // Reading back into rows [page, kv head, row, :] of bfloat16 keys and values (exact: a value has at most 6
-// significant bits).  A block takes 16 rows of one kv head, a thread eight features of a key and of a value.
+// significant bits).  A block takes 16 rows of one kv head, a thread sixteen features (a group) of a key and of a value.
 //   ids      output page i is cache page ids[i]
 //   spans    the output pages hold the tokens of spans of requests, one span's pages after the other's: tokens `first` .. `end` (a
 //            span begins with an output page's first row) of the request in block-table row `row`; rows behind `end`
@@ -240,12 +341,12 @@ struct Spans {
 };
 
 template <int D>
-__global__ void __launch_bounds__(2 * D)
+__global__ void __launch_bounds__(D)
 fp4_rows_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ ids, const __grid_constant__ Spans spans,
                 const int* __restrict__ block_tables, int table_rows, int max_blocks, bf16* __restrict__ k_out, bf16* __restrict__ v_out,
                 int kv_heads, int page_size, int out_page, long pages) {
     using Unit = Fp4Unit<D>;
-    constexpr int LANES = D / 8;
+    constexpr int LANES = D / FP4_GROUP;
     const int units_out = out_page / FP4_TOKENS, units_in = page_size / FP4_TOKENS;
     int i = blockIdx.x / units_out;
     const int unit_out = blockIdx.x - i * units_out, kv_head = blockIdx.y;
@@ -268,42 +369,54 @@ fp4_rows_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
             const int before = span.first / out_page;
             if (threadIdx.x == 0) table[before + in_span] = i;
             if (in_span == 0) {
-                for (int b = threadIdx.x; b < before; b += 2 * D) table[b] = -1;
-                for (int b = before + (span.end - span.first + out_page - 1) / out_page + threadIdx.x; b < spans.table_width; b += 2 * D) table[b] = -1;
-                for (int r0 = threadIdx.x; r0 < span.rows; r0 += 2 * D) spans.span_of_row[span.row0 + r0] = spans.index0 + s;
+                for (int b = threadIdx.x; b < before; b += D) table[b] = -1;
+                for (int b = before + (span.end - span.first + out_page - 1) / out_page + threadIdx.x; b < spans.table_width; b += D) table[b] = -1;
+                for (int r0 = threadIdx.x; r0 < span.rows; r0 += D) spans.span_of_row[span.row0 + r0] = spans.index0 + s;
             }
         }
     }
-    uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    uint4 out[2][2] = {};
     if (page >= 0 && page < pages && r < rows) {
         const unsigned char* unit = cache + ((size_t)(page * kv_heads + kv_head) * units_in + unit_in) * Unit::BYTES;
+        unsigned codes[2][2];
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            const unsigned codes = *reinterpret_cast<const unsigned*>(unit + (kv ? Unit::v_code(r, part * 4) : Unit::k_code(r, part * 4)));
-            const float s = scale_value(unit[kv ? Unit::v_scale(r, part / 2) : Unit::k_scale(r, part / 2)]);
-            __nv_bfloat162* pairs = reinterpret_cast<__nv_bfloat162*>(&out[kv]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const unsigned h = half2_of_codes((codes >> (8 * e)) & 0xFFu);
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                pairs[e] = __floats2bfloat162_rn(f.x * s, f.y * s);
-            }
+        for (int h = 0; h < 2; ++h) {
+            codes[0][h] = *reinterpret_cast<const unsigned*>(unit + Unit::k_code(r, part * 8 + h * 4));
+            codes[1][h] = *reinterpret_cast<const unsigned*>(unit + Unit::v_code(r, part * 8 + h * 4));
         }
+        const float scale[2] = {scale_value(unit[Unit::k_scale(r, part)]), scale_value(unit[Unit::v_scale(r, part)])};
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                __nv_bfloat162* pairs = reinterpret_cast<__nv_bfloat162*>(&out[kv][h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned two = half2_of_codes((codes[kv][h] >> (8 * e)) & 0xFFu);
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+                    pairs[e] = __floats2bfloat162_rn(f.x * scale[kv], f.y * scale[kv]);
+                }
+            }
     }
     const size_t row = ((size_t)i * kv_heads + kv_head) * out_page + unit_out * FP4_TOKENS + r;
-    *reinterpret_cast<uint4*>(k_out + row * D + part * 8) = out[0];
-    *reinterpret_cast<uint4*>(v_out + row * D + part * 8) = out[1];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        *reinterpret_cast<uint4*>(k_out + row * D + part * FP4_GROUP + h * 8) = out[0][h];
+        *reinterpret_cast<uint4*>(v_out + row * D + part * FP4_GROUP + h * 8) = out[1][h];
+    }
 }
 
 template <int D>
 cudaError_t launch_store(const void* qkv, void* q_out, long q_stride, const float* q_weight, const float* k_weight, float eps,
                          const float* rot, int rotary_dim, const int* slots, void* cache, int tokens, int heads, int kv_heads,
                          int page_size, long pages, cudaStream_t stream) {
-    const long groups = (long)tokens * ((heads + 2 * kv_heads + HEADS_PER_GROUP - 1) / HEADS_PER_GROUP);
-    const dim3 grid((unsigned)((groups * (D / 8) + 255) / 256));
-    return launch_kernel(rotary_dim % 16 ? qk_norm_rope_cache_fp4_kernel<D, true> : qk_norm_rope_cache_fp4_kernel<D, false>, grid,
-                         dim3(256), 0, stream, (const bf16*)qkv, (bf16*)q_out, q_stride, q_weight, k_weight, eps, (const float2*)rot,
-                         rotary_dim / 2, slots, (unsigned char*)cache, tokens, heads, kv_heads, page_size, pages);
+    constexpr int GROUPS = STORE_THREADS / (D / 8);
+    const int blocks_per_token = (heads + 2 * kv_heads + GROUPS - 1) / GROUPS;
+    const bool staged = rotary_dim % 16 || (((uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)rot) & 15);
+    return launch_kernel(staged ? qk_norm_rope_cache_fp4_kernel<D, true> : qk_norm_rope_cache_fp4_kernel<D, false>,
+                         dim3((unsigned)tokens * (unsigned)blocks_per_token), dim3(STORE_THREADS), 0, stream, (const bf16*)qkv, (bf16*)q_out, q_stride,
+                         q_weight, k_weight, eps, (const float2*)rot, rotary_dim / 2, slots, (unsigned char*)cache, heads, kv_heads, page_size,
+                         pages, blocks_per_token);
 }
 
 int launch_rows(const void* cache, const int* ids, const Spans& spans, const int* block_tables, int table_rows, int max_blocks, void* k_out,
@@ -315,7 +428,7 @@ int launch_rows(const void* cache, const int* ids, const Spans& spans, const int
     MRUN_REQUIRE(blocks < (1L << 31), "%s: %d pages are more than a launch takes", name, n);
     const dim3 grid((unsigned)blocks, (unsigned)kv_heads);
     const auto launch = [&](auto kernel) {
-        return launch_kernel(kernel, grid, dim3(2 * head_dim), 0, stream, (const unsigned char*)cache, ids, spans, block_tables, table_rows,
+        return launch_kernel(kernel, grid, dim3(head_dim), 0, stream, (const unsigned char*)cache, ids, spans, block_tables, table_rows,
                              max_blocks, (bf16*)k_out, (bf16*)v_out, kv_heads, page_size, out_page, pages);
     };
     MRUN_CHECK_CUDA(head_dim == 64 ? launch(fp4_rows_kernel<64>) : launch(fp4_rows_kernel<128>), name);
@@ -344,11 +457,10 @@ MRUN_API int mrun_qk_norm_rope_cache_fp4(const void* qkv, void* q_out, long q_st
                  "%s: rows and pages start on 16 bytes", name);
     MRUN_REQUIRE(((uintptr_t)rot & 7) == 0, "%s: the table starts on 8 bytes", name);
     if (tokens == 0) return 0;
-    MRUN_CHECK_CUDA(head_dim == 64 ? launch_store<64>(qkv, q_out, q_stride, q_weight, k_weight, eps, rot, rotary_dim, slots, cache, tokens,
-                                                      heads, kv_heads, page_size, pages, stream)
-                                   : launch_store<128>(qkv, q_out, q_stride, q_weight, k_weight, eps, rot, rotary_dim, slots, cache, tokens,
-                                                       heads, kv_heads, page_size, pages, stream),
-                    name);
+    MRUN_REQUIRE((long)tokens * (heads + 2 * kv_heads) < (1L << 31), "%s: %d tokens of %d heads are more than a launch takes", name, tokens, heads);
+    auto launch = head_dim == 64 ? launch_store<64> : launch_store<128>;
+    MRUN_CHECK_CUDA(launch(qkv, q_out, q_stride, q_weight, k_weight, eps, rot, rotary_dim, slots, cache, tokens, heads, kv_heads, page_size,
+                           pages, stream), name);
     MRUN_CHECK_LAUNCH(name);
     return 0;
 }

@@ -484,9 +484,13 @@ def prefill_uses_tcgen05(library, ratio: int, page_size: int) -> bool:
 
 
 # ------------------------------------------------------------------ the 4-bit cache
-# Segments of up to this many tokens take the kernel for single tokens, row by row; longer ones have their keys
-# and values read back.
-FP4_SHORT = 4
+# Which segments of a step with prompt portions take the kernel for single tokens, row by row: the shortest, as long as all their
+# rows times the kv heads are at most this many; the longer ones have their keys and values read back.  A row reads its whole context, but
+# all blocks share the step; the prompt kernels sweep a context with a block a tile and kv head.  The second figure is for segments that
+# fill at most a tile of 64 rows (rows x query heads a kv head), which the slower of the two prompt kernels would take.
+# B200, us by rows / read back, 32 heads over 8 of 128 behind 9,000 tokens: one segment of 16 tokens 44 / 452, of 32 69 / 97, of 64 124 / 97;
+# eight of 16 192 / 607, of 32 369 / 200.  16 heads over 16 behind 9,000: eight of 16 368 / 575, of 32 723 / 584.
+FP4_ROWS, FP4_ROWS_OF_A_TILE = 256, 2048
 FP4_SCRATCH_ROWS = 128     # rows of a page that is read back: a key tile of the tcgen05 prompt kernel
 _fp4_slots = {}            # (device, head size, heads a block) -> blocks of the decode kernel that the device holds
 
@@ -555,16 +559,19 @@ def _fp4_tokens(q, q_stride: int, out, cache, group, ctx, heads: int, head_dim: 
                      units * ops.FP4_TOKENS, pages, scale, window, scratch.data_ptr(), blocks, _queue())
 
 
-def _fp4_portions(ctx, window: int, short: int):
-    """What a step's prompt portions need, made once per step: the rows of its short segments, and for the longer ones the spans of tokens
+def _fp4_portions(ctx, window: int, heads: int, kv_heads: int):
+    """What a step's prompt portions need, made once per step: the rows that go one by one, and for the longer segments the spans of tokens
     to read back, their pages, and a step context and block tables over these, which the first layer's call fills."""
-    key = ("fp4_portions", window, short)
+    key = ("fp4_portions", window, heads, kv_heads)
     found = ctx.shared.get(key)
     if found is not None:
         return found
+    ratio = heads // kv_heads
     rows, spans, longer, pages, width = [], [], [], 0, 0
-    for seg in ctx.segments:
-        if seg.q_len <= short:
+    for seg in sorted(ctx.segments, key=lambda seg: seg.q_len):
+        most = FP4_ROWS if ratio * seg.q_len > 64 else FP4_ROWS_OF_A_TILE
+        # a decoding token is a row; the prompt kernels over tensor cores take up to 64 query heads a kv head
+        if seg.q_len == 1 or ratio > 64 or (len(rows) + seg.q_len) * kv_heads <= most:
             rows.extend(range(seg.q_start, seg.q_start + seg.q_len))
             continue
         end = seg.pos_start + seg.q_len
@@ -595,8 +602,8 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
     """:func:`paged_attention` over a 4-bit cache (``cache``: pages of :func:`mrun_b200.kernels.ops.fp4_cache_shape`): bfloat16, heads
     of 64 or 128 features, pages of a multiple of 16 tokens, any number of query heads a kv head.
 
-    Single tokens, and segments of up to ``FP4_SHORT``, read the 4-bit pages as they are (every step of single tokens may be
-    captured in a graph).  The keys and values of longer segments are read back in bfloat16, 128 tokens a page, for the time of
+    Single tokens, and a few tokens more, read the 4-bit pages as they are (every step of single tokens may be captured in a
+    graph).  The keys and values of longer segments are read back in bfloat16, 128 tokens a page, for the time of
     the call (4 * head_dim bytes a token and kv head of the segments' contexts), and go to the prompt kernels.  A page outside the cache is not
     seen; a row that sees nothing is zeros.  A value that is NaN makes NaN of the rows that see it, and may of other rows of
     the same prompt portion."""
@@ -620,10 +627,8 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
         return out
     if tokens > ctx.real_tokens:
         out[ctx.real_tokens:].zero_()
-    # the prompt kernels over tensor cores take up to 64 query heads a kv head
-    short = FP4_SHORT if heads // kv_heads <= 64 else tokens
-    filled = ("fp4_portions", window, short) in ctx.shared
-    rows, longer = _fp4_portions(ctx, window, short)
+    filled = ("fp4_portions", window, heads, kv_heads) in ctx.shared
+    rows, longer = _fp4_portions(ctx, window, heads, kv_heads)
     if rows:
         _fp4_tokens(q, q_stride, out, cache, group, ctx, heads, head_dim, scale, window, rows)
     if longer is not None:
