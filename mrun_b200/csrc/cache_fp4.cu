@@ -21,10 +21,13 @@ using bf16 = __nv_bfloat16;
 // 2,048 tokens of 32 + 8 + 8 heads of 128.
 // A value is a bfloat16: its quotient by a scale of 4 bits is a border (at most 3 bits) exactly or 2^-9 away from it.
 //
-// A block takes 256 threads' worth of the heads of one token, D / 8 lanes a head, eight features a lane: the token's cosines and sines
-// are read once into the first-level cache.
+// D / 8 lanes take TOGETHER heads of a token, eight features a lane, all asked for before the first is worked on: with one head at a time
+// a multiprocessor had 12 KB under way, where the memory's rate takes three times that (34 us for the write and read back of 2,048 tokens).  A step of few heads
+// gives each lanes of its own.
 // ------------------------------------------------------------------------------------------
 constexpr int STORE_THREADS = 256;
+constexpr int HEADS_TOGETHER = 4;
+constexpr int HEADS_AT_ONCE = 8192;        // a step of up to this many heads gives each lanes of its own
 
 // The byte of the scale nearest to `wanted` (0 .. 10,240), ties to the even byte.  `wanted` has a bit set below
 // its 24 wherever something was cut off, so that this is the only rounding.
@@ -38,10 +41,12 @@ __device__ __forceinline__ float scale_value(unsigned byte) {
     return __half2float(__ushort_as_half((unsigned short)(byte << 7)));
 }
 
-// Two 4-bit floats, `lo` in the low half of the byte: nearest, ties to the even code, at most 6.
-__device__ __forceinline__ unsigned codes_of(float lo, float hi) {
-    unsigned short out;
-    asm("{\n.reg .b8 c;\ncvt.rn.satfinite.e2m1x2.f32 c, %1, %2;\nmov.b16 %0, {c, 0};\n}" : "=h"(out) : "f"(hi), "f"(lo));
+// Eight 4-bit floats, the first in the lowest bits: nearest, ties to the even code, at most 6.
+__device__ __forceinline__ unsigned codes_of(const float (&f)[8]) {
+    unsigned out;
+    asm("{\n.reg .b8 c0, c1, c2, c3;\ncvt.rn.satfinite.e2m1x2.f32 c0, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 c1, %4, %3;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 c2, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 c3, %8, %7;\nmov.b32 %0, {c0, c1, c2, c3};\n}"
+        : "=r"(out) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
     return out;
 }
 
@@ -51,85 +56,77 @@ __device__ __forceinline__ float cut_sticky(double v) {
     return (double)f == v ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
 
-// The largest magnitude of the 16 features that two neighbouring lanes hold; `finite`: none is a NaN or an infinity.
-template <typename F> __device__ __forceinline__ F largest_of(const F (&x)[8], unsigned mask, bool& finite) {
-    F largest = 0;
-    finite = true;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const F a = x[e] < 0 ? -x[e] : x[e];
-        finite = finite && a < (F)INFINITY;
-        largest = a > largest ? a : largest;
-    }
-    const F other = __shfl_xor_sync(mask, largest, 1);
-    finite = __shfl_xor_sync(mask, (int)finite, 1) && finite;
-    return other > largest ? other : largest;
-}
+// Magnitudes as their bits, whose order is theirs; those of NaN and the infinities lie above.
+constexpr unsigned INFINITE = 0x7F800000u;
+__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // The codes (8 features a lane, four bytes) and the scale of the 16 features that two neighbouring lanes hold: of any doubles,
 __device__ __forceinline__ unsigned quantise(const double (&x)[8], unsigned mask, unsigned& scale) {
-    bool finite;
-    const double largest = largest_of(x, mask, finite);
+    double largest = 0.0;
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        finite = finite && fabs(x[e]) < INFINITY;
+        largest = fmax(largest, fabs(x[e]));
+    }
+    largest = fmax(largest, __shfl_xor_sync(mask, largest, 1));
+    finite = __shfl_xor_sync(mask, (int)finite, 1) && finite;
     scale = finite ? scale_byte(cut_sticky(fmin(largest / 6.0, 10240.0))) : (unsigned)FP4_NAN_SCALE;
     if (!finite) return 0u;
     const double s = scale_value(scale);
     // A shade more than 1 / s, so that a quotient that is a border exactly is not cut below it.
     const double inverse = s > 0.0 ? 1.0 / s * (1.0 + 8.8817841970012523e-16) : 0.0;
-    unsigned out = 0;
+    float f[8];
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-        float f[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            f[i] = __double2float_rz(x[e + i] * inverse);
-            if ((double)f[i] * s != x[e + i]) f[i] = __uint_as_float(__float_as_uint(f[i]) | 1u);
-        }
-        out |= codes_of(f[0], f[1]) << (4 * e);
+    for (int e = 0; e < 8; ++e) {
+        f[e] = __double2float_rz(x[e] * inverse);
+        if ((double)f[e] * s != x[e]) f[e] = __uint_as_float(__float_as_uint(f[e]) | 1u);
     }
-    return out;
+    return codes_of(f);
 }
 
 // of floats that hold bfloat16 values,
 __device__ __forceinline__ unsigned quantise(const float (&x)[8], unsigned mask, unsigned& scale) {
-    bool finite;
-    const float largest = largest_of(x, mask, finite);
-    scale = finite ? scale_byte(fminf(__fdiv_rn(largest, 6.f), 10240.f)) : (unsigned)FP4_NAN_SCALE;
-    const float s = scale_value(scale);
-    if (!(s > 0.f)) return 0u;
-    const float inverse = __fdiv_rn(1.f, s);
-    unsigned out = 0;
+    unsigned top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-        float f[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            // the quotient to 12 bits: one that is a border exactly comes out as it
-            const float y = __fmul_rn(fminf(fmaxf(x[e + i], -1e6f), 1e6f), inverse), wide = __fmul_rn(y, 4097.f);
-            f[i] = __fsub_rn(wide, __fsub_rn(wide, y));
-        }
-        out |= codes_of(f[0], f[1]) << (4 * e);
+    for (int e = 0; e < 8; ++e) top = max(top, magnitude(x[e]));
+    top = max(top, __shfl_xor_sync(mask, top, 1));
+    if (top >= INFINITE) {
+        scale = FP4_NAN_SCALE;
+        return 0u;
     }
-    return out;
+    scale = scale_byte(fminf(__fdiv_rn(__uint_as_float(top), 6.f), 10240.f));
+    const float s = scale_value(scale), inverse = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {    // the quotient to 12 bits: one that is a border exactly comes out as it, any other stays on its side
+        const float y = __fmul_rn(x[e], inverse), wide = __fmul_rn(y, 4097.f);
+        f[e] = __fsub_rn(wide, __fsub_rn(wide, y));
+    }
+    return codes_of(f);
 }
 
 // and of floats that are within `off` of the values meant.  `sure`: neither the scale nor a code depends on where within.
 __device__ __forceinline__ unsigned quantise(const float (&x)[8], float off, unsigned mask, unsigned& scale, bool& sure) {
-    bool finite;
-    const float largest = largest_of(x, mask, finite);
-    scale = scale_byte(fminf((largest + off) * (1.f / 6.f) * 1.000001f, 10240.f));
-    sure = finite && off < INFINITY && scale == scale_byte(fminf(fmaxf(largest - off, 0.f) * (1.f / 6.f) * 0.999999f, 10240.f));
-    const float s = scale_value(scale), inverse = s > 0.f ? 1.f / s : 0.f, away = off * inverse * 1.000001f;
-    unsigned low = 0, high = 0;
+    unsigned top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-        // three roundings of the quotient and its ends: 2^-22 of it
-        const float y0 = x[e] * inverse, y1 = x[e + 1] * inverse;
-        const float a0 = fmaf(fabsf(y0), 4.8e-7f, away), a1 = fmaf(fabsf(y1), 4.8e-7f, away);
-        low |= codes_of(y0 - a0, y1 - a1) << (4 * e);
-        high |= codes_of(y0 + a0, y1 + a1) << (4 * e);
+    for (int e = 0; e < 8; ++e) top = max(top, magnitude(x[e]));
+    top = max(top, __shfl_xor_sync(mask, top, 1));
+    const float largest = __uint_as_float(top);
+    scale = scale_byte(fminf((largest + off) * (1.f / 6.f) * 1.000001f, 10240.f));
+    sure = top < INFINITE && off < INFINITY && scale == scale_byte(fminf(fmaxf(largest - off, 0.f) * (1.f / 6.f) * 0.999999f, 10240.f));
+    const float s = scale_value(scale), inverse = s > 0.f ? __fdividef(1.f, s) : 0.f;
+    // the quotients are at most 6.4 where they are not far beyond the last border, and off by 2^-21 of them
+    const float away = fmaf(off, inverse * 1.000001f, 4e-6f);
+    float low[8], high[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        low[e] = fmaf(x[e], inverse, -away);
+        high[e] = fmaf(x[e], inverse, away);
     }
-    sure = sure && low == high;
-    return low;
+    const unsigned codes = codes_of(low);
+    sure = sure && codes == codes_of(high);
+    return codes;
 }
 
 // Eight floats of `src`, on 16 bytes.
@@ -194,37 +191,30 @@ __device__ __forceinline__ void rotate_staged(F (&v)[8], const float2* __restric
 }
 
 // STAGED: rotary sizes that are no multiple of 16, and weights or tables off 16 bytes; keys in 64 bits throughout.
-template <int D, bool STAGED>
-__global__ void __launch_bounds__(STORE_THREADS)
+template <int D, bool STAGED, int TOGETHER>
+__global__ void __launch_bounds__(STORE_THREADS, STAGED ? 1 : 3)
 qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, long q_stride,
                               const float* __restrict__ q_weight, const float* __restrict__ k_weight, float eps,
-                              const float2* __restrict__ rot, int half, const int* __restrict__ slots,
-                              unsigned char* __restrict__ cache, int heads, int kv_heads, int page_size, long pages, int blocks_per_token) {
+                              const float2* __restrict__ rot, int half, const int* __restrict__ slots, unsigned char* __restrict__ cache,
+                              unsigned groups, int heads, int kv_heads, int page_size, long pages, unsigned groups_per_token) {
     using Unit = Fp4Unit<D>;
-    constexpr int LANES = D / 8, GROUPS = STORE_THREADS / LANES;
-    __shared__ double stage_all[STAGED ? GROUPS * D : 1];
+    constexpr int LANES = D / 8;
+    __shared__ double stage_all[STAGED ? STORE_THREADS / LANES * D : 1];
     const int per_token = heads + 2 * kv_heads;
-    const int t = blockIdx.x / blocks_per_token, chunk = blockIdx.x - t * blocks_per_token;
-    const int group = threadIdx.x / LANES, part = threadIdx.x % LANES, head = chunk * GROUPS + group;
-    if (head >= per_token) return;                                 // all lanes of a group together
+    const unsigned group = blockIdx.x * (STORE_THREADS / LANES) + threadIdx.x / LANES;
+    if (group >= groups) return;                                   // all lanes of a group together
+    const int t = (int)(group / groups_per_token), head0 = (int)(group - t * groups_per_token) * TOGETHER, part = threadIdx.x % LANES;
     const unsigned lane = threadIdx.x & 31;
     const unsigned mask = ((1u << LANES) - 1u) << (lane & ~(unsigned)(LANES - 1));
-    const bool is_q = head < heads, is_k = !is_q && head < heads + kv_heads;
 
-    const uint4 raw = *reinterpret_cast<const uint4*>(qkv + ((size_t)t * per_token + head) * D + part * 8);
-    // a slot outside the cache (a padding row's -1) writes nothing
-    const int slot = is_q || slots == nullptr ? -1 : slots[t];
-    const float* weights = is_q ? q_weight : k_weight;
-    const bool normed = weights != nullptr && (is_q || is_k), turned = half > 0 && (is_q || is_k);
-    float weight[8];
-    if (normed) {
-        if constexpr (STAGED) {
+    uint4 raw[TOGETHER];
+    const bf16* row = qkv + ((size_t)t * per_token + head0) * D + part * 8;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) weight[e] = weights[part * 8 + e];
-        } else {
-            load8(weight, weights + part * 8);
-        }
-    }
+    for (int i = 0; i < TOGETHER; ++i)
+        if (head0 + i < per_token) raw[i] = *reinterpret_cast<const uint4*>(row + i * D);
+    // a slot outside the cache (a padding row's -1) writes nothing
+    const int slot = head0 + TOGETHER <= heads || slots == nullptr ? -1 : slots[t];
+    const bool turned = half > 0 && head0 < heads + kv_heads;
     const float2* cs = rot + (size_t)t * half;
     Turn turn;
     if (!STAGED && turned) {
@@ -244,72 +234,92 @@ qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, lon
             }
         }
     }
-    double* stage = stage_all + (STAGED ? group * D : 0);
-    float x[8];
-    {
-        const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = __bfloat1622float2(pairs[e]);
-            x[2 * e] = f.x; x[2 * e + 1] = f.y;
-        }
-    }
-    if (is_q) {
-        if (normed) norm<float, D>(x, weight, eps, mask);
-        if (turned) {
-            if constexpr (STAGED) rotate_staged(x, cs, half, mask, part, reinterpret_cast<float*>(stage));
-            else rotate(x, turn, mask, part);
-        }
-        uint4 packed;
-        __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(&packed);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
-        *reinterpret_cast<uint4*>(q_out + (size_t)t * q_stride + (size_t)head * D + part * 8) = packed;
-        return;
-    }
+    const bool normed = q_weight != nullptr;
+    double* stage = stage_all + (STAGED ? threadIdx.x / LANES * D : 0);
     const int page = slot >= 0 ? slot / page_size : -1;
-    if (page < 0 || page >= pages) return;
+    const bool writes = page >= 0 && page < pages;
     const int off = slot - page * page_size, r = off & (FP4_TOKENS - 1);
-    const int kv_head = is_k ? head - heads : head - heads - kv_heads;
-    unsigned char* unit = cache + (((size_t)page * kv_heads + kv_head) * (page_size / FP4_TOKENS) + off / FP4_TOKENS) * Unit::BYTES;
-    unsigned scale, codes;
-    if (is_k && (normed || turned)) {
-        bool sure = false;
-        if constexpr (!STAGED) {
-            float y[8];
+    unsigned char* units = cache + ((size_t)page * kv_heads * (page_size / FP4_TOKENS) + off / FP4_TOKENS) * Unit::BYTES;
+    const int head_bytes = page_size / FP4_TOKENS * Unit::BYTES;
+
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = x[e];
-            if (normed) norm<float, D>(y, weight, eps, mask);
-            float widest = 0.f;
-            if (turned) {
-                widest = rotate(y, turn, mask, part);
+    for (int i = 0; i < TOGETHER; ++i) {
+        const int head = head0 + i;
+        if (head >= per_token) break;
+        const bool is_q = head < heads, is_k = !is_q && head < heads + kv_heads;
+        if (!is_q && !writes) break;                               // keys and values lie behind the queries
+        float weight[8];
+        if (normed && (is_q || is_k)) {
+            const float* weights = is_q ? q_weight : k_weight;
+            if constexpr (STAGED) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) weight[e] = weights[part * 8 + e];
             } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) widest = fmaxf(widest, fabsf(y[e]));
+                load8(weight, weights + part * 8);
             }
-            widest = fmaxf(widest, __shfl_xor_sync(mask, widest, 1));
-            // The sum of squares is off by 12 roundings at most and half of that under the root, the root by 2^-22, the two products and the
-            // two of the rotation by one each: less than 2^-20 of |first| + |second|.
-            codes = quantise(y, widest * 1.9073486328125e-06f, mask, scale, sure);
-            sure = __all_sync(mask, sure);
         }
-        if (!sure) {
-            double y[8];
+        float x[8];
+        {
+            const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = x[e];
-            if (normed) norm<double, D>(y, weight, eps, mask);
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = __bfloat1622float2(pairs[e]);
+                x[2 * e] = f.x; x[2 * e + 1] = f.y;
+            }
+        }
+        if (is_q) {
+            if (normed) norm<float, D>(x, weight, eps, mask);
             if (turned) {
-                if constexpr (STAGED) rotate_staged(y, cs, half, mask, part, stage);
-                else rotate(y, turn, mask, part);
+                if constexpr (STAGED) rotate_staged(x, cs, half, mask, part, reinterpret_cast<float*>(stage));
+                else rotate(x, turn, mask, part);
             }
-            codes = quantise(y, mask, scale);
+            uint4 packed;
+            __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+            *reinterpret_cast<uint4*>(q_out + (size_t)t * q_stride + (size_t)head * D + part * 8) = packed;
+            continue;
         }
-    } else {
-        codes = quantise(x, mask, scale);
+        unsigned scale, codes;
+        if (is_k && (normed || turned)) {
+            bool sure = false;
+            if constexpr (!STAGED) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = x[e];
+                if (normed) norm<float, D>(y, weight, eps, mask);
+                float widest = 0.f;
+                if (turned) {
+                    widest = rotate(y, turn, mask, part);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) widest = fmaxf(widest, fabsf(y[e]));
+                }
+                widest = fmaxf(widest, __shfl_xor_sync(mask, widest, 1));
+                // The sum of squares is off by 12 roundings at most and half of that under the root, the root by 2^-22, the two products and the
+                // two of the rotation by one each: less than 2^-20 of |first| + |second|.
+                codes = quantise(y, widest * 1.9073486328125e-06f, mask, scale, sure);
+                sure = __all_sync(mask, sure);
+            }
+            if (!sure) {
+                double y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = x[e];
+                if (normed) norm<double, D>(y, weight, eps, mask);
+                if (turned) {
+                    if constexpr (STAGED) rotate_staged(y, cs, half, mask, part, stage);
+                    else rotate(y, turn, mask, part);
+                }
+                codes = quantise(y, mask, scale);
+            }
+        } else {
+            codes = quantise(x, mask, scale);
+        }
+        unsigned char* unit = units + (size_t)(is_k ? head - heads : head - heads - kv_heads) * head_bytes;
+        // eight features are four bytes of one piece: D = 128 has pieces of eight bytes, D = 64 of four
+        *reinterpret_cast<unsigned*>(unit + (is_k ? Unit::k_code(r, part * 4) : Unit::v_code(r, part * 4))) = codes;
+        if ((part & 1) == 0) unit[is_k ? Unit::k_scale(r, part / 2) : Unit::v_scale(r, part / 2)] = (unsigned char)scale;
     }
-    // eight features are four bytes of one piece: D = 128 has pieces of eight bytes, D = 64 of four
-    *reinterpret_cast<unsigned*>(unit + (is_k ? Unit::k_code(r, part * 4) : Unit::v_code(r, part * 4))) = codes;
-    if ((part & 1) == 0) unit[is_k ? Unit::k_scale(r, part / 2) : Unit::v_scale(r, part / 2)] = (unsigned char)scale;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -406,17 +416,17 @@ fp4_rows_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
     }
 }
 
-template <int D>
+template <int D, int TOGETHER>
 cudaError_t launch_store(const void* qkv, void* q_out, long q_stride, const float* q_weight, const float* k_weight, float eps,
                          const float* rot, int rotary_dim, const int* slots, void* cache, int tokens, int heads, int kv_heads,
                          int page_size, long pages, cudaStream_t stream) {
-    constexpr int GROUPS = STORE_THREADS / (D / 8);
-    const int blocks_per_token = (heads + 2 * kv_heads + GROUPS - 1) / GROUPS;
+    constexpr unsigned GROUPS = STORE_THREADS / (D / 8);
+    const unsigned per_token = (unsigned)(heads + 2 * kv_heads + TOGETHER - 1) / TOGETHER, groups = (unsigned)tokens * per_token;
     const bool staged = rotary_dim % 16 || (((uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)rot) & 15);
-    return launch_kernel(staged ? qk_norm_rope_cache_fp4_kernel<D, true> : qk_norm_rope_cache_fp4_kernel<D, false>,
-                         dim3((unsigned)tokens * (unsigned)blocks_per_token), dim3(STORE_THREADS), 0, stream, (const bf16*)qkv, (bf16*)q_out, q_stride,
-                         q_weight, k_weight, eps, (const float2*)rot, rotary_dim / 2, slots, (unsigned char*)cache, heads, kv_heads, page_size,
-                         pages, blocks_per_token);
+    return launch_kernel(staged ? qk_norm_rope_cache_fp4_kernel<D, true, TOGETHER> : qk_norm_rope_cache_fp4_kernel<D, false, TOGETHER>,
+                         dim3((groups + GROUPS - 1) / GROUPS), dim3(STORE_THREADS), 0, stream, (const bf16*)qkv, (bf16*)q_out, q_stride,
+                         q_weight, k_weight, eps, (const float2*)rot, rotary_dim / 2, slots, (unsigned char*)cache, groups, heads, kv_heads,
+                         page_size, pages, per_token);
 }
 
 int launch_rows(const void* cache, const int* ids, const Spans& spans, const int* block_tables, int table_rows, int max_blocks, void* k_out,
@@ -458,7 +468,9 @@ MRUN_API int mrun_qk_norm_rope_cache_fp4(const void* qkv, void* q_out, long q_st
     MRUN_REQUIRE(((uintptr_t)rot & 7) == 0, "%s: the table starts on 8 bytes", name);
     if (tokens == 0) return 0;
     MRUN_REQUIRE((long)tokens * (heads + 2 * kv_heads) < (1L << 31), "%s: %d tokens of %d heads are more than a launch takes", name, tokens, heads);
-    auto launch = head_dim == 64 ? launch_store<64> : launch_store<128>;
+    const bool alone = (long)tokens * (heads + 2 * kv_heads) <= HEADS_AT_ONCE;
+    auto launch = head_dim == 64 ? (alone ? launch_store<64, 1> : launch_store<64, HEADS_TOGETHER>)
+                                 : (alone ? launch_store<128, 1> : launch_store<128, HEADS_TOGETHER>);
     MRUN_CHECK_CUDA(launch(qkv, q_out, q_stride, q_weight, k_weight, eps, rot, rotary_dim, slots, cache, tokens, heads, kv_heads, page_size,
                            pages, stream), name);
     MRUN_CHECK_LAUNCH(name);
