@@ -278,11 +278,11 @@ def fp4_cache_shape(pages: int, kv_heads: int, page_size: int, head_dim: int) ->
 
 def check_fp4_cache(cache: torch.Tensor, head_dim: int, kv_heads: Optional[int] = None) -> tuple:
     """(pages, kv heads, page size) of a 4-bit cache's pages, from their shape."""
-    if cache.dim() != 4 or cache.shape[3] != fp4_unit_bytes(head_dim) or cache.shape[1] < 1 or cache.shape[2] < 1 \
-            or (kv_heads is not None and cache.shape[1] != kv_heads):
-        raise KernelError(f"the 4-bit cache is {tuple(cache.shape)}, expected [pages, {kv_heads or 'kv heads'}, page_size / {FP4_TOKENS}, "
+    shape = cache.shape
+    if len(shape) != 4 or shape[3] != fp4_unit_bytes(head_dim) or shape[1] < 1 or shape[2] < 1 or (kv_heads is not None and shape[1] != kv_heads):
+        raise KernelError(f"the 4-bit cache is {tuple(shape)}, expected [pages, {kv_heads or 'kv heads'}, page_size / {FP4_TOKENS}, "
                           f"{fp4_unit_bytes(head_dim)}] for heads of {head_dim} features")
-    return cache.shape[0], cache.shape[1], cache.shape[2] * FP4_TOKENS
+    return shape[0], shape[1], shape[2] * FP4_TOKENS
 
 
 def qk_norm_rope_cache_fp4(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
@@ -293,47 +293,57 @@ def qk_norm_rope_cache_fp4(qkv: torch.Tensor, heads: int, kv_heads: int, head_di
     or into the rows ``q_out`` (which may be strided) with ``qkv`` left as it is; k (normed, rotated, not rounded in between) and v
     quantised into the places that ``slots`` names (page * page_size + offset, each at most once; outside the cache: not written).
     Returns q's rows."""
-    if qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * kv_heads) * head_dim:
-        raise KernelError(f"qk_norm_rope_cache_fp4: qkv is {tuple(qkv.shape)}, expected width {(heads + 2 * kv_heads) * head_dim}")
+    shape = qkv.shape
+    if len(shape) != 2 or shape[1] != (heads + 2 * kv_heads) * head_dim:
+        raise KernelError(f"qk_norm_rope_cache_fp4: qkv is {tuple(shape)}, expected width {(heads + 2 * kv_heads) * head_dim}")
     if head_dim not in FP4_HEAD_DIMS:
         raise KernelError(f"the 4-bit cache takes heads of 64 or 128 features, not {head_dim}")
-    tokens = qkv.shape[0]
+    tokens = shape[0]
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and w.numel() != head_dim:
+        if w is not None and w.shape != (head_dim,):
             raise KernelError(f"qk_norm_rope_cache_fp4: {name} has {w.numel()} elements, head_dim is {head_dim}")
     if rot is not None and rot.shape != (tokens, rotary_dim // 2, 2):
         raise KernelError(f"qk_norm_rope_cache_fp4: rot is {tuple(rot.shape)}, expected {(tokens, rotary_dim // 2, 2)}")
-    if slots is not None and (cache is None or slots.shape != (tokens,)):
-        raise KernelError("qk_norm_rope_cache_fp4: one slot per token is needed, and the cache they lie in")
     if q_out is not None and q_out.shape != (tokens, heads * head_dim):
         raise KernelError(f"qk_norm_rope_cache_fp4: q_out is {tuple(q_out.shape)}, expected {(tokens, heads * head_dim)}")
     pages, page_size = 0, FP4_TOKENS
     if slots is not None:
+        if cache is None or slots.shape != (tokens,):
+            raise KernelError("qk_norm_rope_cache_fp4: one slot per token is needed, and the cache they lie in")
         pages, _, page_size = check_fp4_cache(cache, head_dim, kv_heads)
-        _check(slots, "slots", torch.int32); _check(cache, "cache", torch.uint8)
     _check(qkv, "qkv", torch.bfloat16)
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("rot", rot)):
-        if t is not None:
-            _check(t, name, torch.float32)
+    if q_weight is not None:
+        _check(q_weight, "q_weight", torch.float32)
+    if k_weight is not None:
+        _check(k_weight, "k_weight", torch.float32)
+    if rot is not None:
+        _check(rot, "rot", torch.float32)
+    cache_at = None
+    if slots is not None:
+        _check(slots, "slots", torch.int32); _check(cache, "cache", torch.uint8)
+        cache_at = cache.data_ptr()
     if q_out is None:
-        q, stride = qkv[:, :heads * head_dim], qkv.shape[1]
+        q, stride = qkv[:, :heads * head_dim], shape[1]
     else:
         _check(q_out, "q_out", torch.bfloat16, dense=False)
-        q, stride = q_out, _strided_rows(q_out, "q_out")
+        if q_out.stride(1) != 1:
+            raise KernelError("q_out must be rows of contiguous features")
+        q, stride = q_out, q_out.stride(0)
     _lib.fp4().call("mrun_qk_norm_rope_cache_fp4", qkv.data_ptr(), q.data_ptr(), stride, _address(q_weight), _address(k_weight), eps,
-                    _address(rot), rotary_dim if rot is not None else 0, _address(slots), cache.data_ptr() if slots is not None else None,
-                    tokens, heads, kv_heads, head_dim, page_size, pages, _queue())
+                    _address(rot), rotary_dim if rot is not None else 0, _address(slots), cache_at, tokens, heads, kv_heads, head_dim,
+                    page_size, pages, _queue())
     return q
 
 
 def fp4_pages(cache: torch.Tensor, head_dim: int, pages: torch.Tensor):
     """(keys, values): bfloat16 [n, kv heads, page_size, head_dim] each, what the pages ``pages`` (int32 [n]) of a 4-bit cache hold,
     exactly; a page outside the cache reads as zeros."""
-    if pages.dim() != 1:
-        raise KernelError(f"fp4_pages: pages is {tuple(pages.shape)}, expected a list")
+    shape = pages.shape
+    if len(shape) != 1:
+        raise KernelError(f"fp4_pages: pages is {tuple(shape)}, expected a list")
     held, kv_heads, page_size = check_fp4_cache(cache, head_dim)
     _check(cache, "cache", torch.uint8); _check(pages, "pages", torch.int32)
-    n = pages.shape[0]
+    n = shape[0]
     k, v = torch.empty((2, n, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=cache.device).unbind(0)
     _lib.fp4().call("mrun_fp4_pages", cache.data_ptr(), pages.data_ptr(), k.data_ptr(), v.data_ptr(), n, kv_heads, head_dim, page_size, held,
                     _queue())
