@@ -23,7 +23,7 @@
 // works on the two before, across pairs: no barrier but where a pair's pieces meet.  Every warp of a block works on the same
 // (token, kv head, group of heads) pair.  The tiles (8 units) of all pairs lie in one list, cut evenly among the
 // blocks that the device holds at once; a pair that lies in several blocks leaves its pieces in scratch, and
-// a second kernel, on the device before the first has ended, adds them in block order.
+// a second kernel, whose launch overlaps the first one's end, adds them in block order.
 #include <atomic>
 #include <cfloat>
 #include <cuda_fp16.h>
@@ -58,14 +58,14 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1,
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same with nothing to add to.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ unsigned transposed(unsigned rows) {
     unsigned out;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(out) : "r"(rows));
-    return out;
-}
-__device__ __forceinline__ unsigned mul_h2(unsigned a, unsigned b) {
-    unsigned out;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(out) : "r"(a), "r"(b));
     return out;
 }
 __device__ __forceinline__ unsigned pack_h2(float lo, float hi) {
@@ -84,9 +84,15 @@ __device__ __forceinline__ void halves_of(unsigned word, unsigned (&h)[4]) {
         "cvt.rn.f16x2.e2m1x2 %0, c0;\ncvt.rn.f16x2.e2m1x2 %1, c1;\ncvt.rn.f16x2.e2m1x2 %2, c2;\ncvt.rn.f16x2.e2m1x2 %3, c3;\n}"
         : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(word));
 }
-// Byte `i` of `bytes`, a scale, as the same half twice.
-template <int I> __device__ __forceinline__ unsigned scale_twice(unsigned bytes) {
-    return __byte_perm(bytes, 0u, (I << 12) | (4 << 8) | (I << 4) | 4) >> 1;
+// Bytes I and I + 1 of `bytes`, scales, as halves.
+template <int I> __device__ __forceinline__ __half2 two_scales(unsigned bytes) {
+    const unsigned bits = __byte_perm(bytes, 0u, ((I + 1) << 12) | (4 << 8) | (I << 4) | 4) >> 1;
+    return *reinterpret_cast<const __half2*>(&bits);
+}
+// Both halves of `codes` times one of two scales, which the multiplication picks itself.
+__device__ __forceinline__ unsigned scaled(unsigned codes, __half2 scales, int which) {
+    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&codes), which ? __high2half2(scales) : __low2half2(scales));
+    return *reinterpret_cast<const unsigned*>(&v);
 }
 
 // A score less the maximum it is taken against.  The product is rounded as the maximum's was: fused, the difference of a huge
@@ -240,7 +246,6 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     const int group = step.heads / step.kv_heads, head_groups = (group + HEADS - 1) / HEADS;
     const int units_a_page = step.page_size / FP4_TOKENS, table_units = step.max_blocks * units_a_page, pairs = step.kv_heads * head_groups;
 
-    dependents_may_start();                            // the second kernel's blocks come as these leave, and wait for the last
     make_plan(prefix, held_pos, step.positions, step.token_slot, rows, step.tokens, step.window, table_units, scratch);
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i <= step.tokens; i += THREADS) step.plan[i] = prefix[i];
@@ -402,7 +407,6 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) {
                 const unsigned char* unit = stage + u * Unit::BYTES;
-                c[u][0] = c[u][1] = c[u][2] = c[u][3] = 0.f;
                 unsigned kw[2][WORDS_K];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -413,13 +417,8 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                 unsigned ks;                               // bytes: D = 128 [token g: 2, token g + 8: 2], D = 64 [1, 1]
                 if constexpr (D == 128) ks = *reinterpret_cast<const unsigned*>(unit + Unit::K_SCALES + lane * 4);
                 else ks = *reinterpret_cast<const unsigned short*>(unit + Unit::K_SCALES + lane * 2);
-                unsigned sc[2][Unit::PER];
-                if constexpr (D == 128) {
-                    sc[0][0] = scale_twice<0>(ks); sc[0][Unit::PER - 1] = scale_twice<1>(ks);
-                    sc[1][0] = scale_twice<2>(ks); sc[1][Unit::PER - 1] = scale_twice<3>(ks);
-                } else {
-                    sc[0][0] = scale_twice<0>(ks); sc[1][0] = scale_twice<1>(ks);
-                }
+                // of token g's and token g + 8's groups: D = 128 two each, D = 64 one each in one pair
+                const __half2 sc[2] = {two_scales<0>(ks), two_scales<(D == 128 ? 2 : 0)>(ks)};
 #pragma unroll
                 for (int w = 0; w < WORDS_K; ++w) {
                     unsigned a[2][4];
@@ -427,11 +426,13 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                     for (int r = 0; r < 2; ++r) {
                         halves_of(kw[r][w], a[r]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) a[r][i] = mul_h2(a[r][i], sc[r][w / 2]);
+                        for (int i = 0; i < 4; ++i) a[r][i] = scaled(a[r][i], sc[r], D == 128 ? w / 2 : r);
                     }
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        mma_f16(c[u], a[0][2 * j], a[1][2 * j], a[0][2 * j + 1], a[1][2 * j + 1], qf[2 * w + j][0], qf[2 * w + j][1]);
+                    for (int j = 0; j < 2; ++j) {
+                        if (w == 0 && j == 0) mma_f16_first(c[u], a[0][0], a[1][0], a[0][1], a[1][1], qf[0][0], qf[0][1]);
+                        else mma_f16(c[u], a[0][2 * j], a[1][2 * j], a[0][2 * j + 1], a[1][2 * j + 1], qf[2 * w + j][0], qf[2 * w + j][1]);
+                    }
                 }
             }
             // Score of the lane's head h with key g or g + 8 (r) of unit u: c[u][h + 2 r].
@@ -509,7 +510,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             for (int u = 0; u < UNITS; ++u) {
                 const unsigned char* unit = stage + u * Unit::BYTES;
                 const unsigned vs = *reinterpret_cast<const unsigned*>(unit + Unit::V_SCALES + (D == 128 ? lane : (g >> 1) * 4 + t) * 4) & seen[u];
-                const unsigned sv[4] = {scale_twice<0>(vs), scale_twice<1>(vs), scale_twice<2>(vs), scale_twice<3>(vs)};
+                const __half2 sv[2] = {two_scales<0>(vs), two_scales<2>(vs)};       // of tokens 2 t and 2 t + 1, then + 8
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     unsigned vw[2][WORDS_V];               // of tokens 2 t and 2 t + 1 (+ 8 half)
@@ -532,7 +533,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                         for (int r = 0; r < 2; ++r) {
                             halves_of(vw[r][w], a[r]);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) a[r][i] = mul_h2(a[r][i], sv[half * 2 + r]);
+                            for (int i = 0; i < 4; ++i) a[r][i] = scaled(a[r][i], sv[half], r);
                         }
 #pragma unroll
                         for (int j = 0; j < 2; ++j)
