@@ -55,17 +55,17 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // The same with nothing to add to.
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ unsigned transposed(unsigned rows) {
     unsigned out;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(out) : "r"(rows));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(out) : "r"(rows));
     return out;
 }
 __device__ __forceinline__ unsigned pack_h2(float lo, float hi) {
@@ -228,7 +228,7 @@ struct Step {
 };
 
 template <int D, bool FOUR>
-__global__ void __launch_bounds__(THREADS, 4)
+__global__ void __launch_bounds__(THREADS, FOUR ? 4 : 3)     // eight heads: 150 registers a thread without spills, 31 us where four blocks took 32
 decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsigned char* __restrict__ cache, const Step step,
                   const __grid_constant__ Rows rows) {
     using Unit = Fp4Unit<D>;
@@ -270,58 +270,53 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
         start.rest = begin - prefix[low] * pairs;
     }
 
-    // ---- the copies: this warp's units of every tile, one tile ahead of the work.  The pages of a tile's units are asked for
-    // one tile before their copies, so that these do not wait for the block table.
+    // ---- the copies: this warp's units of every tile, one tile ahead of the work.  The pages of 16 tiles' units are asked for
+    // together, one a lane, a tile before the first of them is copied.
     Cursor ahead = start;
     Piece ap = {};
-    int ap_tile = 0, located = 0, issued = 0;
-    int a_last = -1, a_unit = 0;                       // of the token whose units are copied: its last unit, this warp's next ones
-    const int* a_table = nullptr;
+    int ap_tile = 0, issued = 0;
+    int a_unit = 0;                                    // this warp's first unit of the piece that is copied
     const unsigned char* a_head = cache;               // the kv head's part of page 0
-    int page[UNITS], in_page[UNITS];                   // of the units that were located last
+    int window = -1;                                   // lane l: the page of unit l % 2 of tile ap_tile / 16 * 16 + l / 2 of the piece
     unsigned arriving = 0;                             // bit u: unit u of the stage that was filled last is there
-    auto locate = [&]() {
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u) page[u] = -1;
-        if (located < count) {
-            if (ap_tile == ap.tiles) {
-                ap = next_piece(ahead, count - located, prefix, step.kv_heads, head_groups);
-                ap_tile = 0;
-                const int pos = held_pos[ap.tok], table_row = held_row[ap.tok];
-                a_last = min(pos / FP4_TOKENS, table_units - 1);
-                a_unit = first_visible(pos, step.window) / FP4_TOKENS + ap.tile0 * UNITS_A_TILE + warp * UNITS;
-                a_table = step.block_tables + (size_t)table_row * step.max_blocks;
-                if (table_row < 0 || table_row >= step.table_rows) a_last = -1;
-                a_head = cache + (size_t)ap.kvh * units_a_page * Unit::BYTES + lane * 16;
-            }
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u) {
-                const int unit = a_unit + u;
-                const int block = step.unit_shift >= 0 ? unit >> step.unit_shift : unit / units_a_page;
-                in_page[u] = (unit - block * units_a_page) * Unit::BYTES;
-                if (unit <= a_last) page[u] = __ldg(a_table + block);
-            }
-            a_unit += UNITS_A_TILE;
-            ++ap_tile;
-            ++located;
+    static_assert(UNITS == 2, "a lane a unit of 16 tiles");
+    auto ask_pages = [&]() {                           // for the tile that is copied next
+        if (issued >= count) return;
+        if (ap_tile == ap.tiles) {
+            ap = next_piece(ahead, count - issued, prefix, step.kv_heads, head_groups);
+            ap_tile = 0;
+            a_unit = first_visible(held_pos[ap.tok], step.window) / FP4_TOKENS + ap.tile0 * UNITS_A_TILE + warp * UNITS;
+            a_head = cache + (size_t)ap.kvh * units_a_page * Unit::BYTES + lane * 16;
+        }
+        if (ap_tile % 16 == 0) {
+            const int table_row = held_row[ap.tok], last = min(held_pos[ap.tok] / FP4_TOKENS, table_units - 1);
+            const int unit = a_unit + (ap_tile + lane / 2) * UNITS_A_TILE + lane % 2;
+            window = -1;
+            if (unit <= last && table_row >= 0 && table_row < step.table_rows)
+                window = __ldg(step.block_tables + (size_t)table_row * step.max_blocks + (step.unit_shift >= 0 ? unit >> step.unit_shift : unit / units_a_page));
         }
     };
-    auto issue = [&]() {                               // copies the units located last (one that is not there as zeros) and locates the next
+    auto issue = [&]() {                               // copies the next tile's units, one that is not there as zeros
         const unsigned dst = smem_addr(ring + (issued % STAGES) * (UNITS * Unit::BYTES)) + lane * 16;
         arriving = 0;
+        if (issued < count) {
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const bool there = (unsigned)page[u] < (unsigned)step.pages;
-            const unsigned char* src = there ? a_head + (size_t)page[u] * step.page_bytes + in_page[u] : cache;
-            const unsigned bytes = there ? 16u : 0u;
+            for (int u = 0; u < UNITS; ++u) {
+                const int page = __shfl_sync(0xffffffffu, window, ap_tile % 16 * 2 + u), unit = a_unit + ap_tile * UNITS_A_TILE + u;
+                const bool there = (unsigned)page < (unsigned)step.pages;
+                const int in_page = step.unit_shift >= 0 ? unit & (units_a_page - 1) : unit % units_a_page;
+                const unsigned char* src = a_head + (size_t)(there ? (unsigned)page : 0u) * step.page_bytes + in_page * Unit::BYTES;
+                const unsigned bytes = there ? 16u : 0u;
 #pragma unroll
-            for (int c = 0; c < Unit::BYTES / 512; ++c) cp_async_16(dst + u * Unit::BYTES + c * 512, src + c * 512, bytes);
-            if (lane < Unit::BYTES % 512 / 16) cp_async_16(dst + u * Unit::BYTES + Unit::BYTES / 512 * 512, src + Unit::BYTES / 512 * 512, bytes);
-            arriving |= (there ? 1u : 0u) << u;
+                for (int c = 0; c < Unit::BYTES / 512; ++c) cp_async_16(dst + u * Unit::BYTES + c * 512, src + c * 512, bytes);
+                if (lane < Unit::BYTES % 512 / 16) cp_async_16(dst + u * Unit::BYTES + Unit::BYTES / 512 * 512, src + Unit::BYTES / 512 * 512, bytes);
+                arriving |= (there ? 1u : 0u) << u;
+            }
+            ++ap_tile;
+            ++issued;
         }
         cp_async_commit();
-        ++issued;
-        locate();
+        ask_pages();
     };
     // The queries of a piece: lane 4 g + t has features D/4 t .. of the head of column g.
     uint4 raw[D / 32];
@@ -337,7 +332,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     };
     Cursor at = start;
     Piece p = next_piece(at, count, prefix, step.kv_heads, head_groups);
-    locate();
+    ask_pages();
     ask_queries(p);
     issue();
 

@@ -152,12 +152,14 @@ template <typename F, int D> __device__ __forceinline__ F sum_of_squares(const F
     return ss;
 }
 
+// Returns the sum of squares.
 template <typename F, int D>
-__device__ __forceinline__ void norm(F (&v)[8], const float (&weight)[8], float eps, unsigned mask) {
+__device__ __forceinline__ F norm(F (&v)[8], const float (&weight)[8], float eps, unsigned mask) {
     const F ss = sum_of_squares<F, D>(v, mask);
     const F inv = sizeof(F) == 4 ? (F)rsqrtf((float)ss / (float)D + eps) : (F)rsqrt((double)ss / (double)D + (double)eps);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * (F)weight[e];
+    return ss;
 }
 
 // Returns the largest |first| + |second| of what is added.
@@ -287,7 +289,12 @@ qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, lon
                 float y[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[e] = x[e];
-                if (normed) norm<float, D>(y, weight, eps, mask);
+                // a sum of squares outside these bounds may have lost digits to the ends of the range (eps hides a small one)
+                bool kept = true;
+                if (normed) {
+                    const float ss = norm<float, D>(y, weight, eps, mask);
+                    kept = ss < 1e36f && (ss > 1e-30f || eps > 1e-20f);
+                }
                 float widest = 0.f;
                 if (turned) {
                     widest = rotate(y, turn, mask, part);
@@ -299,7 +306,7 @@ qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, lon
                 // The sum of squares is off by 12 roundings at most and half of that under the root, the root by 2^-22, the two products and the
                 // two of the rotation by one each: less than 2^-20 of |first| + |second|.
                 codes = quantise(y, widest * 1.9073486328125e-06f, mask, scale, sure);
-                sure = __all_sync(mask, sure);
+                sure = __all_sync(mask, sure && kept);
             }
             if (!sure) {
                 double y[8];

@@ -622,6 +622,10 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
     ops._check(out, "out", torch.bfloat16); ops._check(cache, "cache", torch.uint8)
     for name, t in (("block_tables", group.block_tables), ("positions", ctx.positions), ("token_slot", ctx.token_slot)):
         ops._check(t, name, torch.int32)
+    ops._check_device("paged_attention_fp4", q, out, cache, group.block_tables, ctx.positions, ctx.token_slot)
+    if group.block_tables.dim() != 2 or ctx.positions.numel() != tokens or ctx.token_slot.numel() != tokens:
+        raise ops.KernelError(f"paged_attention_fp4: block_tables {tuple(group.block_tables.shape)}, {ctx.positions.numel()} positions and "
+                              f"{ctx.token_slot.numel()} slots for {tokens} tokens")
     if ctx.all_decode:
         _fp4_tokens(q, q_stride, out, cache, group, ctx, heads, head_dim, scale, window)
         return out

@@ -55,6 +55,14 @@ def _check(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dens
         raise KernelError(f"{name} is not contiguous")
 
 
+def _check_device(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The kernels go to the current device's current stream, so their tensors have to be that device's."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"{name}: a tensor is on {t.device}, the current device is cuda:{device}")
+
+
 def embed(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     """out[t] = float(table[ids[t]]); out is float32 [tokens, hidden]."""
     _check(table, "table"); _check(ids, "ids", torch.int32); _check(out, "out", torch.float32)
@@ -318,6 +326,7 @@ def qk_norm_rope_cache_fp4(qkv: torch.Tensor, heads: int, kv_heads: int, head_di
         _check(k_weight, "k_weight", torch.float32)
     if rot is not None:
         _check(rot, "rot", torch.float32)
+    _check_device("qk_norm_rope_cache_fp4", qkv, q_weight, k_weight, rot, slots, cache if slots is not None else None, q_out)
     cache_at = None
     if slots is not None:
         _check(slots, "slots", torch.int32); _check(cache, "cache", torch.uint8)
@@ -326,9 +335,10 @@ def qk_norm_rope_cache_fp4(qkv: torch.Tensor, heads: int, kv_heads: int, head_di
         q, stride = qkv[:, :heads * head_dim], shape[1]
     else:
         _check(q_out, "q_out", torch.bfloat16, dense=False)
-        if q_out.stride(1) != 1:
-            raise KernelError("q_out must be rows of contiguous features")
-        q, stride = q_out, q_out.stride(0)
+        stride = q_out.stride(0) if tokens > 1 else q_out.shape[1]
+        if q_out.stride(1) != 1 or stride < q_out.shape[1]:
+            raise KernelError(f"qk_norm_rope_cache_fp4: q_out must be rows of contiguous features, it has strides {q_out.stride()}")
+        q = q_out
     _lib.fp4().call("mrun_qk_norm_rope_cache_fp4", qkv.data_ptr(), q.data_ptr(), stride, _address(q_weight), _address(k_weight), eps,
                     _address(rot), rotary_dim if rot is not None else 0, _address(slots), cache_at, tokens, heads, kv_heads, head_dim,
                     page_size, pages, _queue())
@@ -343,6 +353,7 @@ def fp4_pages(cache: torch.Tensor, head_dim: int, pages: torch.Tensor):
         raise KernelError(f"fp4_pages: pages is {tuple(shape)}, expected a list")
     held, kv_heads, page_size = check_fp4_cache(cache, head_dim)
     _check(cache, "cache", torch.uint8); _check(pages, "pages", torch.int32)
+    _check_device("fp4_pages", cache, pages)
     n = shape[0]
     k, v = torch.empty((2, n, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=cache.device).unbind(0)
     _lib.fp4().call("mrun_fp4_pages", cache.data_ptr(), pages.data_ptr(), k.data_ptr(), v.data_ptr(), n, kv_heads, head_dim, page_size, held,
@@ -360,6 +371,7 @@ def fp4_spans(cache: torch.Tensor, head_dim: int, block_tables: torch.Tensor, sp
         raise KernelError(f"fp4_spans: block_tables {tuple(block_tables.shape)}")
     held, kv_heads, page_size = check_fp4_cache(cache, head_dim)
     _check(cache, "cache", torch.uint8); _check(block_tables, "block_tables", torch.int32)
+    _check_device("fp4_spans", cache, block_tables, table, span_of_row)
     if (table is None) != (span_of_row is None) or (table is not None and (table.dim() != 2 or table.shape[0] != len(spans))):
         raise KernelError(f"fp4_spans: table {None if table is None else tuple(table.shape)} for {len(spans)} spans")
     for name, t in (("table", table), ("span_of_row", span_of_row)):

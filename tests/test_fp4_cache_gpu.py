@@ -140,6 +140,59 @@ def test_values_on_borders_and_beyond():
     assert torch.isnan(want).sum() == 48 and (want[1, :16] == 6).all() and (want[1, 16:32] == 7.5).all() and (want[1, 32:48] == 0).all()
 
 
+@pytest.mark.parametrize("rotary", [0, 64])
+def test_keys_far_from_one(rotary):
+    """Rows whose sum of squares leaves the range of 32 bits at either end, without and with an eps, rows with zeros, one value that
+    outweighs all others, a NaN and an infinity: the codes of the formula, which the 32-bit sums cannot tell."""
+    dim, heads = 64, 3
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(12, dim, generator=g).double()
+    x *= 10.0 ** torch.tensor([30, 20, 18.5, 8, 0, -8, -14, -17, -20, -30, -37, 0]).double().view(-1, 1)
+    x[4, ::2] = 0
+    x[11, 7] = 1e6
+    x = x.bfloat16()
+    bad = torch.randn(2, dim, generator=g).bfloat16()
+    bad[0, 3], bad[1, 40] = math.nan, math.inf
+    k = torch.cat([x, bad])
+    tokens = k.shape[0]
+    qkv = torch.cat([torch.zeros(tokens, dim, dtype=torch.bfloat16), k, torch.zeros(tokens, dim, dtype=torch.bfloat16)], 1)
+    weight = 1 + 0.2 * torch.randn(dim, generator=g)
+    rot = None
+    if rotary:
+        angle = torch.rand(tokens, rotary // 2, generator=g).double() * 6
+        rot = torch.stack([angle.cos(), angle.sin()], -1).float()
+    for eps in (0.0, 1e-6, 1e-19):
+        cache = torch.zeros(ops().fp4_cache_shape(1, 1, 16, dim), dtype=torch.uint8, device=DEV)
+        ops().qk_norm_rope_cache_fp4(qkv.to(DEV), 1, 1, dim, weight.to(DEV), weight.to(DEV), eps, to(rot), rotary,
+                                     torch.arange(tokens, dtype=torch.int32, device=DEV), cache)
+        got = ops().fp4_pages(cache, dim, torch.zeros(1, dtype=torch.int32, device=DEV))[0][0, 0, :tokens].double().cpu()
+        y = rotated(normed(k.double().view(tokens, 1, dim), weight, float(torch.tensor(eps, dtype=torch.float32))), rot)
+        want = plain_fp4.held(y)[0].view(tokens, dim)
+        assert torch.equal(got[:12], want[:12]) and torch.isnan(got[12]).all() and torch.equal(torch.isnan(got[13]), torch.isnan(want[13]))
+
+
+def test_calls_on_two_streams_at_once():
+    heads, kv_heads, dim, page = 32, 8, 128, 16
+    lengths = [3000, 20, 1999, 640]
+    c = Filled(lengths, kv_heads, dim, page, seed=8)
+    table = c.table.to(DEV)
+    steps = [step_of([(j, 1, n - 1 - 3 * i) for j, n in enumerate(lengths)], table, page) for i in range(2)]
+    q = [c.queries(4, heads, dim).to(DEV) for _ in range(2)]
+    out = [[torch.zeros_like(q[0]) for _ in range(20)] for _ in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                attention(q[i], heads * dim, out[i][turn], c.cache, steps[i][1], steps[i][0], heads, dim, dim ** -0.5)
+    torch.cuda.synchronize()
+    for i in range(2):
+        want = torch.stack([plain_fp4.attend(q[i][j:j + 1].cpu().view(1, heads, dim), c.k[j], c.v[j], [n - 1 - 3 * i], dim ** -0.5).view(-1)
+                            for j, n in enumerate(lengths)])
+        close(out[i][0], want, c.v, 2.0 ** -10)
+        assert all(torch.equal(out[i][0], x) for x in out[i])
+
+
 def step_of(segments, table, page, tokens=None):
     """A step over segments (slot, tokens, first position), with padding rows up to ``tokens``."""
     from mrun_b200.engine.batch import GroupView, HostStaging, SegmentInfo, StepContext
