@@ -17,16 +17,18 @@ using bf16 = __nv_bfloat16;
 // A key is quantised from its unrounded value, and which side of a border between two codes a value
 // falls on decides a whole step of the code.  So that the codes are those of the formula and do not depend on
 // the order of a sum, a key is computed in 32 bits with a bound of its error, quantised at both ends of the bound, and where
-// the two differ (one head in two hundred) computed again in 64 bits.  In 64 bits throughout the kernel took 32 us for
-// 2,048 tokens of 32 + 8 + 8 heads of 128.
+// the two differ (about one head in a hundred) computed again in 64 bits.  In 64 bits throughout a step of one
+// token took 10.5 us with its read back, 4.2 so.
 // A value is a bfloat16: its quotient by a scale of 4 bits is a border (at most 3 bits) exactly or 2^-9 away from it.
 //
-// D / 8 lanes take TOGETHER heads of a token, eight features a lane, all asked for before the first is worked on: with one head at a time
-// a multiprocessor had 12 KB under way, where the memory's rate takes three times that (34 us for the write and read back of 2,048 tokens).  A step of few heads
-// gives each lanes of its own.
+// D / 8 lanes take TOGETHER heads of a token, eight features a lane, all asked for before the first is worked on, and the token's cosines and
+// sines once for them.  What bounds it is the chain of a head (load, sum over the lanes, root, rotation across lanes, store) with 25 warps a multiprocessor
+// to hide it: 21.7 us for 2,048 tokens of 32 + 8 + 8 heads of 128 (the queries alone 15 to 17; the write of bfloat16 pages 13.7; the bytes
+// take 6.8) with two heads and four blocks a multiprocessor; 23.2 with four heads and three blocks, 28 with one; asking for the next heads
+// while working (25.4) and four chains side by side (26.6) spill.  A step of few heads gives each lanes of its own.
 // ------------------------------------------------------------------------------------------
 constexpr int STORE_THREADS = 256;
-constexpr int HEADS_TOGETHER = 4;
+constexpr int HEADS_TOGETHER = 2;
 constexpr int HEADS_AT_ONCE = 8192;        // a step of up to this many heads gives each lanes of its own
 
 // The byte of the scale nearest to `wanted` (0 .. 10,240), ties to the even byte.  `wanted` has a bit set below
@@ -42,11 +44,11 @@ __device__ __forceinline__ float scale_value(unsigned byte) {
 }
 
 // Eight 4-bit floats, the first in the lowest bits: nearest, ties to the even code, at most 6.
-__device__ __forceinline__ unsigned codes_of(const float (&f)[8]) {
+__device__ __forceinline__ unsigned codes_of(const float2 (&f)[4]) {
     unsigned out;
     asm("{\n.reg .b8 c0, c1, c2, c3;\ncvt.rn.satfinite.e2m1x2.f32 c0, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 c1, %4, %3;\n"
         "cvt.rn.satfinite.e2m1x2.f32 c2, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 c3, %8, %7;\nmov.b32 %0, {c0, c1, c2, c3};\n}"
-        : "=r"(out) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+        : "=r"(out) : "f"(f[0].x), "f"(f[0].y), "f"(f[1].x), "f"(f[1].y), "f"(f[2].x), "f"(f[2].y), "f"(f[3].x), "f"(f[3].y));
     return out;
 }
 
@@ -76,53 +78,63 @@ __device__ __forceinline__ unsigned quantise(const double (&x)[8], unsigned mask
     const double s = scale_value(scale);
     // A shade more than 1 / s, so that a quotient that is a border exactly is not cut below it.
     const double inverse = s > 0.0 ? 1.0 / s * (1.0 + 8.8817841970012523e-16) : 0.0;
-    float f[8];
+    float2 f[4];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        f[e] = __double2float_rz(x[e] * inverse);
-        if ((double)f[e] * s != x[e]) f[e] = __uint_as_float(__float_as_uint(f[e]) | 1u);
+        float& part = e % 2 ? f[e / 2].y : f[e / 2].x;
+        part = __double2float_rz(x[e] * inverse);
+        if ((double)part * s != x[e]) part = __uint_as_float(__float_as_uint(part) | 1u);
     }
     return codes_of(f);
 }
 
-// of floats that hold bfloat16 values,
-__device__ __forceinline__ unsigned quantise(const float (&x)[8], unsigned mask, unsigned& scale) {
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+
+// To 12 bits, by two subtractions (4,097 = 2^12 + 1): of a quotient that is a number of few bits exactly, and was off by some of its last
+// of 24, that number; any quotient that is 2^-10 away from it stays on its side.  One by one: the compiler makes one operation of
+// a product of pairs and the sum behind it.
+__device__ __forceinline__ float to_12_bits(float v) {
+    const float wide = __fmul_rn(v, 4097.f);
+    return __fsub_rn(wide, __fsub_rn(wide, v));
+}
+
+// The largest magnitude of the 16 features that two neighbouring lanes hold, as its bits.
+__device__ __forceinline__ unsigned largest_of(const float2 (&x)[4], unsigned mask) {
     unsigned top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, magnitude(x[e]));
-    top = max(top, __shfl_xor_sync(mask, top, 1));
+    for (int e = 0; e < 4; ++e) top = max(top, max(magnitude(x[e].x), magnitude(x[e].y)));
+    return max(top, __shfl_xor_sync(mask, top, 1));
+}
+
+// of floats that hold bfloat16 values,
+__device__ __forceinline__ unsigned quantise(const float2 (&x)[4], unsigned mask, unsigned& scale) {
+    const unsigned top = largest_of(x, mask);
     if (top >= INFINITE) {
         scale = FP4_NAN_SCALE;
         return 0u;
     }
-    scale = scale_byte(fminf(__fdiv_rn(__uint_as_float(top), 6.f), 10240.f));
-    const float s = scale_value(scale), inverse = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
-    float f[8];
+    scale = scale_byte(to_12_bits(fminf(__uint_as_float(top) * (1.f / 6.f), 10240.f)));
+    const float s = scale_value(scale), inverse = s > 0.f ? __fdividef(1.f, s) : 0.f;
+    float2 f[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {    // the quotient to 12 bits: one that is a border exactly comes out as it, any other stays on its side
-        const float y = __fmul_rn(x[e], inverse), wide = __fmul_rn(y, 4097.f);
-        f[e] = __fsub_rn(wide, __fsub_rn(wide, y));
-    }
+    for (int e = 0; e < 4; ++e) f[e] = make_float2(to_12_bits(__fmul_rn(x[e].x, inverse)), to_12_bits(__fmul_rn(x[e].y, inverse)));
     return codes_of(f);
 }
 
 // and of floats that are within `off` of the values meant.  `sure`: neither the scale nor a code depends on where within.
-__device__ __forceinline__ unsigned quantise(const float (&x)[8], float off, unsigned mask, unsigned& scale, bool& sure) {
-    unsigned top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, magnitude(x[e]));
-    top = max(top, __shfl_xor_sync(mask, top, 1));
+__device__ __forceinline__ unsigned quantise(const float2 (&x)[4], float off, unsigned mask, unsigned& scale, bool& sure) {
+    const unsigned top = largest_of(x, mask);
     const float largest = __uint_as_float(top);
     scale = scale_byte(fminf((largest + off) * (1.f / 6.f) * 1.000001f, 10240.f));
     sure = top < INFINITE && off < INFINITY && scale == scale_byte(fminf(fmaxf(largest - off, 0.f) * (1.f / 6.f) * 0.999999f, 10240.f));
     const float s = scale_value(scale), inverse = s > 0.f ? __fdividef(1.f, s) : 0.f;
     // the quotients are at most 6.4 where they are not far beyond the last border, and off by 2^-21 of them
     const float away = fmaf(off, inverse * 1.000001f, 4e-6f);
-    float low[8], high[8];
+    float2 low[4], high[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        low[e] = fmaf(x[e], inverse, -away);
-        high[e] = fmaf(x[e], inverse, away);
+    for (int e = 0; e < 4; ++e) {
+        low[e] = __ffma2_rn(x[e], twice(inverse), twice(-away));
+        high[e] = __ffma2_rn(x[e], twice(inverse), twice(away));
     }
     const unsigned codes = codes_of(low);
     sure = sure && codes == codes_of(high);
@@ -130,51 +142,69 @@ __device__ __forceinline__ unsigned quantise(const float (&x)[8], float off, uns
 }
 
 // Eight floats of `src`, on 16 bytes.
-__device__ __forceinline__ void load8(float (&v)[8], const float* __restrict__ src) {
+__device__ __forceinline__ void load8(float2 (&v)[4], const float* __restrict__ src) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    v[0] = make_float2(a.x, a.y); v[1] = make_float2(a.z, a.w); v[2] = make_float2(b.x, b.y); v[3] = make_float2(b.z, b.w);
 }
 
-// What a lane needs of the norm and the rotation of its eight features.  Pairs (j, j + half): with a half of a multiple of eight a
+// What a lane needs of the rotation of its eight features.  Pairs (j, j + half): with a half of a multiple of eight a
 // lane's partners are the eight features of another lane, and it holds their cosines and sines (these with their sign).
 struct Turn {
     int partner;            // the lane of the group, itself where nothing turns
     bool turns;
-    float c[8], s[8];
+    float2 c[4], s[4];
 };
 
-template <typename F, int D> __device__ __forceinline__ F sum_of_squares(const F (&v)[8], unsigned mask) {
-    F ss = 0;
+__device__ __forceinline__ float squares(const float2 (&v)[4]) {
+    float2 two = __fmul2_rn(v[0], v[0]);
+#pragma unroll
+    for (int e = 1; e < 4; ++e) two = __ffma2_rn(v[e], v[e], two);
+    return two.x + two.y;
+}
+__device__ __forceinline__ void scale_by(float2 (&v)[4], float inv, const float2 (&weight)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(__fmul2_rn(v[e], twice(inv)), weight[e]);
+}
+
+// The norm in 32 bits, two features an instruction; returns the sum of squares.
+template <int D> __device__ __forceinline__ float norm(float2 (&v)[4], const float2 (&weight)[4], float eps, unsigned mask) {
+    float ss = squares(v);
+#pragma unroll
+    for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+    scale_by(v, rsqrtf(ss * (1.f / D) + eps), weight);
+    return ss;
+}
+template <int D> __device__ __forceinline__ void norm(double (&v)[8], const float2 (&weight)[4], float eps, unsigned mask) {
+    double ss = 0.0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
 #pragma unroll
     for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-    return ss;
+    const double inv = rsqrt(ss / D + (double)eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * (double)(e % 2 ? weight[e / 2].y : weight[e / 2].x);
 }
 
-// Returns the sum of squares.
-template <typename F, int D>
-__device__ __forceinline__ F norm(F (&v)[8], const float (&weight)[8], float eps, unsigned mask) {
-    const F ss = sum_of_squares<F, D>(v, mask);
-    const F inv = sizeof(F) == 4 ? (F)rsqrtf((float)ss / (float)D + eps) : (F)rsqrt((double)ss / (double)D + (double)eps);
+// With WIDEST returns the largest |first| + |second| of what is added.
+template <bool WIDEST> __device__ __forceinline__ float rotate(float2 (&v)[4], const Turn& turn, unsigned mask, int part) {
+    const int from = (int)(threadIdx.x & 31) - part + turn.partner;
+    float widest = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * (F)weight[e];
-    return ss;
-}
-
-// Returns the largest |first| + |second| of what is added.
-template <typename F>
-__device__ __forceinline__ F rotate(F (&v)[8], const Turn& turn, unsigned mask, int part) {
-    const int base = (int)(threadIdx.x & 31) - part;
-    F widest = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const F other = __shfl_sync(mask, v[e], base + turn.partner);
-        const F both = (v[e] < 0 ? -v[e] : v[e]) + (other < 0 ? -other : other);
-        widest = both > widest ? both : widest;
-        if (turn.turns) v[e] = v[e] * (F)turn.c[e] + other * (F)turn.s[e];
+    for (int e = 0; e < 4; ++e) {
+        const float2 other = make_float2(__shfl_sync(mask, v[e].x, from), __shfl_sync(mask, v[e].y, from));
+        if constexpr (WIDEST) widest = fmaxf(widest, fmaxf(fabsf(v[e].x) + fabsf(other.x), fabsf(v[e].y) + fabsf(other.y)));
+        if (turn.turns) v[e] = __ffma2_rn(v[e], turn.c[e], __fmul2_rn(other, turn.s[e]));
     }
     return widest;
+}
+__device__ __forceinline__ void rotate(double (&v)[8], const Turn& turn, unsigned mask, int part) {
+    const int from = (int)(threadIdx.x & 31) - part + turn.partner;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const double other = __shfl_sync(mask, v[e], from);
+        if (turn.turns)
+            v[e] = v[e] * (double)(e % 2 ? turn.c[e / 2].y : turn.c[e / 2].x) + other * (double)(e % 2 ? turn.s[e / 2].y : turn.s[e / 2].x);
+    }
 }
 
 // The rotation with the partners fetched one by one through `stage`, a row of D of the group's own.
@@ -194,7 +224,7 @@ __device__ __forceinline__ void rotate_staged(F (&v)[8], const float2* __restric
 
 // STAGED: rotary sizes that are no multiple of 16, and weights or tables off 16 bytes; keys in 64 bits throughout.
 template <int D, bool STAGED, int TOGETHER>
-__global__ void __launch_bounds__(STORE_THREADS, STAGED ? 1 : 3)
+__global__ void __launch_bounds__(STORE_THREADS, STAGED ? 1 : 4)
 qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, long q_stride,
                               const float* __restrict__ q_weight, const float* __restrict__ k_weight, float eps,
                               const float2* __restrict__ rot, int half, const int* __restrict__ slots, unsigned char* __restrict__ cache,
@@ -225,14 +255,15 @@ qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, lon
         turn.turns = part < 2 * away;
         turn.partner = turn.turns ? (low ? part + away : part - away) : part;
         if (turn.turns) {
-            float two[2][8];
+            float2 two[2][4];                                      // (cosine, sine) of a pair each
             const float* src = reinterpret_cast<const float*>(cs + (low ? part : turn.partner) * 8);
             load8(two[0], src);
             load8(two[1], src + 8);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                turn.c[e] = two[e / 4][e % 4 * 2];
-                turn.s[e] = low ? -two[e / 4][e % 4 * 2 + 1] : two[e / 4][e % 4 * 2 + 1];
+            for (int e = 0; e < 4; ++e) {
+                const float2 a = two[e / 2][e % 2 * 2], b = two[e / 2][e % 2 * 2 + 1];
+                turn.c[e] = make_float2(a.x, b.x);
+                turn.s[e] = low ? make_float2(-a.y, -b.y) : make_float2(a.y, b.y);
             }
         }
     }
@@ -250,35 +281,38 @@ qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, lon
         if (head >= per_token) break;
         const bool is_q = head < heads, is_k = !is_q && head < heads + kv_heads;
         if (!is_q && !writes) break;                               // keys and values lie behind the queries
-        float weight[8];
+        float2 weight[4];
         if (normed && (is_q || is_k)) {
             const float* weights = is_q ? q_weight : k_weight;
             if constexpr (STAGED) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) weight[e] = weights[part * 8 + e];
+                for (int e = 0; e < 4; ++e) weight[e] = make_float2(weights[part * 8 + 2 * e], weights[part * 8 + 2 * e + 1]);
             } else {
                 load8(weight, weights + part * 8);
             }
         }
-        float x[8];
+        float2 x[4];
         {
             const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = __bfloat1622float2(pairs[e]);
-                x[2 * e] = f.x; x[2 * e + 1] = f.y;
-            }
+            for (int e = 0; e < 4; ++e) x[e] = __bfloat1622float2(pairs[e]);
         }
         if (is_q) {
-            if (normed) norm<float, D>(x, weight, eps, mask);
+            if (normed) norm<D>(x, weight, eps, mask);
             if (turned) {
-                if constexpr (STAGED) rotate_staged(x, cs, half, mask, part, reinterpret_cast<float*>(stage));
-                else rotate(x, turn, mask, part);
+                if constexpr (STAGED) {
+                    float y[8] = {x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
+                    rotate_staged(y, cs, half, mask, part, reinterpret_cast<float*>(stage));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = make_float2(y[2 * e], y[2 * e + 1]);
+                } else {
+                    rotate<false>(x, turn, mask, part);
+                }
             }
             uint4 packed;
             __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(&packed);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) out[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+            for (int e = 0; e < 4; ++e) out[e] = __floats2bfloat162_rn(x[e].x, x[e].y);
             *reinterpret_cast<uint4*>(q_out + (size_t)t * q_stride + (size_t)head * D + part * 8) = packed;
             continue;
         }
@@ -286,21 +320,19 @@ qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, lon
         if (is_k && (normed || turned)) {
             bool sure = false;
             if constexpr (!STAGED) {
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = x[e];
+                float2 y[4] = {x[0], x[1], x[2], x[3]};
                 // a sum of squares outside these bounds may have lost digits to the ends of the range (eps hides a small one)
                 bool kept = true;
                 if (normed) {
-                    const float ss = norm<float, D>(y, weight, eps, mask);
+                    const float ss = norm<D>(y, weight, eps, mask);
                     kept = ss < 1e36f && (ss > 1e-30f || eps > 1e-20f);
                 }
                 float widest = 0.f;
                 if (turned) {
-                    widest = rotate(y, turn, mask, part);
+                    widest = rotate<true>(y, turn, mask, part);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) widest = fmaxf(widest, fabsf(y[e]));
+                    for (int e = 0; e < 4; ++e) widest = fmaxf(widest, fmaxf(fabsf(y[e].x), fabsf(y[e].y)));
                 }
                 widest = fmaxf(widest, __shfl_xor_sync(mask, widest, 1));
                 // The sum of squares is off by 12 roundings at most and half of that under the root, the root by 2^-22, the two products and the
@@ -311,8 +343,8 @@ qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, lon
             if (!sure) {
                 double y[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = x[e];
-                if (normed) norm<double, D>(y, weight, eps, mask);
+                for (int e = 0; e < 8; ++e) y[e] = e % 2 ? x[e / 2].y : x[e / 2].x;
+                if (normed) norm<D>(y, weight, eps, mask);
                 if (turned) {
                     if constexpr (STAGED) rotate_staged(y, cs, half, mask, part, stage);
                     else rotate(y, turn, mask, part);
