@@ -2,7 +2,7 @@
 //
 //   o_h = sum_j p_j v_j / sum_j p_j,   p_j = exp2(scale_log2 q_h . k_j - m_h),   j the visible keys whose page is held
 //
-// What bounds it: a key and its value are 2.25 D / 2 bytes of DRAM, a quarter of their bfloat16 size, so the
+// What bounds it: a key and its value are 9/8 D bytes of DRAM, 3.6 times fewer than in bfloat16, so the
 // work on them counts.  At 6.5 TB/s a multiprocessor gets a key and value of 128 features every 6 clocks, 42
 // codes a clock.  cvt.e2m1x2 makes two halves of a byte in one instruction of the integer pipe (two a clock and
 // multiprocessor; integer codes by mask and subtraction take three times as many); times their scale (exact) they are
@@ -24,6 +24,12 @@
 // (token, kv head, group of heads) pair.  The tiles (8 units) of all pairs lie in one list, cut evenly among the
 // blocks that the device holds at once; a pair that lies in several blocks leaves its pieces in scratch, and
 // a second kernel, whose launch overlaps the first one's end, adds them in block order.
+//
+// Measured (B200): 64 requests of up to 8,192 keys, 32 heads over 8 of 128 (456 MB): 90 us at 1,965 MHz, 5.0 TB/s; its copies alone take 84, about
+// ten of them the start (positions, pages, first keys) and the second kernel.  267 instructions a unit, 64 of them conversions (the integer pipe
+// is 48 % busy) and 64 multiplications.  In a run of seconds the power cap brings the clock to 1,600 MHz, and it takes 102.
+// One request of 1,024 keys: 6.7 us, a chain of latencies.  A ring of three stages, twelve warps a multiprocessor instead of sixteen, pages of 64
+// or 256 keys: the same within 2 %.
 #include <atomic>
 #include <cfloat>
 #include <cuda_fp16.h>
