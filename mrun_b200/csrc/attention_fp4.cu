@@ -21,14 +21,15 @@
 //
 // A block is four warps; each copies its own units (two at a time, 32 keys) with cp.async into a ring of its own while it
 // works on the two before, across pairs: no barrier but where a pair's pieces meet.  Every warp of a block works on the same
-// (token, kv head, group of heads) pair.  The tiles (8 units) of all pairs lie in one list, cut evenly among the
-// blocks that the device holds at once; a pair that lies in several blocks leaves its pieces in scratch, and
-// a second kernel, whose launch overlaps the first one's end, adds them in block order.
+// (token, kv head, group of heads) pair.  The tiles (8 units) of short contexts are cut among the one to eight blocks of a pair's
+// cluster, which add their pieces through distributed shared memory.  Those of long ones lie in one list: dealt to the blocks that the
+// device holds at once by whole pairs where that is even, and otherwise cut evenly, so that a pair in several
+// blocks leaves its pieces in scratch, and a second kernel, whose launch overlaps the first one's end, adds them in block order.
 //
-// Measured (B200): 64 requests of up to 8,192 keys, 32 heads over 8 of 128 (456 MB): 90 us at 1,965 MHz, 5.0 TB/s; its copies alone take 84, about
-// ten of them the start (positions, pages, first keys) and the second kernel.  267 instructions a unit, 64 of them conversions (the integer pipe
-// is 48 % busy) and 64 multiplications.  In a run of seconds the power cap brings the clock to 1,600 MHz, and it takes 102.
-// One request of 1,024 keys: 6.7 us, a chain of latencies.  A ring of three stages, twelve warps a multiprocessor instead of sixteen, pages of 64
+// Measured (B200): 64 requests of up to 8,192 keys, 32 heads over 8 of 128 (456 MB): 84 us at 1,965 MHz, 5.5 TB/s, the start (positions, pages, first keys)
+// and the second launch among them.  267 instructions a unit, 64 of them conversions (the integer pipe
+// is 48 % busy) and 64 multiplications.  In a run of seconds the power cap brings the clock to 1,600 MHz.
+// One request of 1,024 keys: 5.6 us, a chain of latencies.  A ring of three stages, twelve warps a multiprocessor instead of sixteen, pages of 64
 // or 256 keys: the same within 2 %.
 #include <atomic>
 #include <cfloat>
@@ -49,6 +50,7 @@ constexpr int STAGES = 2;
 constexpr int UNITS_A_TILE = WARPS * UNITS;
 constexpr int MAX_TOKENS = 256;         // tokens of one launch (their plan lies in shared memory beside the rings of four blocks)
 constexpr int MERGE_THREADS = 128;
+constexpr int MAX_CLUSTER = 8;          // blocks of a cluster that every device takes
 constexpr float LIFT = 5.f;             // log2 of the factor that P carries
 constexpr float SLACK = 8.f;            // how far a score may pass the running maximum (base 2)
 
@@ -164,7 +166,7 @@ struct Shape {
     static constexpr int RING_BYTES = WARPS * STAGES * UNITS * Fp4Unit<D>::BYTES;
     static constexpr int MERGE_BYTES = WARPS * HEADS * ROW * 4;
     // ... and per token its prefix of tiles, position and block-table row
-    static size_t bytes(int tokens) { return RING_BYTES + MERGE_BYTES + (size_t)(3 * tokens + 1) * 4; }
+    static size_t bytes(int tokens) { return RING_BYTES + MERGE_BYTES + (size_t)(3 * tokens + 1) * 4; }        // a cluster's blocks: 0 tokens
 };
 
 // Which rows of the step a launch's tokens are: the first ones, or (listed) these, given by value so that no copy
@@ -176,11 +178,11 @@ struct Rows {
 };
 
 // Sums tiles_of over the tokens into prefix[0 .. tokens], positions into held[0 .. tokens) and block-table rows into
-// held[tokens .. 2 tokens); all threads of the block.
-__device__ __forceinline__ void make_plan(int* prefix, int* held, const int* __restrict__ positions, const int* __restrict__ token_slot,
+// held[tokens .. 2 tokens); all threads of the block.  Returns the most tiles that a token has.
+__device__ __forceinline__ int make_plan(int* prefix, int* held, const int* __restrict__ positions, const int* __restrict__ token_slot,
                                           const Rows& rows, int tokens, int window, int table_units, int* scratch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int carried = 0;
+    int carried = 0, most = 0;
     if (threadIdx.x == 0) prefix[0] = 0;
     for (int first = 0; first < tokens; first += THREADS) {
         const int t = first + threadIdx.x;
@@ -193,6 +195,7 @@ __device__ __forceinline__ void make_plan(int* prefix, int* held, const int* __r
             held[tokens + t] = table_row;
         }
         int sum = tiles_of(pos, window, table_units);
+        most = max(most, sum);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int below = __shfl_up_sync(0xffffffffu, sum, o);
@@ -213,7 +216,12 @@ __device__ __forceinline__ void make_plan(int* prefix, int* held, const int* __r
         if (t < tokens) prefix[t + 1] = before + sum;
         __syncthreads();
     }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) scratch[WARPS + warp] = most;
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) most = max(most, scratch[WARPS + w]);
+    return most;
 }
 
 // Tiles that a block takes.
@@ -230,10 +238,33 @@ struct Step {
     float scale_log2;
     float* part_o;               // [blocks, 2, HEADS, D]
     float2* part_ml;             // [blocks, 2, HEADS]: maximum, sum
-    int* plan;                   // [tokens + 1]: the prefix of tiles
+    int* plan;                   // [tokens + 1] the prefix of tiles, and whether every pair lies in one block
 };
 
-template <int D, bool FOUR>
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// Values at `own`, an address of this block's shared memory, in block `rank` of the cluster.
+__device__ __forceinline__ unsigned in_block(const void* own, unsigned rank) {
+    unsigned out;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(out) : "r"(smem_addr(own)), "r"(rank));
+    return out;
+}
+__device__ __forceinline__ float4 load4_in(unsigned address) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address));
+    return v;
+}
+__device__ __forceinline__ float2 load2_in(unsigned address) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(address));
+    return v;
+}
+
+// CLUSTERED: grid (blocks of a cluster, tokens * pairs), a cluster a pair: its tiles are cut evenly among its blocks, whose pieces the first
+// block adds through distributed shared memory.  Neither plan nor scratch nor a second kernel.
+template <int D, bool FOUR, bool CLUSTERED>
 __global__ void __launch_bounds__(THREADS, FOUR ? 4 : 3)     // eight heads: 150 registers a thread without spills, 31 us where four blocks took 32
 decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsigned char* __restrict__ cache, const Step step,
                   const __grid_constant__ Rows rows) {
@@ -242,7 +273,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     constexpr int HEADS = Sh::HEADS, MINE = Sh::MINE, WORDS_K = D / 32, WORDS_V = D / 64, TILES_M = D / 32;
     constexpr int COLUMNS = FOUR ? 1 : 2;              // products that give 32 features of the heads
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int scratch[WARPS];
+    __shared__ int scratch[2 * WARPS];
     float* merge = reinterpret_cast<float*>(smem + Sh::RING_BYTES);              // [WARPS][HEADS][ROW]
     int* prefix = reinterpret_cast<int*>(smem + Sh::RING_BYTES + Sh::MERGE_BYTES);
     int* held_pos = prefix + step.tokens + 1;
@@ -252,33 +283,65 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     const int group = step.heads / step.kv_heads, head_groups = (group + HEADS - 1) / HEADS;
     const int units_a_page = step.page_size / FP4_TOKENS, table_units = step.max_blocks * units_a_page, pairs = step.kv_heads * head_groups;
 
-    make_plan(prefix, held_pos, step.positions, step.token_slot, rows, step.tokens, step.window, table_units, scratch);
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i <= step.tokens; i += THREADS) step.plan[i] = prefix[i];
-    // rows without a tile (padding) come out as zeros
-    for (int tok = blockIdx.x; tok < step.tokens; tok += gridDim.x)
-        if (prefix[tok] == prefix[tok + 1])
-            for (int i = threadIdx.x; i < step.heads * D / 2; i += THREADS)
-                reinterpret_cast<unsigned*>(out + (size_t)rows.of(tok) * step.heads * D)[i] = 0u;
+    Piece p = {};
+    Cursor at = {};
+    int count, my_pos = -1, my_row = -1;               // CLUSTERED: of the pair's token
+    if constexpr (CLUSTERED) {
+        p.tok = blockIdx.y / pairs;
+        const int pair = blockIdx.y - p.tok * pairs;
+        p.kvh = head_groups == 1 ? pair : pair / head_groups;
+        p.hg = pair - p.kvh * head_groups;
+        my_pos = step.positions[rows.of(p.tok)];
+        my_row = step.token_slot[rows.of(p.tok)];
+        const int tiles = tiles_of(my_pos, step.window, table_units);
+        if (tiles == 0) {                              // the whole cluster leaves
+            const int heads_here = min(HEADS, group - p.hg * HEADS);
+            if (blockIdx.x == 0)
+                for (int i = threadIdx.x; i < heads_here * D / 2; i += THREADS)
+                    reinterpret_cast<unsigned*>(out + ((size_t)rows.of(p.tok) * step.heads + p.kvh * group + p.hg * HEADS) * D)[i] = 0u;
+            return;
+        }
+        const int base = tiles / (int)gridDim.x, more = tiles - base * (int)gridDim.x, rank = blockIdx.x;
+        p.tile0 = rank * base + min(rank, more);
+        count = p.tiles = base + (rank < more ? 1 : 0);
+    } else {
+        const int most = make_plan(prefix, held_pos, step.positions, step.token_slot, rows, step.tokens, step.window, table_units, scratch);
+        if (blockIdx.x == 0)
+            for (int i = threadIdx.x; i <= step.tokens; i += THREADS) step.plan[i] = prefix[i];
+        // rows without a tile (padding) come out as zeros
+        for (int tok = blockIdx.x; tok < step.tokens; tok += gridDim.x)
+            if (prefix[tok] == prefix[tok + 1])
+                for (int i = threadIdx.x; i < step.heads * D / 2; i += THREADS)
+                    reinterpret_cast<unsigned*>(out + (size_t)rows.of(tok) * step.heads * D)[i] = 0u;
 
-    const int total = prefix[step.tokens] * pairs, per = tiles_a_block(total, gridDim.x), begin = blockIdx.x * per;
-    if (begin >= total) return;
-    const int count = min(per, total - begin);
-    Cursor start;
-    {   // the token whose tiles hold the block's first one
-        int low = 0, high = step.tokens - 1;
+        // Whole pairs to a block where that leaves none with much more than its share: no piece is handed over then (64 requests of 512 to
+        // 1,024 keys, 8 kv heads: 17 us where the even cut takes 21).
+        const int total = prefix[step.tokens] * pairs, per = tiles_a_block(total, gridDim.x);
+        const int pairs_a_block = (step.tokens * pairs + (int)gridDim.x - 1) / (int)gridDim.x;
+        const bool aligned = pairs_a_block * most <= per + max(2, per / 4);
+        if (blockIdx.x == 0 && threadIdx.x == 0) step.plan[step.tokens + 1] = aligned;
+        auto tiles_before = [&](int pair) {            // of all tokens' pairs
+            if (pair >= step.tokens * pairs) return total;
+            const int tok = pair / pairs;
+            return prefix[tok] * pairs + (pair - tok * pairs) * (prefix[tok + 1] - prefix[tok]);
+        };
+        const int begin = aligned ? tiles_before(min((int)blockIdx.x * pairs_a_block, step.tokens * pairs)) : min((int)blockIdx.x * per, total);
+        count = (aligned ? tiles_before(min(((int)blockIdx.x + 1) * pairs_a_block, step.tokens * pairs)) : min(begin + per, total)) - begin;
+        if (count == 0) return;
+        int low = 0, high = step.tokens - 1;           // the token whose tiles hold the block's first one
         while (low < high) {
             const int mid = (low + high) / 2;
             if (prefix[mid + 1] * pairs <= begin) low = mid + 1;
             else high = mid;
         }
-        start.tok = low;
-        start.rest = begin - prefix[low] * pairs;
+        at.tok = low;
+        at.rest = begin - prefix[low] * pairs;
     }
+    auto position = [&](const Piece& of) { return CLUSTERED ? my_pos : held_pos[of.tok]; };
 
     // ---- the copies: this warp's units of every tile, one tile ahead of the work.  The pages of 16 tiles' units are asked for
     // together, one a lane, a tile before the first of them is copied.
-    Cursor ahead = start;
+    Cursor ahead = at;
     Piece ap = {};
     int ap_tile = 0, issued = 0;
     int a_unit = 0;                                    // this warp's first unit of the piece that is copied
@@ -289,13 +352,13 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     auto ask_pages = [&]() {                           // for the tile that is copied next
         if (issued >= count) return;
         if (ap_tile == ap.tiles) {
-            ap = next_piece(ahead, count - issued, prefix, step.kv_heads, head_groups);
+            ap = CLUSTERED ? p : next_piece(ahead, count - issued, prefix, step.kv_heads, head_groups);
             ap_tile = 0;
-            a_unit = first_visible(held_pos[ap.tok], step.window) / FP4_TOKENS + ap.tile0 * UNITS_A_TILE + warp * UNITS;
+            a_unit = first_visible(position(ap), step.window) / FP4_TOKENS + ap.tile0 * UNITS_A_TILE + warp * UNITS;
             a_head = cache + (size_t)ap.kvh * units_a_page * Unit::BYTES + lane * 16;
         }
         if (ap_tile % 16 == 0) {
-            const int table_row = held_row[ap.tok], last = min(held_pos[ap.tok] / FP4_TOKENS, table_units - 1);
+            const int table_row = CLUSTERED ? my_row : held_row[ap.tok], last = min(position(ap) / FP4_TOKENS, table_units - 1);
             const int unit = a_unit + (ap_tile + lane / 2) * UNITS_A_TILE + lane % 2;
             window = -1;
             if (unit <= last && table_row >= 0 && table_row < step.table_rows)
@@ -336,14 +399,14 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             if (h < group - p.hg * HEADS) raw[c] = *reinterpret_cast<const uint4*>(src + c * 8);
         }
     };
-    Cursor at = start;
-    Piece p = next_piece(at, count, prefix, step.kv_heads, head_groups);
+    if constexpr (!CLUSTERED) p = next_piece(at, count, prefix, step.kv_heads, head_groups);
     ask_pages();
     ask_queries(p);
     issue();
 
-    for (int done = 0, seg = 0; done < count; ++seg) {
-        const int pos = held_pos[p.tok], lo = first_visible(pos, step.window), first_unit = lo / FP4_TOKENS;
+    int done = 0, seg = 0;
+    do {
+        const int pos = position(p), lo = first_visible(pos, step.window), first_unit = lo / FP4_TOKENS;
         const size_t row = rows.of(p.tok);
         const int head0 = p.kvh * group + p.hg * HEADS, heads_here = min(HEADS, group - p.hg * HEADS);
 
@@ -547,8 +610,11 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
         }
 
         // ---- the four warps' results meet; the next piece's queries are on their way meanwhile
-        const Piece next = done < count ? next_piece(at, count - done, prefix, step.kv_heads, head_groups) : p;
-        ask_queries(next);
+        Piece next = p;
+        if constexpr (!CLUSTERED) {
+            if (done < count) next = next_piece(at, count - done, prefix, step.kv_heads, head_groups);
+            ask_queries(next);
+        }
 #pragma unroll
         for (int h = 0; h < MINE; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
@@ -570,7 +636,13 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
         }
         __syncthreads();
         const size_t my = (size_t)blockIdx.x * 2 + (seg == 0 ? 0 : 1);
-        for (int i = threadIdx.x; i < heads_here * (D / 4); i += THREADS) {
+        constexpr int ITEMS = (HEADS * (D / 4) + THREADS - 1) / THREADS;         // four values of a head each
+        float4 sums[ITEMS];
+        float2 tops[ITEMS];
+#pragma unroll
+        for (int item = 0; item < ITEMS; ++item) {
+            const int i = item * THREADS + threadIdx.x;
+            if (i >= heads_here * (D / 4)) break;
             const int head = i / (D / 4), d = (i - head * (D / 4)) * 4;
             float mm = -INFINITY;
 #pragma unroll
@@ -585,6 +657,9 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                 acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
                 ll += src[D + 1] * f;
             }
+            sums[item] = acc;
+            tops[item] = make_float2(mm, ll);
+            if constexpr (CLUSTERED) continue;
             if (p.complete) {
                 store_row(out + row * step.heads * D + (size_t)(head0 + head) * D + d, acc, ll);
             } else {
@@ -593,8 +668,42 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             }
         }
         __syncthreads();
+        if constexpr (CLUSTERED) {
+#pragma unroll
+            for (int item = 0; item < ITEMS; ++item) {
+                const int i = item * THREADS + threadIdx.x, head = i / (D / 4), d = (i - head * (D / 4)) * 4;
+                if (i >= heads_here * (D / 4)) break;
+                *reinterpret_cast<float4*>(merge + head * Sh::ROW + d) = sums[item];
+                if (d == 0) *reinterpret_cast<float2*>(merge + head * Sh::ROW + D) = tops[item];
+            }
+            cluster_sync();
+            if (blockIdx.x == 0)
+                for (int i = threadIdx.x; i < heads_here * (D / 4); i += THREADS) {
+                    const int head = i / (D / 4), d = (i - head * (D / 4)) * 4;
+                    float2 ml[MAX_CLUSTER];
+                    float mm = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < MAX_CLUSTER; ++b) {
+                        ml[b] = b < (int)gridDim.x ? load2_in(in_block(merge + head * Sh::ROW + D, b)) : make_float2(-INFINITY, 0.f);
+                        mm = fmaxf(mm, ml[b].x);
+                    }
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float ll = 0.f;
+#pragma unroll
+                    for (int b = 0; b < MAX_CLUSTER; ++b) {
+                        if (b >= (int)gridDim.x) break;
+                        const float f = weight_of(ml[b].x, ml[b].y, mm);
+                        const float4 v = load4_in(in_block(merge + head * Sh::ROW + d, b));
+                        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+                        ll += ml[b].y * f;
+                    }
+                    store_row(out + row * step.heads * D + (size_t)(head0 + head) * D + d, acc, ll);
+                }
+            cluster_sync();                                // the pieces are read
+        }
         p = next;
-    }
+        ++seg;
+    } while (!CLUSTERED && done < count);
     cp_async_wait<0>();
 }
 
@@ -614,7 +723,7 @@ merge_fp4_kernel(bf16* __restrict__ out, const Step step, const __grid_constant_
     wait_for_kernel_before();
     const int before = __ldcg(step.plan + tok), tiles = __ldcg(step.plan + tok + 1) - before;
     const int total = __ldcg(step.plan + step.tokens) * pairs;
-    if (tiles == 0) return;
+    if (tiles == 0 || __ldcg(step.plan + step.tokens + 1)) return;
     const int per = tiles_a_block(total, blocks), start = before * pairs + pair * tiles;
     const int first = start / per, last = (start + tiles - 1) / per;
     if (first == last) return;
@@ -675,29 +784,46 @@ merge_fp4_kernel(bf16* __restrict__ out, const Step step, const __grid_constant_
 }
 
 // Lets the decode kernel have its shared memory on the current device, once a device.
-template <int D, bool FOUR> cudaError_t allow_shared() {
+template <int D, bool FOUR, bool CLUSTERED> cudaError_t allow_shared() {
     static std::atomic<unsigned long long> allowed{0};
     int device = 0;
     cudaError_t err = cudaGetDevice(&device);
     if (err != cudaSuccess) return err;
     const unsigned long long bit = 1ull << (device & 63);
     if (device < 64 && (allowed.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-    err = cudaFuncSetAttribute(decode_fp4_kernel<D, FOUR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<D, FOUR>::bytes(MAX_TOKENS));
+    err = cudaFuncSetAttribute(decode_fp4_kernel<D, FOUR, CLUSTERED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<D, FOUR>::bytes(MAX_TOKENS));
     if (err == cudaSuccess && device < 64) allowed.fetch_or(bit, std::memory_order_relaxed);
     return err;
 }
 
 template <int D, bool FOUR>
-cudaError_t launch_decode(const bf16* q, bf16* out, const unsigned char* cache, const Step& step, const Rows& rows, int blocks,
+cudaError_t launch_decode(const bf16* q, bf16* out, const unsigned char* cache, const Step& step, const Rows& rows, int blocks, int cluster,
                           cudaStream_t stream) {
     using Sh = Shape<D, FOUR>;
-    cudaError_t err = allow_shared<D, FOUR>();
+    const int group = step.heads / step.kv_heads, head_groups = (group + Sh::HEADS - 1) / Sh::HEADS;
+    const int pairs = step.tokens * step.kv_heads * head_groups;
+    if (cluster) {
+        cudaError_t err = allow_shared<D, FOUR, true>();
+        if (err != cudaSuccess) return err;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(cluster, pairs);
+        config.blockDim = dim3(THREADS);
+        config.dynamicSmemBytes = Sh::bytes(0);
+        config.stream = stream;
+        cudaLaunchAttribute attribute[1];
+        attribute[0].id = cudaLaunchAttributeClusterDimension;
+        attribute[0].val.clusterDim.x = cluster;
+        attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+        config.attrs = attribute;
+        config.numAttrs = 1;
+        return cudaLaunchKernelEx(&config, decode_fp4_kernel<D, FOUR, true>, q, out, cache, step, rows);
+    }
+    cudaError_t err = allow_shared<D, FOUR, false>();
     if (err != cudaSuccess) return err;
-    err = launch_kernel(decode_fp4_kernel<D, FOUR>, dim3(blocks), dim3(THREADS), Sh::bytes(step.tokens), stream, q, out, cache, step, rows);
+    err = launch_kernel(decode_fp4_kernel<D, FOUR, false>, dim3(blocks), dim3(THREADS), Sh::bytes(step.tokens), stream, q, out, cache, step, rows);
     if (err != cudaSuccess) return err;
     constexpr int GROUPS = MERGE_THREADS / (D / 4);
-    const int group = step.heads / step.kv_heads, head_groups = (group + Sh::HEADS - 1) / Sh::HEADS;
-    const int pairs = step.tokens * step.kv_heads * head_groups, heads = group < Sh::HEADS ? group : Sh::HEADS;
+    const int heads = group < Sh::HEADS ? group : Sh::HEADS;
     const int deep = 4 * pairs < blocks;               // more than four pieces a pair
     return launch_kernel_overlapped(merge_fp4_kernel<D, FOUR>, dim3(pairs, deep ? heads : (heads + GROUPS - 1) / GROUPS), dim3(MERGE_THREADS), 0,
                                     stream, out, step, rows, blocks, deep);
@@ -706,8 +832,8 @@ cudaError_t launch_decode(const bf16* q, bf16* out, const unsigned char* cache, 
 template <int D, bool FOUR> int occupancy() {
     int n = 0;
     const size_t smem = Shape<D, FOUR>::bytes(MAX_TOKENS);
-    if (allow_shared<D, FOUR>() != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_fp4_kernel<D, FOUR>, THREADS, smem) != cudaSuccess) return 0;
+    if (allow_shared<D, FOUR, false>() != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_fp4_kernel<D, FOUR, false>, THREADS, smem) != cudaSuccess) return 0;
     return n;
 }
 
@@ -726,14 +852,16 @@ MRUN_API int mrun_attn_fp4_occupancy(int head_dim, int group) {
 
 
 // One token a row of q, out, positions and token_slot: the first `tokens` rows, or those that `rows` (host memory) names.  scratch:
-// 4-byte words: blocks * 2 * (4 or 8 heads) * (head_dim + 2) + tokens + 1, on 16 bytes.
+// 4-byte words: blocks * 2 * (4 or 8 heads) * (head_dim + 2) + tokens + 2, on 16 bytes.  cluster: 0, or the blocks of a
+// cluster (1, 2, 4, 8) that takes a pair; `scratch` and `blocks` are not used then.
 MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const void* cache, const int* block_tables, int table_rows,
                                   int max_blocks, const int* token_slot, const int* positions, const int* rows, int tokens, int heads,
                                   int kv_heads, int head_dim, int page_size, long pages, float scale, int window, void* scratch,
-                                  int blocks, cudaStream_t stream) {
+                                  int blocks, int cluster, cudaStream_t stream) {
     const char* name = "paged_attention_fp4";
     MRUN_REQUIRE(tokens >= 0 && tokens <= MAX_TOKENS, "%s: %d tokens, a launch takes up to %d", name, tokens, MAX_TOKENS);
-    MRUN_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && blocks > 0 && pages >= 0 && max_blocks >= 0 && table_rows >= 0,
+    MRUN_REQUIRE(cluster == 0 || cluster == 1 || cluster == 2 || cluster == 4 || cluster == MAX_CLUSTER, "%s: a cluster of %d blocks", name, cluster);
+    MRUN_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && (cluster || (blocks > 0 && scratch)) && pages >= 0 && max_blocks >= 0 && table_rows >= 0,
                  "%s: bad sizes", name);
     MRUN_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim=%d: the 4-bit cache takes heads of 64 or 128 features", name, head_dim);
     MRUN_REQUIRE(page_size > 0 && page_size % FP4_TOKENS == 0, "%s: page_size=%d is not a multiple of 16", name, page_size);
@@ -747,6 +875,8 @@ MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const
     MRUN_REQUIRE(scale > 0.f && scale < FLT_MAX, "%s: scale=%g is not a positive number", name, (double)scale);
     if (tokens == 0) return 0;
     const int group = heads / kv_heads, block_heads = heads_a_block(group);
+    MRUN_REQUIRE(!cluster || (long)tokens * kv_heads * ((group + block_heads - 1) / block_heads) < 65536,
+                 "%s: %d tokens of %d heads are too many for clusters", name, tokens, heads);
     float* part_o = (float*)scratch;
     float2* part_ml = (float2*)(part_o + (size_t)blocks * 2 * block_heads * head_dim);
     Rows selected;
@@ -758,7 +888,7 @@ MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const
                        scale * 1.4426950408889634f, part_o, part_ml, (int*)(part_ml + (size_t)blocks * 2 * block_heads)};
     auto launch = head_dim == 64 ? (group <= 4 ? launch_decode<64, true> : launch_decode<64, false>)
                                  : (group <= 4 ? launch_decode<128, true> : launch_decode<128, false>);
-    MRUN_CHECK_CUDA(launch((const bf16*)q, (bf16*)out, (const unsigned char*)cache, step, selected, blocks, stream), name);
+    MRUN_CHECK_CUDA(launch((const bf16*)q, (bf16*)out, (const unsigned char*)cache, step, selected, blocks, cluster, stream), name);
     MRUN_CHECK_LAUNCH(name);
     return 0;
 }

@@ -533,6 +533,27 @@ FP4_MAX_TOKENS = 256       # tokens of one launch of the decode kernel
 FP4_TILE_KEYS = 128        # keys that its blocks are dealt together
 
 
+# The most tiles that a block of a cluster takes, where the clusters leave most of the device empty, and where they do not.
+FP4_CLUSTER_TILES = (4, 8)
+
+
+def fp4_cluster(pairs: int, slots: int, longest: int) -> int:
+    """Blocks of a cluster that takes a (token, kv head) pair, or 0 where the tiles of all pairs are dealt to all blocks and a second
+    kernel adds their pieces.
+
+    A tile takes a block about 1.4 us, and a cluster of 2, 4 or 8 costs 0.3, 0.8 or 1.5 us over a single block: hence two tiles a block,
+    as far as the device holds the blocks (B200, 32 heads over 8 of 128, one request, us in clusters of 1 / 2 / 4 / 8 / dealt: 128 keys
+    4.0 / 4.3 / 4.8 / 5.4 / 5.4; 512 6.2 / 5.0 / 4.9 / 5.5 / 6.9; 2,048 15.0 / 9.4 / 7.2 / 6.1 / 7.4).  Long contexts are dealt, since a
+    step would wait for the cluster of the longest of them (two requests of 8,192 keys and thirty of 512: 29 in clusters, 18 dealt; of
+    2,048 and 128: 10.8 and 12.6), and sooner where the clusters fill little of the device (one request of 4,096: 10.0 and 9.7; 32 of
+    2,048: 14.9 and 19.5)."""
+    tiles, cluster = -(-longest // FP4_TILE_KEYS), 1
+    while cluster < 8 and tiles > 2 * cluster and 2 * cluster * pairs <= slots:
+        cluster *= 2
+    few = tiles <= cluster * FP4_CLUSTER_TILES[5 * cluster * pairs >= 2 * slots]
+    return cluster if few and pairs < 65536 else 0         # pairs are the second axis of a grid
+
+
 def _fp4_tokens(q, q_stride: int, out, cache, group, ctx, heads: int, head_dim: int, scale: float, window: int, rows=None) -> None:
     """Single tokens: all rows of the step, or those that ``rows`` lists."""
     pages, kv_heads, units, _ = cache.shape
@@ -546,9 +567,12 @@ def _fp4_tokens(q, q_stride: int, out, cache, group, ctx, heads: int, head_dim: 
     tokens = ctx.num_tokens if rows is None else len(rows)
     for first in range(0, tokens, FP4_MAX_TOKENS):
         n = min(FP4_MAX_TOKENS, tokens - first)
-        blocks = max(1, min(slots, n * tiles_a_token))
-        # the pieces of two pairs a block (sums, maximum and sum a head), and the prefix of tiles
-        scratch = torch.empty(blocks * 2 * block_heads * (head_dim + 2) + n + 1, dtype=torch.float32, device=q.device)
+        cluster = fp4_cluster(n * kv_heads * -(-ratio // block_heads), slots, longest)
+        blocks, scratch = 0, None
+        if not cluster:
+            blocks = max(1, min(slots, n * tiles_a_token))
+            # the pieces of two pairs a block (sums, maximum and sum a head), and the prefix of tiles
+            scratch = torch.empty(blocks * 2 * block_heads * (head_dim + 2) + n + 2, dtype=torch.float32, device=q.device)
         if rows is None:
             listed, at = None, first
         else:
@@ -556,7 +580,7 @@ def _fp4_tokens(q, q_stride: int, out, cache, group, ctx, heads: int, head_dim: 
         library.call("mrun_attn_fp4_decode", q.data_ptr() + 2 * at * q_stride, q_stride, out.data_ptr() + 2 * at * heads * head_dim,
                      cache.data_ptr(), tables.data_ptr(), tables.shape[0], tables.shape[1], ctx.token_slot.data_ptr() + 4 * at,
                      ctx.positions.data_ptr() + 4 * at, None if listed is None else ctypes.addressof(listed), n, heads, kv_heads, head_dim,
-                     units * ops.FP4_TOKENS, pages, scale, window, scratch.data_ptr(), blocks, _queue())
+                     units * ops.FP4_TOKENS, pages, scale, window, _address(scratch), blocks, cluster, _queue())
 
 
 def _fp4_portions(ctx, window: int, heads: int, kv_heads: int):

@@ -274,6 +274,44 @@ def test_single_tokens(heads, kv_heads, dim, page, lengths, window):
     close(out[:len(lengths)], want, c.v, 2.0 ** -10)
 
 
+@pytest.mark.parametrize("tiles", [0, 1, 2, 1 << 20])
+@pytest.mark.parametrize("heads, kv_heads, dim, lengths, window", [
+    (8, 2, 128, [1, 900, 129, 2500], 0), (16, 1, 64, [128, 700, 5000], 0), (5, 1, 128, [3000, 60], 1000), (32, 8, 128, [2000], 0)])
+def test_pairs_in_clusters_and_dealt_to_all_blocks(monkeypatch, tiles, heads, kv_heads, dim, lengths, window):
+    """The same steps with a cluster a pair (of 8 blocks to one, some without a tile) and with the tiles of all pairs dealt to all blocks."""
+    from mrun_b200.kernels import attention as module
+    rule = module.fp4_cluster
+    assert [rule(8, 592, keys) for keys in (1, 256, 257, 513, 1025, 4096, 4097)] == [1, 1, 2, 4, 8, 8, 0]
+    assert [rule(pairs, 592, 2048) for pairs in (74, 75, 148, 149, 296, 297)] == [8, 4, 4, 2, 2, 0]
+    assert [rule(pairs, 592, 1024) for pairs in (296, 297, 2048)] == [2, 1, 1] and rule(2048, 592, 1025) == 0 and rule(65536, 592, 1) == 0
+    monkeypatch.setattr(module, "FP4_CLUSTER_TILES", (tiles,) * 2)
+    page = 16
+    c = Filled(lengths, kv_heads, dim, page, seed=heads)
+    repeat = 1 + tiles % 2 * 20                                # also with so many pairs that clusters are smaller
+    tokens = repeat * len(lengths) + 1
+    q = c.queries(tokens, heads, dim)
+    segments = [(i, 1, n - 1) for _ in range(repeat) for i, n in enumerate(lengths)]
+    ctx, group = step_of(segments, c.table.to(DEV), page, tokens=tokens)
+    out = torch.full((tokens, heads * dim), 3.0, dtype=torch.bfloat16, device=DEV)
+    attention(q.to(DEV), heads * dim, out, c.cache, group, ctx, heads, dim, dim ** -0.5, window)
+    want = torch.cat([plain_fp4.attend(q[t:t + 1].view(1, heads, dim), c.k[i], c.v[i], [pos], dim ** -0.5, window).view(1, -1)
+                      for t, (i, _, pos) in enumerate(segments)])
+    assert (out[-1] == 0).all()
+    close(out[:-1], want, c.v, 2.0 ** -10)
+
+
+def test_more_heads_than_a_grid_of_clusters_takes():
+    heads, dim, page, tokens = 256, 64, 16, 256
+    c = Filled([40], heads, dim, page, seed=5)
+    q = c.queries(tokens, heads, dim)
+    ctx, group = step_of([(0, 1, t % 40) for t in range(tokens)], c.table.to(DEV), page)
+    out = torch.empty(tokens, heads * dim, dtype=torch.bfloat16, device=DEV)
+    attention(q.to(DEV), heads * dim, out, c.cache, group, ctx, heads, dim, 0.1)
+    rows = list(range(0, tokens, 37)) + [tokens - 1]
+    want = torch.cat([plain_fp4.attend(q[t:t + 1].view(1, heads, dim), c.k[0], c.v[0], [t % 40], 0.1).view(1, -1) for t in rows])
+    close(out[rows], want, c.v, 2.0 ** -10)
+
+
 def test_many_tokens_of_a_launch_and_more():
     """More tokens than a launch takes, many of them of the same request, with rows of padding between them."""
     heads, kv_heads, dim, page = 4, 2, 64, 16
