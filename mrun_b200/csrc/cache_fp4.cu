@@ -21,15 +21,17 @@ using bf16 = __nv_bfloat16;
 // token took 10.5 us with its read back, 4.2 so.
 // A value is a bfloat16: its quotient by a scale of 4 bits is a border (at most 3 bits) exactly or 2^-9 away from it.
 //
-// D / 8 lanes take TOGETHER heads of a token, eight features a lane, all asked for before the first is worked on, and the token's cosines and
-// sines once for them.  What bounds it is the chain of a head (load, sum over the lanes, root, rotation across lanes, store) with 25 warps a multiprocessor
-// to hide it: 21.7 us for 2,048 tokens of 32 + 8 + 8 heads of 128 (the queries alone 15 to 17; the write of bfloat16 pages 13.7; the bytes
-// take 6.8) with two heads and four blocks a multiprocessor; 23.2 with four heads and three blocks, 28 with one; asking for the next heads
-// while working (25.4) and four chains side by side (26.6) spill.  A step of few heads gives each lanes of its own.
+// D / 8 lanes take a run of heads of a token, eight features a lane, with the token's cosines and sines loaded once and the features of
+// the next three heads on their way into shared memory, where a lane reads what it copied itself.  What bounds it is the chain of a head
+// (sum over the lanes, root, rotation across lanes) and its instructions, with 28 warps a multiprocessor to hide it: 14.4 us for 2,048 tokens of 32 + 8 + 8 heads
+// of 128 in runs of 6, of which the queries alone take 9.4 (the bytes take 6.8, the write of bfloat16 pages 13.7); a copy to every two heads, in
+// registers, took 21.7.  Longer runs save instructions and leave fewer lanes at work, hence as long as the step has
+// heads for them (us in runs of 2 / 4 / 6 / 12: 512 tokens 8.3 / 8.1 / 8.5 / 9.9; 2,048 18.8 / 14.9 / 14.2 / 14.8; 8,192 72.5 / 55.5 / 50.5 / 47.1).
 // ------------------------------------------------------------------------------------------
 constexpr int STORE_THREADS = 256;
-constexpr int HEADS_TOGETHER = 2;
-constexpr int HEADS_AT_ONCE = 8192;        // a step of up to this many heads gives each lanes of its own
+constexpr int RUN_THREADS = 128, RUN_DEPTH = 4;
+constexpr unsigned MOST_A_RUN = 12;
+constexpr unsigned HEADS_A_RUN = 16384;    // a run gets a head more for every so many heads of the step
 
 // The byte of the scale nearest to `wanted` (0 .. 10,240), ties to the even byte.  `wanted` has a bit set below
 // its 24 wherever something was cut off, so that this is the only rounding.
@@ -222,143 +224,211 @@ __device__ __forceinline__ void rotate_staged(F (&v)[8], const float2* __restric
     }
 }
 
-// STAGED: rotary sizes that are no multiple of 16, and weights or tables off 16 bytes; keys in 64 bits throughout.
-template <int D, bool STAGED, int TOGETHER>
-__global__ void __launch_bounds__(STORE_THREADS, STAGED ? 1 : 4)
-qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, long q_stride,
-                              const float* __restrict__ q_weight, const float* __restrict__ k_weight, float eps,
-                              const float2* __restrict__ rot, int half, const int* __restrict__ slots, unsigned char* __restrict__ cache,
-                              unsigned groups, int heads, int kv_heads, int page_size, long pages, unsigned groups_per_token) {
+// What the lanes of a token need of it.
+template <int D> struct Token {
+    int part;                           // of the D / 8 lanes of a head
+    unsigned mask;                      // theirs
+    Turn turn;
+    bool turned, normed, writes;        // writes: its slot lies in the cache
+    int off_row;                        // its row of a unit
+    unsigned char* units;               // its unit of the first kv head
+    int head_bytes;                     // from a kv head to the next
+};
+
+template <int D, bool STAGED>
+__device__ __forceinline__ Token<D> token_of(const float* q_weight, const float2* __restrict__ cs, int half, bool turned, int slot,
+                                             unsigned char* cache, int kv_heads, int page_size, long pages) {
     using Unit = Fp4Unit<D>;
     constexpr int LANES = D / 8;
-    __shared__ double stage_all[STAGED ? STORE_THREADS / LANES * D : 1];
-    const int per_token = heads + 2 * kv_heads;
-    const unsigned group = blockIdx.x * (STORE_THREADS / LANES) + threadIdx.x / LANES;
-    if (group >= groups) return;                                   // all lanes of a group together
-    const int t = (int)(group / groups_per_token), head0 = (int)(group - t * groups_per_token) * TOGETHER, part = threadIdx.x % LANES;
-    const unsigned lane = threadIdx.x & 31;
-    const unsigned mask = ((1u << LANES) - 1u) << (lane & ~(unsigned)(LANES - 1));
-
-    uint4 raw[TOGETHER];
-    const bf16* row = qkv + ((size_t)t * per_token + head0) * D + part * 8;
-#pragma unroll
-    for (int i = 0; i < TOGETHER; ++i)
-        if (head0 + i < per_token) raw[i] = *reinterpret_cast<const uint4*>(row + i * D);
-    // a slot outside the cache (a padding row's -1) writes nothing
-    const int slot = head0 + TOGETHER <= heads || slots == nullptr ? -1 : slots[t];
-    const bool turned = half > 0 && head0 < heads + kv_heads;
-    const float2* cs = rot + (size_t)t * half;
-    Turn turn;
+    Token<D> t;
+    t.part = threadIdx.x % LANES;
+    t.mask = ((1u << LANES) - 1u) << (threadIdx.x & 31 & ~(unsigned)(LANES - 1));
+    t.normed = q_weight != nullptr;
+    t.turned = turned;
     if (!STAGED && turned) {
         const int away = half / 8;
-        const bool low = part < away;
-        turn.turns = part < 2 * away;
-        turn.partner = turn.turns ? (low ? part + away : part - away) : part;
-        if (turn.turns) {
+        const bool low = t.part < away;
+        t.turn.turns = t.part < 2 * away;
+        t.turn.partner = t.turn.turns ? (low ? t.part + away : t.part - away) : t.part;
+        if (t.turn.turns) {
             float2 two[2][4];                                      // (cosine, sine) of a pair each
-            const float* src = reinterpret_cast<const float*>(cs + (low ? part : turn.partner) * 8);
+            const float* src = reinterpret_cast<const float*>(cs + (low ? t.part : t.turn.partner) * 8);
             load8(two[0], src);
             load8(two[1], src + 8);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float2 a = two[e / 2][e % 2 * 2], b = two[e / 2][e % 2 * 2 + 1];
-                turn.c[e] = make_float2(a.x, b.x);
-                turn.s[e] = low ? make_float2(-a.y, -b.y) : make_float2(a.y, b.y);
+                t.turn.c[e] = make_float2(a.x, b.x);
+                t.turn.s[e] = low ? make_float2(-a.y, -b.y) : make_float2(a.y, b.y);
             }
         }
     }
-    const bool normed = q_weight != nullptr;
-    double* stage = stage_all + (STAGED ? threadIdx.x / LANES * D : 0);
-    const int page = slot >= 0 ? slot / page_size : -1;
-    const bool writes = page >= 0 && page < pages;
-    const int off = slot - page * page_size, r = off & (FP4_TOKENS - 1);
-    unsigned char* units = cache + ((size_t)page * kv_heads * (page_size / FP4_TOKENS) + off / FP4_TOKENS) * Unit::BYTES;
-    const int head_bytes = page_size / FP4_TOKENS * Unit::BYTES;
+    const int page = slot >= 0 ? slot / page_size : -1, off = slot - page * page_size;
+    t.writes = page >= 0 && page < pages;
+    t.off_row = off & (FP4_TOKENS - 1);
+    t.units = cache + ((size_t)page * kv_heads * (page_size / FP4_TOKENS) + off / FP4_TOKENS) * Unit::BYTES;
+    t.head_bytes = page_size / FP4_TOKENS * Unit::BYTES;
+    return t;
+}
 
+__device__ __forceinline__ void unpack(float2 (&x)[4], const uint4& raw) {
+    const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
-    for (int i = 0; i < TOGETHER; ++i) {
-        const int head = head0 + i;
-        if (head >= per_token) break;
-        const bool is_q = head < heads, is_k = !is_q && head < heads + kv_heads;
-        if (!is_q && !writes) break;                               // keys and values lie behind the queries
-        float2 weight[4];
-        if (normed && (is_q || is_k)) {
-            const float* weights = is_q ? q_weight : k_weight;
-            if constexpr (STAGED) {
+    for (int e = 0; e < 4; ++e) x[e] = __bfloat1622float2(pairs[e]);
+}
+
+template <int D, bool STAGED>
+__device__ __forceinline__ void store_query(const uint4& raw, const float2 (&weight)[4], const Token<D>& t, float eps,
+                                            const float2* __restrict__ cs, int half, float* stage, bf16* out) {
+    float2 x[4];
+    unpack(x, raw);
+    if (t.normed) norm<D>(x, weight, eps, t.mask);
+    if (t.turned) {
+        if constexpr (STAGED) {
+            float y[8] = {x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
+            rotate_staged(y, cs, half, t.mask, t.part, stage);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) weight[e] = make_float2(weights[part * 8 + 2 * e], weights[part * 8 + 2 * e + 1]);
-            } else {
-                load8(weight, weights + part * 8);
-            }
-        }
-        float2 x[4];
-        {
-            const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = __bfloat1622float2(pairs[e]);
-        }
-        if (is_q) {
-            if (normed) norm<D>(x, weight, eps, mask);
-            if (turned) {
-                if constexpr (STAGED) {
-                    float y[8] = {x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
-                    rotate_staged(y, cs, half, mask, part, reinterpret_cast<float*>(stage));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = make_float2(y[2 * e], y[2 * e + 1]);
-                } else {
-                    rotate<false>(x, turn, mask, part);
-                }
-            }
-            uint4 packed;
-            __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(&packed);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) out[e] = __floats2bfloat162_rn(x[e].x, x[e].y);
-            *reinterpret_cast<uint4*>(q_out + (size_t)t * q_stride + (size_t)head * D + part * 8) = packed;
-            continue;
-        }
-        unsigned scale, codes;
-        if (is_k && (normed || turned)) {
-            bool sure = false;
-            if constexpr (!STAGED) {
-                float2 y[4] = {x[0], x[1], x[2], x[3]};
-                // a sum of squares outside these bounds may have lost digits to the ends of the range (eps hides a small one)
-                bool kept = true;
-                if (normed) {
-                    const float ss = norm<D>(y, weight, eps, mask);
-                    kept = ss < 1e36f && (ss > 1e-30f || eps > 1e-20f);
-                }
-                float widest = 0.f;
-                if (turned) {
-                    widest = rotate<true>(y, turn, mask, part);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) widest = fmaxf(widest, fmaxf(fabsf(y[e].x), fabsf(y[e].y)));
-                }
-                widest = fmaxf(widest, __shfl_xor_sync(mask, widest, 1));
-                // The sum of squares is off by 12 roundings at most and half of that under the root, the root by 2^-22, the two products and the
-                // two of the rotation by one each: less than 2^-20 of |first| + |second|.
-                codes = quantise(y, widest * 1.9073486328125e-06f, mask, scale, sure);
-                sure = __all_sync(mask, sure && kept);
-            }
-            if (!sure) {
-                double y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = e % 2 ? x[e / 2].y : x[e / 2].x;
-                if (normed) norm<D>(y, weight, eps, mask);
-                if (turned) {
-                    if constexpr (STAGED) rotate_staged(y, cs, half, mask, part, stage);
-                    else rotate(y, turn, mask, part);
-                }
-                codes = quantise(y, mask, scale);
-            }
+            for (int e = 0; e < 4; ++e) x[e] = make_float2(y[2 * e], y[2 * e + 1]);
         } else {
-            codes = quantise(x, mask, scale);
+            rotate<false>(x, t.turn, t.mask, t.part);
         }
-        unsigned char* unit = units + (size_t)(is_k ? head - heads : head - heads - kv_heads) * head_bytes;
-        // eight features are four bytes of one piece: D = 128 has pieces of eight bytes, D = 64 of four
-        *reinterpret_cast<unsigned*>(unit + (is_k ? Unit::k_code(r, part * 4) : Unit::v_code(r, part * 4))) = codes;
-        if ((part & 1) == 0) unit[is_k ? Unit::k_scale(r, part / 2) : Unit::v_scale(r, part / 2)] = (unsigned char)scale;
     }
+    uint4 packed;
+    __nv_bfloat162* pairs = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pairs[e] = __floats2bfloat162_rn(x[e].x, x[e].y);
+    *reinterpret_cast<uint4*>(out + t.part * 8) = packed;
+}
+
+// A key, or a value, of kv head `head`.
+template <int D, bool STAGED>
+__device__ __forceinline__ void store_held(const uint4& raw, bool is_k, int head, const float2 (&weight)[4], const Token<D>& t, float eps,
+                                           const float2* __restrict__ cs, int half, double* stage) {
+    using Unit = Fp4Unit<D>;
+    float2 x[4];
+    unpack(x, raw);
+    unsigned scale, codes;
+    if (is_k && (t.normed || t.turned)) {
+        bool sure = false;
+        if constexpr (!STAGED) {
+            float2 y[4] = {x[0], x[1], x[2], x[3]};
+            // a sum of squares outside these bounds may have lost digits to the ends of the range (eps hides a small one)
+            bool kept = true;
+            if (t.normed) {
+                const float ss = norm<D>(y, weight, eps, t.mask);
+                kept = ss < 1e36f && (ss > 1e-30f || eps > 1e-20f);
+            }
+            float widest = 0.f;
+            if (t.turned) {
+                widest = rotate<true>(y, t.turn, t.mask, t.part);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) widest = fmaxf(widest, fmaxf(fabsf(y[e].x), fabsf(y[e].y)));
+            }
+            widest = fmaxf(widest, __shfl_xor_sync(t.mask, widest, 1));
+            // The sum of squares is off by 12 roundings at most and half of that under the root, the root by 2^-22, the two products and the
+            // two of the rotation by one each: less than 2^-20 of |first| + |second|.
+            codes = quantise(y, widest * 1.9073486328125e-06f, t.mask, scale, sure);
+            sure = __all_sync(t.mask, sure && kept);
+        }
+        if (!sure) {
+            double y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = e % 2 ? x[e / 2].y : x[e / 2].x;
+            if (t.normed) norm<D>(y, weight, eps, t.mask);
+            if (t.turned) {
+                if constexpr (STAGED) rotate_staged(y, cs, half, t.mask, t.part, stage);
+                else rotate(y, t.turn, t.mask, t.part);
+            }
+            codes = quantise(y, t.mask, scale);
+        }
+    } else {
+        codes = quantise(x, t.mask, scale);
+    }
+    unsigned char* unit = t.units + (size_t)head * t.head_bytes;
+    const int part = t.part, r = t.off_row;
+    // eight features are four bytes of one piece: D = 128 has pieces of eight bytes, D = 64 of four
+    *reinterpret_cast<unsigned*>(unit + (is_k ? Unit::k_code(r, part * 4) : Unit::v_code(r, part * 4))) = codes;
+    if ((part & 1) == 0) unit[is_k ? Unit::k_scale(r, part / 2) : Unit::v_scale(r, part / 2)] = (unsigned char)scale;
+}
+
+// A head to every D / 8 lanes.  STAGED: rotary sizes that are no multiple of 16, and weights or tables off 16 bytes; keys in 64 bits throughout.
+template <int D, bool STAGED>
+__global__ void __launch_bounds__(STORE_THREADS, STAGED ? 1 : 4)
+qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, long q_stride,
+                              const float* __restrict__ q_weight, const float* __restrict__ k_weight, float eps,
+                              const float2* __restrict__ rot, int half, const int* __restrict__ slots, unsigned char* __restrict__ cache,
+                              unsigned groups, int heads, int kv_heads, int page_size, long pages) {
+    constexpr int LANES = D / 8;
+    __shared__ double stage_all[STAGED ? STORE_THREADS / LANES * D : 1];
+    const int per_token = heads + 2 * kv_heads;
+    const unsigned group = blockIdx.x * (STORE_THREADS / LANES) + threadIdx.x / LANES;
+    if (group >= groups) return;                                   // all lanes of a head together
+    const int t = (int)(group / per_token), head = (int)(group - t * per_token), part = threadIdx.x % LANES;
+    const uint4 raw = *reinterpret_cast<const uint4*>(qkv + (size_t)group * D + part * 8);
+    const bool is_q = head < heads, is_k = !is_q && head < heads + kv_heads;
+    // a slot outside the cache (a padding row's -1) writes nothing
+    const int slot = is_q || slots == nullptr ? -1 : slots[t];
+    const float2* cs = rot + (size_t)t * half;
+    const Token<D> token = token_of<D, STAGED>(q_weight, cs, half, half > 0 && (is_q || is_k), slot, cache, kv_heads, page_size, pages);
+    double* stage = stage_all + (STAGED ? threadIdx.x / LANES * D : 0);
+    if (!is_q && !token.writes) return;
+    float2 weight[4];
+    if (token.normed && (is_q || is_k)) {
+        const float* weights = is_q ? q_weight : k_weight;
+        if constexpr (STAGED) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) weight[e] = make_float2(weights[part * 8 + 2 * e], weights[part * 8 + 2 * e + 1]);
+        } else {
+            load8(weight, weights + part * 8);
+        }
+    }
+    if (is_q) store_query<D, STAGED>(raw, weight, token, eps, cs, half, reinterpret_cast<float*>(stage), q_out + (size_t)t * q_stride + (size_t)head * D);
+    else store_held<D, STAGED>(raw, is_k, is_k ? head - heads : head - heads - kv_heads, weight, token, eps, cs, half, stage);
+}
+
+// `run` heads of a token, one after the other, to every D / 8 lanes; a lane copies its own features of the next heads into shared memory
+// meanwhile.  The lanes of a warp have the same heads of several tokens, so that they go the same way; those that quantise begin first.
+template <int D>
+__global__ void __launch_bounds__(RUN_THREADS, 7)
+qk_norm_rope_cache_fp4_runs_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, long q_stride,
+                                   const float* __restrict__ q_weight, const float* __restrict__ k_weight, float eps,
+                                   const float2* __restrict__ rot, int half, const int* __restrict__ slots, unsigned char* __restrict__ cache,
+                                   unsigned tokens, unsigned runs, int run, int heads, int kv_heads, int page_size, long pages) {
+    constexpr int LANES = D / 8;
+    __shared__ uint4 ring[RUN_DEPTH][RUN_THREADS];
+    const int per_token = heads + 2 * kv_heads;
+    const unsigned group = blockIdx.x * (RUN_THREADS / LANES) + threadIdx.x / LANES;
+    if (group >= tokens * runs) return;                            // all lanes of a run together
+    const unsigned before = group / tokens, t = group - before * tokens, part = threadIdx.x % LANES;
+    const int first = (int)(runs - 1 - before) * run, end = min(first + run, per_token);
+    const bf16* row = qkv + (size_t)t * per_token * D + part * 8;
+    auto ask = [&](int head) {
+        const unsigned dst = (unsigned)__cvta_generic_to_shared(&ring[(head - first) % RUN_DEPTH][threadIdx.x]);
+        if (head < end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(row + (size_t)head * D) : "memory");
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < RUN_DEPTH - 1; ++i) ask(first + i);
+    const int slot = end <= heads || slots == nullptr ? -1 : slots[t];
+    const Token<D> token = token_of<D, false>(q_weight, rot + (size_t)t * half, half, half > 0 && first < heads + kv_heads, slot, cache, kv_heads,
+                                              page_size, pages);
+    float2 weight[4];
+    if (token.normed && first < heads + kv_heads) load8(weight, (first < heads ? q_weight : k_weight) + part * 8);
+    for (int head = first; head < end; ++head) {
+        if (head >= heads && !token.writes) break;                 // keys and values lie behind the queries
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(RUN_DEPTH - 2) : "memory");
+        const uint4 raw = ring[(head - first) % RUN_DEPTH][threadIdx.x];
+        ask(head + RUN_DEPTH - 1);                                 // into the place of the head before, whose features are used
+        if (head < heads) {
+            store_query<D, false>(raw, weight, token, eps, nullptr, 0, nullptr, q_out + (size_t)t * q_stride + (size_t)head * D);
+        } else {
+            const bool is_k = head < heads + kv_heads;
+            if (token.normed && head == heads) load8(weight, k_weight + part * 8);
+            store_held<D, false>(raw, is_k, is_k ? head - heads : head - heads - kv_heads, weight, token, eps, nullptr, 0, nullptr);
+        }
+    }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
 }
 
 // ------------------------------------------------------------------------------------------
@@ -455,17 +525,25 @@ fp4_rows_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
     }
 }
 
-template <int D, int TOGETHER>
+template <int D>
 cudaError_t launch_store(const void* qkv, void* q_out, long q_stride, const float* q_weight, const float* k_weight, float eps,
                          const float* rot, int rotary_dim, const int* slots, void* cache, int tokens, int heads, int kv_heads,
                          int page_size, long pages, cudaStream_t stream) {
-    constexpr unsigned GROUPS = STORE_THREADS / (D / 8);
-    const unsigned per_token = (unsigned)(heads + 2 * kv_heads + TOGETHER - 1) / TOGETHER, groups = (unsigned)tokens * per_token;
+    const unsigned per_token = (unsigned)(heads + 2 * kv_heads), groups = (unsigned)tokens * per_token;
     const bool staged = rotary_dim % 16 || (((uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)rot) & 15);
-    return launch_kernel(staged ? qk_norm_rope_cache_fp4_kernel<D, true, TOGETHER> : qk_norm_rope_cache_fp4_kernel<D, false, TOGETHER>,
+    const unsigned run = (groups + HEADS_A_RUN - 1) / HEADS_A_RUN < MOST_A_RUN ? (groups + HEADS_A_RUN - 1) / HEADS_A_RUN : MOST_A_RUN;
+    if (!staged && run > 1) {
+        constexpr unsigned GROUPS = RUN_THREADS / (D / 8);
+        const unsigned runs = (per_token + run - 1) / run;
+        return launch_kernel(qk_norm_rope_cache_fp4_runs_kernel<D>, dim3(((unsigned)tokens * runs + GROUPS - 1) / GROUPS), dim3(RUN_THREADS), 0, stream,
+                             (const bf16*)qkv, (bf16*)q_out, q_stride, q_weight, k_weight, eps, (const float2*)rot, rotary_dim / 2, slots,
+                             (unsigned char*)cache, (unsigned)tokens, runs, (int)run, heads, kv_heads, page_size, pages);
+    }
+    constexpr unsigned GROUPS = STORE_THREADS / (D / 8);
+    return launch_kernel(staged ? qk_norm_rope_cache_fp4_kernel<D, true> : qk_norm_rope_cache_fp4_kernel<D, false>,
                          dim3((groups + GROUPS - 1) / GROUPS), dim3(STORE_THREADS), 0, stream, (const bf16*)qkv, (bf16*)q_out, q_stride,
                          q_weight, k_weight, eps, (const float2*)rot, rotary_dim / 2, slots, (unsigned char*)cache, groups, heads, kv_heads,
-                         page_size, pages, per_token);
+                         page_size, pages);
 }
 
 int launch_rows(const void* cache, const int* ids, const Spans& spans, const int* block_tables, int table_rows, int max_blocks, void* k_out,
@@ -507,9 +585,7 @@ MRUN_API int mrun_qk_norm_rope_cache_fp4(const void* qkv, void* q_out, long q_st
     MRUN_REQUIRE(((uintptr_t)rot & 7) == 0, "%s: the table starts on 8 bytes", name);
     if (tokens == 0) return 0;
     MRUN_REQUIRE((long)tokens * (heads + 2 * kv_heads) < (1L << 31), "%s: %d tokens of %d heads are more than a launch takes", name, tokens, heads);
-    const bool alone = (long)tokens * (heads + 2 * kv_heads) <= HEADS_AT_ONCE;
-    auto launch = head_dim == 64 ? (alone ? launch_store<64, 1> : launch_store<64, HEADS_TOGETHER>)
-                                 : (alone ? launch_store<128, 1> : launch_store<128, HEADS_TOGETHER>);
+    auto launch = head_dim == 64 ? launch_store<64> : launch_store<128>;
     MRUN_CHECK_CUDA(launch(qkv, q_out, q_stride, q_weight, k_weight, eps, rot, rotary_dim, slots, cache, tokens, heads, kv_heads, page_size,
                            pages, stream), name);
     MRUN_CHECK_LAUNCH(name);

@@ -111,6 +111,33 @@ def test_write_and_read_back(heads, kv_heads, dim, rotary, page, tokens, norm):
             assert torch.equal(k[i, :, offset], kk) and torch.equal(v[i, :, offset], vv)
 
 
+@pytest.mark.parametrize("heads, kv_heads, dim, rotary, tokens, norm", [
+    (32, 8, 128, 128, 357, True), (12, 4, 64, 32, 1337, True), (5, 3, 64, 64, 3001, True), (1, 1, 64, 0, 66001, False),
+    (4, 1, 128, 0, 9001, True), (20, 4, 128, 96, 8003, True), (1, 3, 128, 64, 12001, False)])
+def test_write_of_many_tokens(heads, kv_heads, dim, rotary, tokens, norm):
+    """Steps of so many heads that lanes take several of a token: what the same tokens give in steps of few."""
+    qkv, (qw, kw), rot = inputs(tokens, heads, kv_heads, dim, rotary, seed=tokens, norm=norm)
+    qw, kw, rot, qkv = to(qw), to(kw), to(rot), qkv.to(DEV)
+    page, eps = 32, 1e-6
+    pages = tokens // page + 1
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(1))[:tokens].int()
+    slots[::7], slots[3::50] = -1, pages * page
+    slots = slots.to(DEV)
+    caches = [torch.zeros(ops().fp4_cache_shape(pages, kv_heads, page, dim), dtype=torch.uint8, device=DEV) for _ in range(3)]
+    write = lambda x, t0, t1, cache, **kw_: ops().qk_norm_rope_cache_fp4(
+        x[t0:t1], heads, kv_heads, dim, qw, kw, eps, rot if rot is None else rot[t0:t1], rotary, slots[t0:t1], cache, **kw_)
+    q = torch.empty(tokens, heads * dim, dtype=torch.bfloat16, device=DEV)
+    write(qkv, 0, tokens, caches[0], q_out=q)
+    few = 16384 // (heads + 2 * kv_heads)
+    apart = torch.empty_like(q)
+    for t0 in range(0, tokens, few):
+        write(qkv, t0, min(t0 + few, tokens), caches[1], q_out=apart[t0:t0 + few])
+    given = qkv.clone()
+    in_place = write(given, 0, tokens, caches[2])
+    assert torch.equal(q, apart) and torch.equal(in_place, q) and torch.equal(given[:, heads * dim:], qkv[:, heads * dim:])
+    assert torch.equal(caches[0], caches[1]) and torch.equal(caches[0], caches[2]) and caches[0].any()
+
+
 def test_values_on_borders_and_beyond():
     """Ties of codes and of scales, groups of zeros, tiny, huge and infinite values, and NaN."""
     dim, kv_heads, page = 64, 1, 16
