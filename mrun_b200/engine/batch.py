@@ -77,18 +77,15 @@ class HostStaging:
         self.device = device
         self._buffers: List[Optional[torch.Tensor]] = [None] * depth
         self._views: List[Optional[np.ndarray]] = [None] * depth          # of the buffers
-        self._events: List[Optional[torch.cuda.Event]] = [None] * depth   # recorded behind a buffer's last copy
+        self._events: List[Optional[torch.cuda.Event]] = [None] * depth
         self._turn = 0
         self.bytes_uploaded = 0
 
     def upload(self, host: np.ndarray, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         i = self._turn
         self._turn = (self._turn + 1) % len(self._buffers)
-        event = self._events[i]
-        if event is None:
-            event = self._events[i] = torch.cuda.Event()
-        else:
-            event.synchronize()
+        if self._events[i] is not None:
+            self._events[i].synchronize()
         n = host.size
         if self._buffers[i] is None or self._buffers[i].numel() < n:
             self._buffers[i] = torch.empty(max(4096, 2 * n), dtype=torch.int32, pin_memory=True)
@@ -99,7 +96,9 @@ class HostStaging:
             out.copy_(self._buffers[i][:n], non_blocking=True)
         else:
             out[:n].copy_(self._buffers[i][:n], non_blocking=True)
+        event = torch.cuda.Event()
         event.record()
+        self._events[i] = event
         self.bytes_uploaded += 4 * n
         return out
 
