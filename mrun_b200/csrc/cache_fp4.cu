@@ -611,7 +611,7 @@ MRUN_API int mrun_fp4_spans(const void* cache, const int* spans, int n, const in
     int next = 0;
     for (int s = 0; s < n; ++s) {
         const int* v = spans + 6 * s;
-        MRUN_REQUIRE(v[1] >= 0 && v[1] % out_page == 0 && v[2] > v[1] && v[3] == next && v[5] >= 0, "%s: span %d is [%d, %d) at page %d", name, s,
+        MRUN_REQUIRE(v[1] >= 0 && v[1] % out_page == 0 && v[2] > v[1] && v[3] == next && v[4] >= 0 && v[5] >= 0, "%s: span %d is [%d, %d) at page %d", name, s,
                      v[1], v[2], v[3]);
         next += (v[2] - v[1] + out_page - 1) / out_page;
         MRUN_REQUIRE(table == nullptr || v[1] / out_page + (v[2] - v[1] + out_page - 1) / out_page <= table_width, "%s: table_width=%d", name, table_width);

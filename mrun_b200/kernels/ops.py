@@ -378,7 +378,8 @@ def fp4_spans(cache: torch.Tensor, head_dim: int, block_tables: torch.Tensor, sp
         if t is not None:
             _check(t, name, torch.int32)
     for span in spans:
-        if span[2] - span[1] + span[3] * rows > pages * rows or (table is not None and span[4] + span[5] > span_of_row.numel()):
+        if (not all(0 <= value < 1 << 31 for value in span[1:]) or span[2] - span[1] + span[3] * rows > pages * rows
+                or (table is not None and span[4] + span[5] > span_of_row.numel())):
             raise KernelError(f"fp4_spans: span {span} does not fit {pages} pages of {rows} rows")
     k, v = torch.empty((2, pages, kv_heads, rows, head_dim), dtype=torch.bfloat16, device=cache.device).unbind(0)
     flat = (ctypes.c_int * (6 * len(spans)))(*[value for span in spans for value in span])

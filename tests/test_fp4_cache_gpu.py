@@ -327,6 +327,45 @@ def test_pairs_in_clusters_and_dealt_to_all_blocks(monkeypatch, tiles, heads, kv
     close(out[:-1], want, c.v, 2.0 ** -10)
 
 
+def test_spans_that_do_not_fit_are_refused():
+    c = Filled([100], 2, 64, 16)
+    table = torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+    rows = torch.zeros(8, dtype=torch.int32, device=DEV)
+    for span in ((0, 0, 100, 0, -1, 4), (0, 0, 100, 0, 5, 4), (0, 0, 100, 0, 0, -1), (0, -64, 36, 0, 0, 4), (0, 0, 300, 0, 0, 4), (0, 0, 100, 1, 0, 4),
+                 (0, 64, 64, 0, 0, 4), (0, 0, 100, -1, 0, 4), (0, 1 << 32, (1 << 32) + 50, 0, 0, 4), (0, 128, 228, 0, 0, 4)):
+        with pytest.raises(ops().KernelError):
+            ops().fp4_spans(c.cache, 64, c.table.to(DEV), [span], 2, 64, table, rows)
+    assert not table.any() and not rows.any()
+
+
+def test_pages_far_behind_the_first_bytes():
+    """A cache of more than 2^32 bytes: writing, reading back, and attention of both kinds in its last pages, as in a small one."""
+    heads, kv_heads, dim, page, n = 16, 8, 128, 32, 700
+    shape = ops().fp4_cache_shape(130_000, kv_heads, page, dim)
+    blocks = -(-n // page)
+    assert math.prod(shape) > 2 ** 32
+    qkv, (qw, kw), rot = inputs(n, heads, kv_heads, dim, dim, seed=3)
+    got = []
+    for pages in (blocks, shape[0]):
+        cache = torch.empty((pages,) + shape[1:], dtype=torch.uint8, device=DEV)
+        first = pages - blocks
+        slots = (torch.arange(n, dtype=torch.int32) + first * page).to(DEV)
+        table = torch.arange(first, pages, dtype=torch.int32, device=DEV).view(1, -1)
+        q = ops().qk_norm_rope_cache_fp4(qkv.to(DEV), heads, kv_heads, dim, to(qw), to(kw), 1e-6, to(rot), dim, slots, cache)
+        back = ops().fp4_pages(cache, dim, table[0])
+        outs = []
+        for segments in ([(0, n, 0)], [(0, 1, t) for t in range(0, n, 9)]):
+            ctx, group = step_of(segments, table, page)
+            out = torch.empty(ctx.num_tokens, heads * dim, dtype=torch.bfloat16, device=DEV)
+            rows = q if len(segments) == 1 else q[::9]
+            attention(rows.contiguous(), heads * dim, out, cache, group, ctx, heads, dim, dim ** -0.5)
+            outs.append(out)
+        got.append([q.clone(), *(x.reshape(blocks, kv_heads, page, dim).transpose(1, 2).reshape(-1, kv_heads, dim)[:n] for x in back), *outs])
+        del cache
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
 def test_more_heads_than_a_grid_of_clusters_takes():
     heads, dim, page, tokens = 256, 64, 16, 256
     c = Filled([40], heads, dim, page, seed=5)
@@ -522,3 +561,12 @@ def test_write_then_attend():
         want = plain_fp4.attend(q, torch.cat(keys), torch.cat(values), positions.tolist(), dim ** -0.5).view(n, -1)
         close(out, want, values, 2.0 ** -7)
         done += n
+
+
+@pytest.mark.parametrize("test", [
+    test_calls_on_two_streams_at_once, test_many_tokens_of_a_launch_and_more, test_pages_that_are_not_held, test_large_and_small_magnitudes,
+    test_nan_where_it_is_seen_and_only_there, test_captured_twice_and_replayed_at_once, test_same_bits_every_time, test_write_then_attend])
+def test_the_same_dealt_to_all_blocks(monkeypatch, test):
+    from mrun_b200.kernels import attention as module
+    monkeypatch.setattr(module, "FP4_CLUSTER_TILES", (0, 0))
+    test()
