@@ -86,12 +86,6 @@ __device__ __forceinline__ float exp2_fast(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(out) : "f"(v));
     return out;
 }
-// The eight codes of a word as four pairs of halves.
-__device__ __forceinline__ void halves_of(unsigned word, unsigned (&h)[4]) {
-    asm("{\n.reg .b8 c0, c1, c2, c3;\nmov.b32 {c0, c1, c2, c3}, %4;\n"
-        "cvt.rn.f16x2.e2m1x2 %0, c0;\ncvt.rn.f16x2.e2m1x2 %1, c1;\ncvt.rn.f16x2.e2m1x2 %2, c2;\ncvt.rn.f16x2.e2m1x2 %3, c3;\n}"
-        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(word));
-}
 // Bytes I and I + 1 of `bytes`, scales, as halves.
 template <int I> __device__ __forceinline__ __half2 two_scales(unsigned bytes) {
     const unsigned bits = __byte_perm(bytes, 0u, ((I + 1) << 12) | (4 << 8) | (I << 4) | 4) >> 1;

@@ -40,4 +40,11 @@ template <int D> struct Fp4Unit {
     }
 };
 
+// The eight codes of a word as four pairs of halves.
+__device__ __forceinline__ void halves_of(unsigned word, unsigned (&h)[4]) {
+    asm("{\n.reg .b8 c0, c1, c2, c3;\nmov.b32 {c0, c1, c2, c3}, %4;\n"
+        "cvt.rn.f16x2.e2m1x2 %0, c0;\ncvt.rn.f16x2.e2m1x2 %1, c1;\ncvt.rn.f16x2.e2m1x2 %2, c2;\ncvt.rn.f16x2.e2m1x2 %3, c3;\n}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(word));
+}
+
 }  // namespace mrun
