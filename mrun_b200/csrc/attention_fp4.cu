@@ -22,11 +22,11 @@
 // A block is four warps; each copies its own units (two at a time, 32 keys) with cp.async into a ring of its own while it
 // works on the two before, across pairs: no barrier but where a pair's pieces meet.  Every warp of a block works on the same
 // (token, kv head, group of heads) pair.  The tiles (8 units) of short contexts are cut among the one to eight blocks of a pair's
-// cluster, which add their pieces through distributed shared memory.  Those of long ones lie in one list: dealt to the blocks that the
-// device holds at once by whole pairs where that is even, and otherwise cut evenly, so that a pair in several
-// blocks leaves its pieces in scratch, and a second kernel, whose launch overlaps the first one's end, adds them in block order.
+// cluster, which add their pieces through distributed shared memory.  Those of long ones lie in one list, cut evenly among the
+// blocks that the device holds at once (by whole pairs, where that is nearly even, 64 requests of 8,192 keys take 115 us and not 107); a pair that
+// lies in several blocks leaves its pieces in scratch, and a second kernel, whose launch overlaps the first one's end, adds them in block order.
 //
-// Measured (B200): 64 requests of up to 8,192 keys, 32 heads over 8 of 128 (456 MB): 84 us at 1,965 MHz, 5.5 TB/s, the start (positions, pages, first keys)
+// Measured (B200): 64 requests of up to 8,192 keys, 32 heads over 8 of 128 (456 MB): 81 us at 1,965 MHz, 5.6 TB/s, the start (positions, pages, first keys)
 // and the second launch among them.  267 instructions a unit, 64 of them conversions (the integer pipe
 // is 48 % busy) and 64 multiplications.  In a run of seconds the power cap brings the clock to 1,600 MHz.
 // One request of 1,024 keys: 5.6 us, a chain of latencies.  A ring of three stages, twelve warps a multiprocessor instead of sixteen, pages of 64
@@ -172,11 +172,11 @@ struct Rows {
 };
 
 // Sums tiles_of over the tokens into prefix[0 .. tokens], positions into held[0 .. tokens) and block-table rows into
-// held[tokens .. 2 tokens); all threads of the block.  Returns the most tiles that a token has.
-__device__ __forceinline__ int make_plan(int* prefix, int* held, const int* __restrict__ positions, const int* __restrict__ token_slot,
+// held[tokens .. 2 tokens); all threads of the block.
+__device__ __forceinline__ void make_plan(int* prefix, int* held, const int* __restrict__ positions, const int* __restrict__ token_slot,
                                           const Rows& rows, int tokens, int window, int table_units, int* scratch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int carried = 0, most = 0;
+    int carried = 0;
     if (threadIdx.x == 0) prefix[0] = 0;
     for (int first = 0; first < tokens; first += THREADS) {
         const int t = first + threadIdx.x;
@@ -189,7 +189,6 @@ __device__ __forceinline__ int make_plan(int* prefix, int* held, const int* __re
             held[tokens + t] = table_row;
         }
         int sum = tiles_of(pos, window, table_units);
-        most = max(most, sum);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int below = __shfl_up_sync(0xffffffffu, sum, o);
@@ -210,12 +209,7 @@ __device__ __forceinline__ int make_plan(int* prefix, int* held, const int* __re
         if (t < tokens) prefix[t + 1] = before + sum;
         __syncthreads();
     }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) scratch[WARPS + warp] = most;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) most = max(most, scratch[WARPS + w]);
-    return most;
 }
 
 // Tiles that a block takes.
@@ -232,7 +226,7 @@ struct Step {
     float scale_log2;
     float* part_o;               // [blocks, 2, HEADS, D]
     float2* part_ml;             // [blocks, 2, HEADS]: maximum, sum
-    int* plan;                   // [tokens + 1] the prefix of tiles, and whether every pair lies in one block
+    int* plan;                   // [tokens + 1]: the prefix of tiles
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -266,8 +260,8 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
     using Sh = Shape<D, FOUR>;
     constexpr int HEADS = Sh::HEADS, MINE = Sh::MINE, WORDS_K = D / 32, WORDS_V = D / 64, TILES_M = D / 32;
     constexpr int COLUMNS = FOUR ? 1 : 2;              // products that give 32 features of the heads
-    extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int scratch[2 * WARPS];
+    extern __shared__ __align__(128) unsigned char smem[];      // on 16 bytes the copies took 64 requests of up to 8,192 keys from 81 to 90 us
+    __shared__ int scratch[WARPS];
     float* merge = reinterpret_cast<float*>(smem + Sh::RING_BYTES);              // [WARPS][HEADS][ROW]
     int* prefix = reinterpret_cast<int*>(smem + Sh::RING_BYTES + Sh::MERGE_BYTES);
     int* held_pos = prefix + step.tokens + 1;
@@ -299,7 +293,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
         p.tile0 = rank * base + min(rank, more);
         count = p.tiles = base + (rank < more ? 1 : 0);
     } else {
-        const int most = make_plan(prefix, held_pos, step.positions, step.token_slot, rows, step.tokens, step.window, table_units, scratch);
+        make_plan(prefix, held_pos, step.positions, step.token_slot, rows, step.tokens, step.window, table_units, scratch);
         if (blockIdx.x == 0)
             for (int i = threadIdx.x; i <= step.tokens; i += THREADS) step.plan[i] = prefix[i];
         // rows without a tile (padding) come out as zeros
@@ -308,20 +302,9 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                 for (int i = threadIdx.x; i < step.heads * D / 2; i += THREADS)
                     reinterpret_cast<unsigned*>(out + (size_t)rows.of(tok) * step.heads * D)[i] = 0u;
 
-        // Whole pairs to a block where that leaves none with much more than its share: no piece is handed over then (64 requests of 512 to
-        // 1,024 keys, 8 kv heads: 17 us where the even cut takes 21).
-        const int total = prefix[step.tokens] * pairs, per = tiles_a_block(total, gridDim.x);
-        const int pairs_a_block = (step.tokens * pairs + (int)gridDim.x - 1) / (int)gridDim.x;
-        const bool aligned = pairs_a_block * most <= per + max(2, per / 4);
-        if (blockIdx.x == 0 && threadIdx.x == 0) step.plan[step.tokens + 1] = aligned;
-        auto tiles_before = [&](int pair) {            // of all tokens' pairs
-            if (pair >= step.tokens * pairs) return total;
-            const int tok = pair / pairs;
-            return prefix[tok] * pairs + (pair - tok * pairs) * (prefix[tok + 1] - prefix[tok]);
-        };
-        const int begin = aligned ? tiles_before(min((int)blockIdx.x * pairs_a_block, step.tokens * pairs)) : min((int)blockIdx.x * per, total);
-        count = (aligned ? tiles_before(min(((int)blockIdx.x + 1) * pairs_a_block, step.tokens * pairs)) : min(begin + per, total)) - begin;
-        if (count == 0) return;
+        const int total = prefix[step.tokens] * pairs, per = tiles_a_block(total, gridDim.x), begin = blockIdx.x * per;
+        if (begin >= total) return;
+        count = min(per, total - begin);
         int low = 0, high = step.tokens - 1;           // the token whose tiles hold the block's first one
         while (low < high) {
             const int mid = (low + high) / 2;
@@ -717,7 +700,7 @@ merge_fp4_kernel(bf16* __restrict__ out, const Step step, const __grid_constant_
     wait_for_kernel_before();
     const int before = __ldcg(step.plan + tok), tiles = __ldcg(step.plan + tok + 1) - before;
     const int total = __ldcg(step.plan + step.tokens) * pairs;
-    if (tiles == 0 || __ldcg(step.plan + step.tokens + 1)) return;
+    if (tiles == 0) return;
     const int per = tiles_a_block(total, blocks), start = before * pairs + pair * tiles;
     const int first = start / per, last = (start + tiles - 1) / per;
     if (first == last) return;
@@ -846,7 +829,7 @@ MRUN_API int mrun_attn_fp4_occupancy(int head_dim, int group) {
 
 
 // One token a row of q, out, positions and token_slot: the first `tokens` rows, or those that `rows` (host memory) names.  scratch:
-// 4-byte words: blocks * 2 * (4 or 8 heads) * (head_dim + 2) + tokens + 2, on 16 bytes.  cluster: 0, or the blocks of a
+// 4-byte words: blocks * 2 * (4 or 8 heads) * (head_dim + 2) + tokens + 1, on 16 bytes.  cluster: 0, or the blocks of a
 // cluster (1, 2, 4, 8) that takes a pair; `scratch` and `blocks` are not used then.
 MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const void* cache, const int* block_tables, int table_rows,
                                   int max_blocks, const int* token_slot, const int* positions, const int* rows, int tokens, int heads,

@@ -71,6 +71,8 @@ class Executor:
         # captured decode steps: rows (a power of two) -> reach -> graph.  The reach is an upper
         # bound of the contexts a graph was captured for (parts see it as ``ctx.max_kv_len`` and
         # may choose kernels by it); the host takes the smallest reach that covers the step.
+        if kv_cache == "fp4":      # its attention takes short contexts in another way (``kernels.attention.fp4_cluster``)
+            self.REACHES = (2048, *self.REACHES)
         self._graphs: Dict[int, Dict[int, "DecodeGraph"]] = {}
         self._graph_tokens: Dict[int, torch.Tensor] = {}
         self._last_graph: Dict[int, "DecodeGraph"] = {}
@@ -151,7 +153,7 @@ class Executor:
 
     def decode_reach(self, longest: int) -> int:
         """The context bound of the captured step that takes a step whose longest request will
-        hold ``longest`` tokens: 4,096, 16,384 or the model's positions."""
+        hold ``longest`` tokens: 4,096, 16,384 or the model's positions (with a 4-bit cache also 2,048)."""
         for reach in self.REACHES:
             if longest <= reach < self.spec.max_positions:
                 return reach

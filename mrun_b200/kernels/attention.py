@@ -533,8 +533,9 @@ FP4_MAX_TOKENS = 256       # tokens of one launch of the decode kernel
 FP4_TILE_KEYS = 128        # keys that its blocks are dealt together
 
 
-# The most tiles that a block of a cluster takes, where the clusters leave most of the device empty, and where they do not.
-FP4_CLUSTER_TILES = (4, 8)
+# The most tiles that a block takes of a pair that is a cluster's: where the clusters leave most of the device empty, where they do not, and
+# where a single block is one.
+FP4_CLUSTER_TILES = (4, 8, 16)
 
 
 def fp4_cluster(pairs: int, slots: int, longest: int) -> int:
@@ -544,14 +545,15 @@ def fp4_cluster(pairs: int, slots: int, longest: int) -> int:
     A tile takes a block about 1.4 us, and a cluster of 2, 4 or 8 costs 0.3, 0.8 or 1.5 us over a single block: hence two tiles a block,
     as far as the device holds the blocks (B200, 32 heads over 8 of 128, one request, us in clusters of 1 / 2 / 4 / 8 / dealt: 128 keys
     4.0 / 4.3 / 4.8 / 5.4 / 5.4; 512 6.2 / 5.0 / 4.9 / 5.5 / 6.9; 2,048 15.0 / 9.4 / 7.2 / 6.1 / 7.4).  Long contexts are dealt, since a
-    step would wait for the cluster of the longest of them (two requests of 8,192 keys and thirty of 512: 29 in clusters, 18 dealt; of
-    2,048 and 128: 10.8 and 12.6), and sooner where the clusters fill little of the device (one request of 4,096: 10.0 and 9.7; 32 of
-    2,048: 14.9 and 19.5)."""
+    step would wait for the cluster of the longest of them (in clusters / dealt: one request of 4,096 keys 10.0 / 9.7; 32 of 2,048 17.8 / 21.4, of
+    4,096 32.0 / 34.6, of up to 4,096 28.9 / 26.0, two of 8,192 and thirty of 512 29 / 18; 64 of 2,048 31.7 / 35.4, of up to 2,048
+    21.1 / 25.7, of 8,192 121 / 107; 256 of 2,048 111 / 113, of up to 2,048 56 / 71)."""
     tiles, cluster = -(-longest // FP4_TILE_KEYS), 1
     while cluster < 8 and tiles > 2 * cluster and 2 * cluster * pairs <= slots:
         cluster *= 2
-    few = tiles <= cluster * FP4_CLUSTER_TILES[5 * cluster * pairs >= 2 * slots]
-    return cluster if few and pairs < 65536 else 0         # pairs are the second axis of a grid
+    empty, full, single = FP4_CLUSTER_TILES
+    most = single if cluster == 1 else full if 5 * cluster * pairs >= 2 * slots else empty
+    return cluster if tiles <= cluster * most and pairs < 65536 else 0        # pairs are the second axis of a grid
 
 
 def _fp4_tokens(q, q_stride: int, out, cache, group, ctx, heads: int, head_dim: int, scale: float, window: int, rows=None) -> None:
@@ -572,7 +574,7 @@ def _fp4_tokens(q, q_stride: int, out, cache, group, ctx, heads: int, head_dim: 
         if not cluster:
             blocks = max(1, min(slots, n * tiles_a_token))
             # the pieces of two pairs a block (sums, maximum and sum a head), and the prefix of tiles
-            scratch = torch.empty(blocks * 2 * block_heads * (head_dim + 2) + n + 2, dtype=torch.float32, device=q.device)
+            scratch = torch.empty(blocks * 2 * block_heads * (head_dim + 2) + n + 1, dtype=torch.float32, device=q.device)
         if rows is None:
             listed, at = None, first
         else:

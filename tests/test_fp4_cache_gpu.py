@@ -309,9 +309,9 @@ def test_pairs_in_clusters_and_dealt_to_all_blocks(monkeypatch, tiles, heads, kv
     from mrun_b200.kernels import attention as module
     rule = module.fp4_cluster
     assert [rule(8, 592, keys) for keys in (1, 256, 257, 513, 1025, 4096, 4097)] == [1, 1, 2, 4, 8, 8, 0]
-    assert [rule(pairs, 592, 2048) for pairs in (74, 75, 148, 149, 296, 297)] == [8, 4, 4, 2, 2, 0]
-    assert [rule(pairs, 592, 1024) for pairs in (296, 297, 2048)] == [2, 1, 1] and rule(2048, 592, 1025) == 0 and rule(65536, 592, 1) == 0
-    monkeypatch.setattr(module, "FP4_CLUSTER_TILES", (tiles,) * 2)
+    assert [rule(pairs, 592, 2048) for pairs in (74, 75, 148, 149, 296, 297)] == [8, 4, 4, 2, 2, 1]
+    assert [rule(pairs, 592, 2049) for pairs in (296, 297, 2048)] == [0, 0, 0] and rule(2048, 592, 2048) == 1 and rule(65536, 592, 1) == 0
+    monkeypatch.setattr(module, "FP4_CLUSTER_TILES", (tiles,) * 3)
     page = 16
     c = Filled(lengths, kv_heads, dim, page, seed=heads)
     repeat = 1 + tiles % 2 * 20                                # also with so many pairs that clusters are smaller
@@ -568,5 +568,5 @@ def test_write_then_attend():
     test_nan_where_it_is_seen_and_only_there, test_captured_twice_and_replayed_at_once, test_same_bits_every_time, test_write_then_attend])
 def test_the_same_dealt_to_all_blocks(monkeypatch, test):
     from mrun_b200.kernels import attention as module
-    monkeypatch.setattr(module, "FP4_CLUSTER_TILES", (0, 0))
+    monkeypatch.setattr(module, "FP4_CLUSTER_TILES", (0, 0, 0))
     test()

@@ -110,6 +110,31 @@ def test_logits_under_every_cutting(name, tmp_path, monkeypatch):
     ex.cache.check_invariants()
 
 
+def test_captured_steps_of_several_bounds(tmp_path, monkeypatch):
+    """A request that grows past the bounds of its captured steps, beside a short one: the logits of the plain model."""
+    from mrun_b200.engine import StepEntry
+    from mrun_b200.engine.loading import executor_from_folder
+    folder = make_folder("E", str(tmp_path / "m"))
+    cfg, weights = plain.load_folder(folder)
+    tokens = random_tokens(cfg["vocab_size"], 150, seed=6)
+    exact = plain.forward(cfg, weights, tokens).numpy()
+    monkeypatch.setattr(plain, "attention_block", held_block)
+    want = plain.forward(cfg, weights, tokens).numpy()
+    allowed = TOLERANCE["bfloat16"] + rel_error(exact, want)
+    assert executor_from_folder(folder, num_pages=8, max_requests=2).REACHES == (4096, 16384)
+    ex = executor_from_folder(folder, num_pages=32, max_requests=2, kv_cache="fp4")
+    assert ex.REACHES == (2048, 4096, 16384)
+    ex.REACHES = (40, 100)
+    long, short = ex.admit("long"), ex.admit("short")
+    ex.step([StepEntry(long, tokens[:30], [])])
+    ex.step([StepEntry(short, tokens[:2], [])])
+    for i in range(110):
+        ex.decode_step([StepEntry(long, [tokens[30 + i]], [0]), StepEntry(short, [tokens[2 + i]], [0])])
+        got = ex.decode_logits([None, None]).cpu().numpy()
+        assert rel_error(got, want[[30 + i, 2 + i]]) <= allowed
+    assert [reach for reach in ex._graphs[2] if reach <= 100] == [40, 100] and len(ex._graphs[2]) == 3
+
+
 def test_generation_is_the_same_every_time_and_in_company(tmp_path):
     from mrun_b200 import Engine
     folder = make_folder("E", str(tmp_path / "m"))
