@@ -12,8 +12,8 @@
 //                                      neighbouring features of one key, not two keys of one feature.
 // The second product gets its sum over keys all the same: its k index is (key, parity of the feature), and a column
 // of P has zeros in the places of one parity, so that it gives the features of the other.  A group of up to four query
-// heads has both columns of a head in one product; a wider one takes two products, one a parity, still a fifth of the tensor
-// pipe's time at the memory's rate, and no permutation of the values.
+// heads has both columns of a head in one product (the tensor pipe is 28 % busy); a wider one takes two products, one a parity, and
+// no permutation of the values.
 // P comes out of the first product by rows and goes into the second by columns: one movmatrix for 8 keys.
 // Queries are scaled by a power of two into a half's range (exact for 24 binary digits below the largest);
 // P carries a factor of 32, so that a half keeps its digits down to 2^-19 of the running maximum, which is raised
