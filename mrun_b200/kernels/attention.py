@@ -587,7 +587,8 @@ def _fp4_tokens(q, q_stride: int, out, cache, group, ctx, heads: int, head_dim: 
 
 def _fp4_portions(ctx, window: int, heads: int, kv_heads: int):
     """What a step's prompt portions need, made once per step: the rows that go one by one, and for the longer segments the spans of tokens
-    to read back, their pages, and a step context and block tables over these, which the first layer's call fills."""
+    to read back, their pages, and a step context and block tables over these, which every call's read back writes (a few words:
+    nothing then depends on whether an earlier call came to its end, and on which stream)."""
     key = ("fp4_portions", window, heads, kv_heads)
     found = ctx.shared.get(key)
     if found is not None:
@@ -657,13 +658,11 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
         return out
     if tokens > ctx.real_tokens:
         out[ctx.real_tokens:].zero_()
-    filled = ("fp4_portions", window, heads, kv_heads) in ctx.shared
     rows, longer = _fp4_portions(ctx, window, heads, kv_heads)
     if rows:
         _fp4_tokens(q, q_stride, out, cache, group, ctx, heads, head_dim, scale, window, rows)
     if longer is not None:
         spans, n, table, span_of_row, inner, view = longer
-        k, v = ops.fp4_spans(cache, head_dim, group.block_tables, spans, n, FP4_SCRATCH_ROWS, None if filled else table,
-                             None if filled else span_of_row)
+        k, v = ops.fp4_spans(cache, head_dim, group.block_tables, spans, n, FP4_SCRATCH_ROWS, table, span_of_row)
         paged_attention(q, q_stride, out, _Pages(k, v), view, inner, heads, scale, window)
     return out
