@@ -113,6 +113,17 @@ __device__ __forceinline__ void store_row(bf16* dst, float4 acc, float l) {
     *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(two);
 }
 
+// Powers of two that bring a head's queries, the largest of them `largest`, into [128, 256) and its scores back; a head of zeros or with an
+// infinity stays as it is.
+struct Powers {
+    float up, down;
+};
+__device__ __forceinline__ Powers powers_of(float largest) {
+    int ex = (int)(__float_as_uint(largest) >> 23);
+    ex = ex == 255 || largest == 0.f ? 134 : max(ex, 8);
+    return {__uint_as_float((unsigned)(261 - ex) << 23), __uint_as_float((unsigned)(ex - 7) << 23)};
+}
+
 // Tiles of a token that sees the keys from the first visible one to its own position, as far as its block table goes.
 __device__ __forceinline__ int tiles_of(int pos, int window, int table_units) {
     if (pos < 0) return 0;
@@ -402,10 +413,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
             }
             largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
             largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-            // 2^(7 - exponent) and its inverse; a head of zeros or with an infinity stays as it is
-            int ex = (int)(__float_as_uint(largest) >> 23);
-            ex = ex == 255 || largest == 0.f ? 134 : max(ex, 8);
-            const float up = __uint_as_float((unsigned)(261 - ex) << 23), down = __uint_as_float((unsigned)(ex - 7) << 23);
+            const auto [up, down] = powers_of(largest);
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
                 const __nv_bfloat162* two = reinterpret_cast<const __nv_bfloat162*>(&raw[c]);
@@ -760,6 +768,114 @@ merge_fp4_kernel(bf16* __restrict__ out, const Step step, const __grid_constant_
     store_row(dst, acc, l);
 }
 
+// ------------------------------------------------------------------------------------------
+// Rows of prompt portions that see a page which is not held, or a position behind their block table.  The portions' keys are read back for
+// the prompt kernels, which know no hole among the keys of a row: there such a key is one of zeros, with a score of 0.  This kernel runs
+// behind them: a block looks through the pages that its portion sees, and where one is not held (the books of an engine's cache never
+// leave that) computes the portion's rows again from the 4-bit pages, a warp a row and query head, a key to eight or sixteen lanes, in 32 bits.
+// Nothing is tuned but the look: a call of 2,048 tokens, or of 1,531 behind 9,000, takes 2 us longer with it (55 -> 57, 265 -> 267).
+// ------------------------------------------------------------------------------------------
+constexpr int UNHELD_THREADS = 256, MAX_PORTIONS = 64;
+
+struct Portion {
+    int table_row, position, row0, rows;     // its block-table row, its first token's position, its rows of the step
+};
+struct Portions {
+    int n;
+    Portion portion[MAX_PORTIONS];
+};
+
+template <int D>
+__global__ void __launch_bounds__(UNHELD_THREADS)
+unheld_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsigned char* __restrict__ cache, const Step step,
+                  const __grid_constant__ Portions portions) {
+    using Unit = Fp4Unit<D>;
+    constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;      // lanes of a key, eight features each; keys that a warp takes at a time
+    const Portion portion = portions.portion[blockIdx.y];
+    const int units_a_page = step.page_size / FP4_TOKENS, lane = threadIdx.x & 31, part = lane % LANES;
+    const bool listed = portion.table_row >= 0 && portion.table_row < step.table_rows;
+    const int* table = step.block_tables + (size_t)(listed ? portion.table_row : 0) * step.max_blocks;
+    auto page_of = [&](int block) { return listed && block < step.max_blocks ? __ldg(table + block) : -1; };
+    const int last_block = (portion.position + portion.rows - 1) / step.page_size;
+    int missing = 0;
+    for (int block = first_visible(portion.position, step.window) / step.page_size + threadIdx.x; block <= last_block && !missing; block += UNHELD_THREADS)
+        missing |= (unsigned)page_of(block) >= (unsigned)step.pages;
+    if (!__syncthreads_or(missing)) return;
+
+    const int group = step.heads / step.kv_heads;
+    const unsigned items = (unsigned)portion.rows * step.heads;
+    for (unsigned item = blockIdx.x * (UNHELD_THREADS / 32) + (threadIdx.x >> 5); item < items; item += gridDim.x * (UNHELD_THREADS / 32)) {
+        const int i = item / step.heads, head = item - i * step.heads, kvh = head / group;
+        const size_t row = portion.row0 + i;
+        const int pos = portion.position + i, lo = first_visible(pos, step.window);
+        const uint4 raw = *reinterpret_cast<const uint4*>(q + row * step.q_stride + (size_t)head * D + part * 8);
+        const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
+        float qs[8], largest = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            qs[e] = __bfloat162float(e % 2 ? pairs[e / 2].y : pairs[e / 2].x);
+            largest = fmaxf(largest, fabsf(qs[e]));
+        }
+        const auto [up, down] = powers_of(warp_max(largest));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qs[e] *= up;
+        const float scale = fmaxf(down * step.scale_log2, FLT_MIN);
+        float m = -INFINITY, l = 0.f, acc[8] = {};               // of every AT_ONCE-th key
+        for (int unit = lo / FP4_TOKENS, last = min(pos / FP4_TOKENS, step.max_blocks * units_a_page - 1); unit <= last; ++unit) {
+            const int block = unit / units_a_page, page = page_of(block);
+            if ((unsigned)page >= (unsigned)step.pages) continue;
+            const unsigned char* at = cache + (size_t)page * step.page_bytes + (size_t)(kvh * units_a_page + unit - block * units_a_page) * Unit::BYTES;
+#pragma unroll 1
+            for (int r = lane / LANES; r < FP4_TOKENS; r += AT_ONCE) {
+                auto values = [&](int code, int scale_byte, float (&x)[8]) {
+                    unsigned two[4];
+                    halves_of(*reinterpret_cast<const unsigned*>(at + code), two);
+                    const float s = __half2float(__ushort_as_half((unsigned short)(at[scale_byte] << 7)));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two[e]));
+                        x[2 * e] = f.x * s;
+                        x[2 * e + 1] = f.y * s;
+                    }
+                };
+                float x[8], dot = 0.f;
+                values(Unit::k_code(r, part * 4), Unit::k_scale(r, part / 2), x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dot = fmaf(qs[e], x[e], dot);
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+                const int key = unit * FP4_TOKENS + r;
+                if (key >= lo && key <= pos) {                   // a hidden key may lie in memory that nothing has written
+                    const float score = __fmul_rn(dot, scale), top = fmaxf(m, score);
+                    const float corr = m == -INFINITY ? 0.f : exp2f(m - top), p = top == -INFINITY && score == top ? 0.f : exp2f(score - top);
+                    values(Unit::v_code(r, part * 4), Unit::v_scale(r, part / 2), x);
+                    m = top;
+                    l = l * corr + p;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[e] = acc[e] * corr + p * x[e];
+                }
+                __syncwarp();
+            }
+        }
+        const float top = warp_max(m), f = weight_of(m, l, top);
+        l *= f;
+#pragma unroll
+        for (int o = LANES; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint4 packed;
+        __nv_bfloat162* sums = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            acc[e] *= f;
+#pragma unroll
+            for (int o = LANES; o < 32; o <<= 1) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[e] = __floats2bfloat162_rn(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+        if (lane < LANES) *reinterpret_cast<uint4*>(out + (row * step.heads + head) * D + part * 8) = packed;
+    }
+}
+
 // Lets the decode kernel have its shared memory on the current device, once a device.
 template <int D, bool FOUR, bool CLUSTERED> cudaError_t allow_shared() {
     static std::atomic<unsigned long long> allowed{0};
@@ -867,5 +983,54 @@ MRUN_API int mrun_attn_fp4_decode(const void* q, long q_stride, void* out, const
                                  : (group <= 4 ? launch_decode<128, true> : launch_decode<128, false>);
     MRUN_CHECK_CUDA(launch((const bf16*)q, (bf16*)out, (const unsigned char*)cache, step, selected, blocks, cluster, stream), name);
     MRUN_CHECK_LAUNCH(name);
+    return 0;
+}
+
+// The rows of `portions` (host memory: int [n, 4], see Portion) that see a page which is not held, or a position behind their block table, again, such
+// keys left out; the others stay as they are.  Rows and positions come from `portions` alone.
+MRUN_API int mrun_attn_fp4_unheld(const void* q, long q_stride, void* out, const void* cache, const int* block_tables, int table_rows,
+                                  int max_blocks, const int* portions, int n, int heads, int kv_heads, int head_dim, int page_size, long pages,
+                                  float scale, int window, cudaStream_t stream) {
+    const char* name = "paged_attention_fp4";
+    MRUN_REQUIRE(n >= 0 && (n == 0 || portions) && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && pages >= 0 && max_blocks >= 0 && table_rows >= 0,
+                 "%s: bad sizes", name);
+    MRUN_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim=%d: the 4-bit cache takes heads of 64 or 128 features", name, head_dim);
+    MRUN_REQUIRE(page_size > 0 && page_size % FP4_TOKENS == 0, "%s: page_size=%d is not a multiple of 16", name, page_size);
+    MRUN_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) & 15) == 0 && q_stride % 8 == 0, "%s: rows and pages start on 16 bytes", name);
+    const long page_units = page_size / FP4_TOKENS;
+    MRUN_REQUIRE(pages < (1L << 31) && page_units * kv_heads * 18 * head_dim < (1L << 31), "%s: pages=%ld of %d tokens and %d kv heads", name,
+                 pages, page_size, kv_heads);
+    MRUN_REQUIRE(max_blocks * page_units < (1L << 31), "%s: block tables of %d pages of %d tokens", name, max_blocks, page_size);
+    MRUN_REQUIRE(scale > 0.f && scale < FLT_MAX, "%s: scale=%g is not a positive number", name, (double)scale);
+    Step step = {};
+    step.block_tables = block_tables;
+    step.max_blocks = max_blocks;
+    step.table_rows = table_rows;
+    step.heads = heads;
+    step.kv_heads = kv_heads;
+    step.page_size = page_size;
+    step.window = window;
+    step.pages = (int)pages;
+    step.page_bytes = (unsigned)(page_units * kv_heads * 18 * head_dim);
+    step.q_stride = q_stride;
+    step.scale_log2 = scale * 1.4426950408889634f;
+    for (int first = 0; first < n; first += MAX_PORTIONS) {
+        Portions part = {};
+        part.n = n - first < MAX_PORTIONS ? n - first : MAX_PORTIONS;
+        int most = 1;
+        for (int i = 0; i < part.n; ++i) {
+            const int* v = portions + 4 * (first + i);
+            MRUN_REQUIRE(v[1] >= 0 && v[2] >= 0 && v[3] > 0 && (long)v[1] + v[3] < (1L << 31) && (long)v[3] * heads < (1L << 30),
+                         "%s: a portion of %d tokens of %d heads at position %d", name, v[3], heads, v[1]);
+            part.portion[i] = Portion{v[0], v[1], v[2], v[3]};
+            most = v[3] > most ? v[3] : most;
+        }
+        // about two blocks a multiprocessor look at the pages; a portion whose rows are computed again has them as well
+        const int blocks = 296 / part.n > 1 ? 296 / part.n : 1, wanted = (int)(((long)most * heads + UNHELD_THREADS / 32 - 1) / (UNHELD_THREADS / 32));
+        const dim3 grid((unsigned)(blocks < wanted ? blocks : wanted), (unsigned)part.n);
+        MRUN_CHECK_CUDA(launch_kernel(head_dim == 64 ? unheld_fp4_kernel<64> : unheld_fp4_kernel<128>, grid, dim3(UNHELD_THREADS), 0, stream,
+                                      (const bf16*)q, (bf16*)out, (const unsigned char*)cache, step, part), name);
+        MRUN_CHECK_LAUNCH(name);
+    }
     return 0;
 }

@@ -631,9 +631,10 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
 
     Single tokens, and a few tokens more, read the 4-bit pages as they are (every step of single tokens may be captured in a
     graph).  The keys and values of longer segments are read back in bfloat16, 128 tokens a page, for the time of
-    the call (4 * head_dim bytes a token and kv head of the segments' contexts), and go to the prompt kernels.  A page outside the cache is not
-    seen; a row that sees nothing is zeros.  A value that is NaN makes NaN of the rows that see it, and may of other rows of
-    the same prompt portion."""
+    the call (4 * head_dim bytes a token and kv head of the segments' contexts), and go to the prompt kernels.  A page outside the cache,
+    and a position behind the block table, is not seen; a row that sees nothing is zeros.  Unless the step says that its pages are held
+    (``ctx.pages_held``) the longer segments' pages are looked through for such ones.  A value that is NaN makes NaN of the rows that see
+    it, and may of other rows of the same prompt portion."""
     pages, kv_heads, page_size = ops.check_fp4_cache(cache, head_dim)
     if heads < 1 or heads % kv_heads:
         raise ops.KernelError(f"paged_attention_fp4: heads={heads} is not a multiple of kv_heads={kv_heads}")
@@ -665,4 +666,11 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
         spans, n, table, span_of_row, inner, view = longer
         k, v = ops.fp4_spans(cache, head_dim, group.block_tables, spans, n, FP4_SCRATCH_ROWS, table, span_of_row)
         paged_attention(q, q_stride, out, _Pages(k, v), view, inner, heads, scale, window)
+        if not ctx.pages_held:
+            # what is read back has zeros in the places of keys that are not there: rows that see such ones are computed again
+            flat = (ctypes.c_int * (4 * len(spans)))(*[v for (slot, *_), seg in zip(spans, inner.segments)
+                                                      for v in (slot, seg.pos_start, seg.q_start, seg.q_len)])
+            tables = group.block_tables
+            _lib.fp4().call("mrun_attn_fp4_unheld", q.data_ptr(), q_stride, out.data_ptr(), cache.data_ptr(), tables.data_ptr(), tables.shape[0],
+                            tables.shape[1], ctypes.addressof(flat), len(spans), heads, kv_heads, head_dim, page_size, pages, scale, window, _queue())
     return out

@@ -18,7 +18,8 @@ def step_of(segments, page=16):
     return StepContext(num_tokens=at, num_segments=len(infos), segments=infos, token_ids=None, positions=positions,
                        token_slot=torch.cat([torch.full((n,), slot, dtype=torch.int32) for slot, n, _ in segments]), seg_q_start=None,
                        seg_kv_len=None, seg_slot=None, groups={}, max_q_len=max(n for _, n, _ in segments),
-                       max_kv_len=max(n + first for _, n, first in segments), page_size=page, real_tokens=at)
+                       max_kv_len=max(n + first for _, n, first in segments), page_size=page, real_tokens=at,
+                       pages_held=True)
 
 
 class Calls:
