@@ -78,13 +78,13 @@ __device__ __forceinline__ unsigned quantise(const double (&x)[8], unsigned mask
     scale = finite ? scale_byte(cut_sticky(fmin(largest / 6.0, 10240.0))) : (unsigned)FP4_NAN_SCALE;
     if (!finite) return 0u;
     const double s = scale_value(scale);
-    // A shade more than 1 / s, so that a quotient that is a border exactly is not cut below it.
-    const double inverse = s > 0.0 ? 1.0 / s * (1.0 + 8.8817841970012523e-16) : 0.0;
+    // A shade more than 1 / s, so that a quotient that is a border exactly is not cut below it.  Under a scale of zero any quotient rounds to zero.
+    const double inverse = s > 0.0 ? 1.0 / s * (1.0 + 8.8817841970012523e-16) : 1.0;
     float2 f[4];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         float& part = e % 2 ? f[e / 2].y : f[e / 2].x;
-        part = __double2float_rz(x[e] * inverse);
+        part = __double2float_rz(__fma_rn(x[e], inverse, 0.0));          // -0 + 0 is 0: only what is below zero keeps a sign
         if ((double)part * s != x[e]) part = __uint_as_float(__float_as_uint(part) | 1u);
     }
     return codes_of(f);
@@ -116,10 +116,10 @@ __device__ __forceinline__ unsigned quantise(const float2 (&x)[4], unsigned mask
         return 0u;
     }
     scale = scale_byte(to_12_bits(fminf(__uint_as_float(top) * (1.f / 6.f), 10240.f)));
-    const float s = scale_value(scale), inverse = s > 0.f ? __fdividef(1.f, s) : 0.f;
-    float2 f[4];
+    const float s = scale_value(scale), inverse = s > 0.f ? __fdividef(1.f, s) : 1.f;
+    float2 f[4];                                       // -0 + 0 is 0: only what is below zero keeps a sign
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = make_float2(to_12_bits(__fmul_rn(x[e].x, inverse)), to_12_bits(__fmul_rn(x[e].y, inverse)));
+    for (int e = 0; e < 4; ++e) f[e] = make_float2(to_12_bits(__fmaf_rn(x[e].x, inverse, 0.f)), to_12_bits(__fmaf_rn(x[e].y, inverse, 0.f)));
     return codes_of(f);
 }
 

@@ -1,9 +1,9 @@
 // The 4-bit key/value cache's unit: 16 tokens of one kv head, their keys and their values.
 //
 // Sixteen neighbouring features of a token share a scale; a value is scale * code.  The code is a
-// 4-bit float (E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign), two to a byte, the even feature in the
-// low half; the scale is an unsigned byte of 5 exponent and 3 mantissa bits, which are bits 7 to
-// 14 of the half of the same value (byte << 7 is that half).  The largest scale that is written is
+// 4-bit float (E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign: the bit of 8, set for values below zero, also where they
+// round to zero; a zero of either sign is code 0), two to a byte, the even feature in the low half; the scale is an
+// unsigned byte of 5 exponent and 3 mantissa bits, which are bits 7 to 14 of the half of the same value (byte << 7 is that half).  The largest scale that is written is
 // 10,240: every value is then a half and a bfloat16 exactly.  A group that holds a value that is not finite has
 // the scale byte 0xFF, a NaN.
 //
