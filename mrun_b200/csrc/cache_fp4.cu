@@ -187,15 +187,21 @@ template <int D> __device__ __forceinline__ void norm(double (&v)[8], const floa
     for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * (double)(e % 2 ? weight[e / 2].y : weight[e / 2].x);
 }
 
-// With WIDEST returns the largest |first| + |second| of what is added.
+// With WIDEST returns the largest |first| + |second| of the two products that are added, whatever the size of the cosines and sines.
 template <bool WIDEST> __device__ __forceinline__ float rotate(float2 (&v)[4], const Turn& turn, unsigned mask, int part) {
     const int from = (int)(threadIdx.x & 31) - part + turn.partner;
     float widest = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const float2 other = make_float2(__shfl_sync(mask, v[e].x, from), __shfl_sync(mask, v[e].y, from));
-        if constexpr (WIDEST) widest = fmaxf(widest, fmaxf(fabsf(v[e].x) + fabsf(other.x), fabsf(v[e].y) + fabsf(other.y)));
-        if (turn.turns) v[e] = __ffma2_rn(v[e], turn.c[e], __fmul2_rn(other, turn.s[e]));
+        if (turn.turns) {
+            const float2 second = __fmul2_rn(other, turn.s[e]);
+            if constexpr (WIDEST)
+                widest = fmaxf(widest, fmaxf(fmaf(fabsf(v[e].x), fabsf(turn.c[e].x), fabsf(second.x)), fmaf(fabsf(v[e].y), fabsf(turn.c[e].y), fabsf(second.y))));
+            v[e] = __ffma2_rn(v[e], turn.c[e], second);
+        } else if constexpr (WIDEST) {
+            widest = fmaxf(widest, fmaxf(fabsf(v[e].x), fabsf(v[e].y)));
+        }
     }
     return widest;
 }

@@ -47,3 +47,23 @@ def test_bytes_of_zeros_and_borders(dim, norm, rotary):
                                  cache)
     k = rotated(normed(v.double().view(16, 1, dim), weight, float(torch.tensor(1e-6))), rot).view(16, dim)
     assert torch.equal(cache.view(-1).cpu(), plain_fp4.unit_of(k, v.double()))
+
+
+@pytest.mark.parametrize("factor", [1.0, 1e3, 1e6])
+@pytest.mark.parametrize("norm", [True, False])
+def test_keys_under_a_rotary_table_of_any_size(factor, norm):
+    """Pairs whose two products all but cancel, under tables of any size: the bound within which a key is computed in 32 bits follows the
+    products, not the features alone."""
+    dim, tokens, page = 128, 1500, 16
+    qkv, (qw, kw), _ = inputs(tokens, 1, 1, dim, 0, seed=11, norm=norm)
+    x = normed(qkv.double().view(tokens, 3, dim)[:, 1:2], kw, float(torch.tensor(1e-6)))
+    g = torch.Generator().manual_seed(6)
+    a, b = x[:, 0, :dim // 2], x[:, 0, dim // 2:]
+    size = factor * torch.rand(tokens, dim // 2, generator=g).double() / torch.maximum(a.abs(), b.abs()).clamp(min=1e-3)
+    rot = torch.stack([size * b, size * a * (1 + 1e-3 * torch.randn(tokens, dim // 2, generator=g).double())], -1).float()
+    pages = -(-tokens // page)
+    cache = torch.zeros(ops().fp4_cache_shape(pages, 1, page, dim), dtype=torch.uint8, device=DEV)
+    ops().qk_norm_rope_cache_fp4(qkv.to(DEV), 1, 1, dim, to(qw), to(kw), 1e-6, to(rot), dim, torch.arange(tokens, dtype=torch.int32, device=DEV), cache)
+    k = ops().fp4_pages(cache, dim, torch.arange(pages, dtype=torch.int32, device=DEV))[0]
+    k = k.transpose(1, 2).reshape(-1, 1, dim)[:tokens].double().cpu()
+    assert torch.equal(k, plain_fp4.held(rotated(x, rot))[0])
