@@ -432,7 +432,7 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
 #pragma unroll
         for (int h = 0; h < MINE; ++h) {
             m[h] = -INFINITY;
-            nbase[h] = 1e38f;                              // any score raises it; one of -inf stays -inf
+            nbase[h] = FLT_MAX;                            // any score raises it; one of -inf stays -inf
             l[h] = 0.f;
         }
 #pragma unroll

@@ -67,3 +67,48 @@ def test_keys_under_a_rotary_table_of_any_size(factor, norm):
     k = ops().fp4_pages(cache, dim, torch.arange(pages, dtype=torch.int32, device=DEV))[0]
     k = k.transpose(1, 2).reshape(-1, 1, dim)[:tokens].double().cpu()
     assert torch.equal(k, plain_fp4.held(rotated(x, rot))[0])
+
+
+def rows_of(values, dim):
+    return torch.tensor(values, dtype=torch.float64).view(-1, 1, 1).expand(-1, 1, dim).contiguous()
+
+
+def fill(c, k, v):
+    """Writes float64 keys and values [n, 1, dim] into the pages of request 0 (16 keys a page)."""
+    units = -(-k.shape[0] // 16)
+    pad = lambda x: torch.cat([x, torch.zeros(units * 16 - x.shape[0], *x.shape[1:], dtype=torch.float64)]).view(units, 16, 1, -1).transpose(1, 2)
+    packed = plain_fp4.units_of(pad(k), pad(v))
+    for b in range(units):
+        c.cache[int(c.table[0, b]), :, 0] = packed[b].to(DEV)
+
+
+@pytest.mark.parametrize("tiles", [None, 0])
+@pytest.mark.parametrize("heads, n", [(1, 1), (4, 40), (8, 700)])
+def test_scores_near_the_end_of_32_bits(monkeypatch, tiles, heads, n):
+    """Every score of a row below -1e38: the row still is the softmax of them (here the value of the least negative one)."""
+    from mrun_b200.kernels import attention as module
+    if tiles is not None:
+        monkeypatch.setattr(module, "FP4_CLUSTER_TILES", (tiles,) * 3)
+    dim = 64
+    c = Filled([n], 1, dim, 16, seed=1)
+    g = torch.Generator().manual_seed(n)
+    size = torch.tensor([61440.0, 43008.0])[torch.randint(0, 2, (n,), generator=g)]
+    size[n // 2] = 30720.0
+    k, v = rows_of(size.tolist(), dim), torch.randn(n, 1, dim, generator=g).double()
+    fill(c, k, v)
+    k, v = plain_fp4.held(k)[0], plain_fp4.held(v)[0]
+    assert torch.equal(k[:, 0, 0].float(), size)
+    for sign in (-1.0, 1.0):
+        q = torch.full((1, heads * dim), sign * 2.0 ** 105).bfloat16()
+        size[n // 2] = 30720.0 if sign < 0 else 61440.0
+        score = q[0, 0].double() * dim * k[:, 0, 0] * 1.4426950408889634
+        assert score.abs().min() > 1e38 and score.abs().max() < 3e38
+        if sign > 0 and n > 1:          # one key above the others
+            size = torch.full((n,), 43008.0)
+            size[n // 3] = 61440.0
+            k = rows_of(size.tolist(), dim)
+            fill(c, k, v)
+        ctx, group = step_of([(0, 1, n - 1)], c.table.to(DEV), 16)
+        out = torch.empty(1, heads * dim, dtype=torch.bfloat16, device=DEV)
+        attention(q.to(DEV), heads * dim, out, c.cache, group, ctx, heads, dim, 1.0)
+        close(out, plain_fp4.attend(q.view(1, heads, dim), k, v, [n - 1], 1.0).view(1, -1), [v], 2.0 ** -10)
