@@ -124,6 +124,10 @@ __device__ __forceinline__ Powers powers_of(float largest) {
     return {__uint_as_float((unsigned)(261 - ex) << 23), __uint_as_float((unsigned)(ex - 7) << 23)};
 }
 
+// What a product with such queries is multiplied by.  Never 0, which would make NaN of a hidden key's score (a head that small has scores of 0
+// either way), nor infinite, which would make NaN of a key of zeros (any other score of such a head is beyond 32 bits either way).
+__device__ __forceinline__ float score_scale(float down, float scale_log2) { return fminf(fmaxf(down * scale_log2, FLT_MIN), FLT_MAX); }
+
 // Tiles of a token that sees the keys from the first visible one to its own position, as far as its block table goes.
 __device__ __forceinline__ int tiles_of(int pos, int window, int table_units) {
     if (pos < 0) return 0;
@@ -423,9 +427,8 @@ decode_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
                     qf[c * 2 + (e >> 1)][e & 1] = pack_h2(f.x * up, f.y * up);
                 }
             }
-            // never 0, which would make NaN of a hidden key's score (a head that small has scores of 0 either way)
 #pragma unroll
-            for (int h = 0; h < MINE; ++h) scale[h] = fmaxf(__shfl_sync(0xffffffffu, down, 8 * t + 4 * h) * step.scale_log2, FLT_MIN);
+            for (int h = 0; h < MINE; ++h) scale[h] = score_scale(__shfl_sync(0xffffffffu, down, 8 * t + 4 * h), step.scale_log2);
         }
 
         float m[MINE], nbase[MINE], l[MINE], o[TILES_M][COLUMNS][4];         // nbase: LIFT less the maximum
@@ -819,7 +822,7 @@ unheld_fp4_kernel(const bf16* __restrict__ q, bf16* __restrict__ out, const unsi
         const auto [up, down] = powers_of(warp_max(largest));
 #pragma unroll
         for (int e = 0; e < 8; ++e) qs[e] *= up;
-        const float scale = fmaxf(down * step.scale_log2, FLT_MIN);
+        const float scale = score_scale(down, step.scale_log2);
         float m = -INFINITY, l = 0.f, acc[8] = {};               // of every AT_ONCE-th key
         for (int unit = lo / FP4_TOKENS, last = min(pos / FP4_TOKENS, step.max_blocks * units_a_page - 1); unit <= last; ++unit) {
             const int block = unit / units_a_page, page = page_of(block);

@@ -112,3 +112,21 @@ def test_scores_near_the_end_of_32_bits(monkeypatch, tiles, heads, n):
         out = torch.empty(1, heads * dim, dtype=torch.bfloat16, device=DEV)
         attention(q.to(DEV), heads * dim, out, c.cache, group, ctx, heads, dim, 1.0)
         close(out, plain_fp4.attend(q.view(1, heads, dim), k, v, [n - 1], 1.0).view(1, -1), [v], 2.0 ** -10)
+
+
+@pytest.mark.parametrize("tiles", [None, 0])
+def test_keys_of_zeros_under_a_scale_that_leaves_the_range(monkeypatch, tiles):
+    """2^126 times 2^10 is no 32-bit number, its product with a key of zeros is 0: the mean of the values."""
+    from mrun_b200.kernels import attention as module
+    if tiles is not None:
+        monkeypatch.setattr(module, "FP4_CLUSTER_TILES", (tiles,) * 3)
+    heads, dim, n = 4, 128, 50
+    c = Filled([n], 1, dim, 16, seed=1)
+    v = torch.randn(n, 1, dim, generator=torch.Generator().manual_seed(2)).double()
+    fill(c, torch.zeros_like(v), v)
+    v = plain_fp4.held(v)[0]
+    q = torch.full((1, heads * dim), 2.0 ** 126).bfloat16()
+    ctx, group = step_of([(0, 1, n - 1)], c.table.to(DEV), 16)
+    out = torch.empty(1, heads * dim, dtype=torch.bfloat16, device=DEV)
+    attention(q.to(DEV), heads * dim, out, c.cache, group, ctx, heads, dim, 2.0 ** 10)
+    close(out, v.mean(0).repeat(1, heads).view(1, -1), [v], 2.0 ** -10)
