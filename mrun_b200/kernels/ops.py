@@ -366,7 +366,9 @@ def fp4_spans(cache: torch.Tensor, head_dim: int, block_tables: torch.Tensor, sp
     """(keys, values): bfloat16 [pages, kv heads, rows, head_dim] each, the contexts of several requests one after the other.  ``spans``: a
     tuple (block-table row, first token, end, first output page, first row of the step, rows of the step) for each; a span begins with a
     page's first row, and rows behind its end are zeros.  ``table`` (int32 [spans, blocks]) gets the spans' own block tables over the
-    output, ``span_of_row`` (int32 [rows of the step]) the span of their rows of the step."""
+    output, ``span_of_row`` (int32 [rows of the step]) the span of their rows of the step.  The spans take all of the ``pages``."""
+    if rows < 1 or rows % FP4_TOKENS:
+        raise KernelError(f"fp4_spans: pages of {rows} rows, a multiple of {FP4_TOKENS} is needed")
     if block_tables.dim() != 2:
         raise KernelError(f"fp4_spans: block_tables {tuple(block_tables.shape)}")
     held, kv_heads, page_size = check_fp4_cache(cache, head_dim)
@@ -378,9 +380,12 @@ def fp4_spans(cache: torch.Tensor, head_dim: int, block_tables: torch.Tensor, sp
         if t is not None:
             _check(t, name, torch.int32)
     for span in spans:
-        if (not all(0 <= value < 1 << 31 for value in span[1:]) or span[2] - span[1] + span[3] * rows > pages * rows
+        if (not all(0 <= value < 1 << 31 for value in span[1:]) or not -1 << 31 <= span[0] < 1 << 31 or span[2] - span[1] + span[3] * rows > pages * rows
                 or (table is not None and span[4] + span[5] > span_of_row.numel())):
             raise KernelError(f"fp4_spans: span {span} does not fit {pages} pages of {rows} rows")
+    taken = spans[-1][3] - (spans[-1][1] - spans[-1][2]) // rows if spans else 0
+    if taken != pages:
+        raise KernelError(f"fp4_spans: the spans take {taken} of {pages} pages, nothing would be written to the others")
     k, v = torch.empty((2, pages, kv_heads, rows, head_dim), dtype=torch.bfloat16, device=cache.device).unbind(0)
     flat = (ctypes.c_int * (6 * len(spans)))(*[value for span in spans for value in span])
     _lib.fp4().call("mrun_fp4_spans", cache.data_ptr(), ctypes.addressof(flat), len(spans), block_tables.data_ptr(), block_tables.shape[0],

@@ -85,3 +85,18 @@ def test_a_step_whose_pages_are_held_is_not_looked_through():
         attention(q, heads * dim, outs[-1], c.cache, group, ctx, heads, dim, dim ** -0.5)
         calls.append(lib.call_count() - before)
     assert torch.equal(*outs) and calls[0] == calls[1] + 1
+
+
+def test_spans_that_leave_pages_or_name_no_row_are_refused():
+    """Pages that no span takes would come back as memory that nobody wrote; a row number of more than 32 bits is not cut to another row."""
+    from mrun_b200.kernels import KernelError, ops
+    c = Filled([100], 2, 64, 16)
+    table = c.table.to(DEV)
+    for spans, pages, rows in (([(0, 0, 100, 0, 0, 4)], 3, 64), ([], 1, 64), ([(0, 0, 64, 0, 0, 4)], 2, 64), ([(1 << 32, 0, 100, 0, 0, 4)], 2, 64),
+                               ([(-1 << 33, 0, 100, 0, 0, 4)], 2, 64), ([(0, 0, 100, 0, 0, 4)], 2, 0), ([(0, 0, 100, 0, 0, 4)], 2, 60)):
+        with pytest.raises(KernelError):
+            ops.fp4_spans(c.cache, 64, table, spans, pages, rows)
+    k, v = ops.fp4_spans(c.cache, 64, table, [(0, 0, 64, 0, 0, 1), (-7, 0, 65, 1, 0, 1), (0, 64, 100, 3, 0, 1)], 4, 64)
+    got = torch.cat([k[0], k[3]], 1).double().cpu().transpose(0, 1)
+    assert torch.equal(got[:100], c.k[0]) and not got[100:].any() and not k[1:3].any() and not v[1:3].any()
+    assert [x.shape[0] for x in ops.fp4_spans(c.cache, 64, table, [], 0, 64)] == [0, 0]
