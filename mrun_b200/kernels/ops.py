@@ -298,7 +298,7 @@ def qk_norm_rope_cache_fp4(qkv: torch.Tensor, heads: int, kv_heads: int, head_di
                            rot: Optional[torch.Tensor], rotary_dim: int, slots: Optional[torch.Tensor],
                            cache: Optional[torch.Tensor], q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """As :func:`qk_norm_rope_cache` for bfloat16 rows and a 4-bit cache (``cache``: pages of :func:`fp4_cache_shape`): q in place,
-    or into the rows ``q_out`` (which may be strided) with ``qkv`` left as it is; k (normed, rotated, not rounded in between) and v
+    or into the rows ``q_out`` (which may be strided, and share no memory with ``qkv`` unless they are its q) with ``qkv`` left as it is; k (normed, rotated, not rounded in between) and v
     quantised into the places that ``slots`` names (page * page_size + offset, each at most once; outside the cache: not written).
     Returns q's rows."""
     shape = qkv.shape
@@ -338,6 +338,10 @@ def qk_norm_rope_cache_fp4(qkv: torch.Tensor, heads: int, kv_heads: int, head_di
         stride = q_out.stride(0) if tokens > 1 else q_out.shape[1]
         if q_out.stride(1) != 1 or stride < q_out.shape[1]:
             raise KernelError(f"qk_norm_rope_cache_fp4: q_out must be rows of contiguous features, it has strides {q_out.stride()}")
+        first, at = qkv.data_ptr(), q_out.data_ptr()
+        if (tokens and at < first + 2 * tokens * shape[1] and first < at + 2 * ((tokens - 1) * stride + q_out.shape[1])
+                and (at != first or (tokens > 1 and stride != shape[1]))):
+            raise KernelError("qk_norm_rope_cache_fp4: q_out lies in qkv's rows, and is not their q: lanes would read what others wrote")
         q = q_out
     _lib.fp4().call("mrun_qk_norm_rope_cache_fp4", qkv.data_ptr(), q.data_ptr(), stride, _address(q_weight), _address(k_weight), eps,
                     _address(rot), rotary_dim if rot is not None else 0, _address(slots), cache_at, tokens, heads, kv_heads, head_dim,

@@ -130,3 +130,25 @@ def test_keys_of_zeros_under_a_scale_that_leaves_the_range(monkeypatch, tiles):
     out = torch.empty(1, heads * dim, dtype=torch.bfloat16, device=DEV)
     attention(q.to(DEV), heads * dim, out, c.cache, group, ctx, heads, dim, 2.0 ** 10)
     close(out, v.mean(0).repeat(1, heads).view(1, -1), [v], 2.0 ** -10)
+
+
+def test_rows_for_q_that_lie_in_the_projection_are_refused():
+    """Other lanes still read the keys, the values or other rows there.  The projection's own q columns are written in place."""
+    from mrun_b200.kernels import KernelError
+    heads, kv_heads, dim, tokens = 2, 2, 64, 5
+    qkv, (qw, kw), rot = inputs(tokens, heads, kv_heads, dim, dim, seed=1)
+    memory = torch.zeros(3 * tokens, 3 * heads * dim, dtype=torch.bfloat16, device=DEV)
+    rows, wide = memory[tokens:2 * tokens], heads * dim
+    rows.copy_(qkv)
+    cache = torch.zeros(ops().fp4_cache_shape(1, kv_heads, 16, dim), dtype=torch.uint8, device=DEV)
+    slots = torch.arange(tokens, dtype=torch.int32, device=DEV)
+    call = lambda q_out: ops().qk_norm_rope_cache_fp4(rows, heads, kv_heads, dim, to(qw), to(kw), 1e-6, to(rot), dim, slots, cache, q_out=q_out)
+    flat = memory.view(-1)
+    for q_out in (rows[:, wide:2 * wide], rows[:, 2 * wide:], rows[:, 8:8 + wide], memory[tokens - 1:2 * tokens - 1, :wide],
+                  memory[2 * tokens - 1:3 * tokens - 1, :wide], flat[tokens * 3 * wide:tokens * 4 * wide].view(tokens, wide)):
+        with pytest.raises(KernelError, match="q_out lies in"):
+            call(q_out)
+    assert torch.equal(rows.cpu(), qkv) and not cache.any()
+    apart = [call(memory[:tokens, :wide]).clone(), call(memory[2 * tokens:, wide:2 * wide]).clone()]
+    assert torch.equal(rows.cpu(), qkv)
+    assert torch.equal(call(rows[:, :wide]), apart[0]) and torch.equal(*apart)
