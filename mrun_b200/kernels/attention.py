@@ -484,12 +484,15 @@ def prefill_uses_tcgen05(library, ratio: int, page_size: int) -> bool:
 
 
 # ------------------------------------------------------------------ the 4-bit cache
-# Which segments of a step with prompt portions take the kernel for single tokens, row by row: the shortest, as long as all their
-# rows times the kv heads are at most this many; the longer ones have their keys and values read back.  A row reads its whole context, but
-# all blocks share the step; the prompt kernels sweep a context with a block a tile and kv head.  The second figure is for segments that
-# fill at most a tile of 64 rows (rows x query heads a kv head), which the slower of the two prompt kernels would take.
-# B200, us by rows / read back, 32 heads over 8 of 128 behind 9,000 tokens: one segment of 16 tokens 44 / 452, of 32 69 / 97, of 64 124 / 97;
-# eight of 16 192 / 607, of 32 369 / 200.  16 heads over 16 behind 9,000: eight of 16 368 / 575, of 32 723 / 584.
+# Which segments of a step with prompt portions take the kernel for single tokens, row by row.  A row reads its whole context, but all blocks
+# share the step; the prompt kernels sweep a context with a block a tile and kv head, which takes the same time for one short segment as for
+# several.  So the segments of a kind go together: by rows where all their rows times the kv heads are at most this many, else read back (the step's
+# decoding tokens go by rows beside either and are not counted).  The kinds are segments of more than a tile of 64 rows (rows x query heads a kv
+# head) and, the second figure, those that fill at most one, which the slower of the two prompt kernels would take.
+# B200, us by rows / read back, 32 heads over 8 of 128 behind 9,000 tokens: one segment of 16 tokens 36 / 447, of 32 62 / 92, of 64 124 / 97;
+# two, three and eight of 32 111 / 101, 163 / 109, 418 / 149 (parted, one by rows and seven read back, 202); eight, 16 and 24 of 16 213 / 508,
+# 417 / 585, 632 / 728 (parted, 16 and eight, 936).  16 heads over 16 behind 9,000: two and eight of 32 212 / 466, 824 / 556 (parted 925).  One
+# of 30 behind 2,100 beside 8 / 64 / 256 decoding tokens there 25 / 50, 49 / 76, 131 / 150.
 FP4_ROWS, FP4_ROWS_OF_A_TILE = 256, 2048
 FP4_SCRATCH_ROWS = 128     # rows of a page that is read back: a key tile of the tcgen05 prompt kernel
 _fp4_slots = {}            # (device, head size, heads a block) -> blocks of the decode kernel that the device holds
@@ -595,10 +598,13 @@ def _fp4_portions(ctx, window: int, heads: int, kv_heads: int):
         return found
     ratio = heads // kv_heads
     rows, spans, longer, pages, width = [], [], [], 0, 0
+    prompts = [seg for seg in ctx.segments if seg.q_len > 1]
+    fits = {}                  # whether the segments of a tile, and the longer ones, go by rows
+    for of_a_tile, most in ((False, FP4_ROWS), (True, FP4_ROWS_OF_A_TILE)):
+        fits[of_a_tile] = kv_heads * sum(seg.q_len for seg in prompts if (ratio * seg.q_len <= 64) == of_a_tile) <= most
     for seg in sorted(ctx.segments, key=lambda seg: seg.q_len):
-        most = FP4_ROWS if ratio * seg.q_len > 64 else FP4_ROWS_OF_A_TILE
         # a decoding token is a row; the prompt kernels over tensor cores take up to 64 query heads a kv head
-        if seg.q_len == 1 or ratio > 64 or (len(rows) + seg.q_len) * kv_heads <= most:
+        if seg.q_len == 1 or ratio > 64 or fits[ratio * seg.q_len <= 64]:
             rows.extend(range(seg.q_start, seg.q_start + seg.q_len))
             continue
         end = seg.pos_start + seg.q_len

@@ -63,3 +63,44 @@ def test_a_call_that_failed_leaves_no_tables_that_nobody_wrote(monkeypatch):
     for (spans, _, table, span_of_row), (view, inner) in zip(calls.spans, calls.prompts):
         assert table is not None and span_of_row is not None and len(spans) == 2
         assert view.block_tables.data_ptr() == table.data_ptr() and inner.token_slot.data_ptr() == span_of_row.data_ptr()
+
+
+def portioned(segments, heads=32, kv_heads=8, window=0):
+    """(rows that go one by one, slots of the segments that are read back)."""
+    rows, longer = attention._fp4_portions(step_of(segments), window, heads, kv_heads)
+    return rows, [] if longer is None else sorted(span[0] for span in longer[0])
+
+
+def rows_of(segments, slots):
+    at, out = 0, []
+    for slot, n, _ in segments:
+        out += range(at, at + n) if slot in slots else []
+        at += n
+    return out
+
+
+@pytest.mark.parametrize("decoding", [8, 33, 64, 300])
+@pytest.mark.parametrize("n", [4, 16, 30, 32])
+def test_decoding_tokens_leave_short_portions_their_way(decoding, n):
+    """A few tokens behind a context go by rows whatever the number of decoding requests beside them."""
+    segments = [(i, 1, 2000 + i) for i in range(decoding)] + [(decoding, n, 2100)]
+    rows, back = portioned(segments)
+    assert not back and sorted(rows) == list(range(decoding + n))
+
+
+@pytest.mark.parametrize("heads, kv_heads, count, n, by_rows", [
+    (32, 8, 1, 32, True), (32, 8, 2, 32, False), (32, 8, 8, 32, False), (32, 8, 16, 16, True), (32, 8, 17, 16, False), (32, 8, 24, 16, False),
+    (16, 16, 4, 32, True), (16, 16, 5, 32, False), (16, 16, 8, 32, False), (128, 1, 3, 200, True)])
+def test_segments_of_a_kind_go_the_same_way(heads, kv_heads, count, n, by_rows):
+    segments = [(i, n, 9000) for i in range(count)]
+    rows, back = portioned(segments, heads, kv_heads)
+    assert (sorted(rows), back) == ((list(range(count * n)), []) if by_rows else ([], list(range(count))))
+
+
+def test_the_two_kinds_are_decided_apart():
+    segments = [(0, 16, 9000), (1, 1500, 0), (2, 1, 50), (3, 30, 2100), (4, 5, 0)]
+    rows, back = portioned(segments)
+    assert back == [1, 3] and sorted(rows) == rows_of(segments, (0, 2, 4))
+    segments = [(i, 16, 100) for i in range(17)] + [(17, 20, 100)]
+    rows, back = portioned(segments)
+    assert back == list(range(17)) and sorted(rows) == rows_of(segments, (17,))
