@@ -588,16 +588,20 @@ def _fp4_tokens(q, q_stride: int, out, cache, group, ctx, heads: int, head_dim: 
                      units * ops.FP4_TOKENS, pages, scale, window, _address(scratch), blocks, cluster, _queue())
 
 
-def _fp4_portions(ctx, window: int, heads: int, kv_heads: int):
+def _fp4_portions(ctx, window: int, heads: int, kv_heads: int, capacity: int = 1 << 62):
     """What a step's prompt portions need, made once per step: the rows that go one by one, and for the longer segments the spans of tokens
     to read back, their pages, and a step context and block tables over these, which every call's read back writes (a few words:
-    nothing then depends on whether an earlier call came to its end, and on which stream)."""
-    key = ("fp4_portions", window, heads, kv_heads)
+    nothing then depends on whether an earlier call came to its end, and on which stream).
+
+    ``capacity``: tokens of the cache.  A page that is read back has 128 rows; where that rounds the spans up to more tokens than the cache
+    holds, the part of a cache page that divides 128, so that what is read back is never more than the cache itself (the memory budget
+    counts on it).  1,531 tokens behind 9,000 take 269 us with pages of 16 rows, 265 with 128."""
+    key = ("fp4_portions", window, heads, kv_heads, capacity)
     found = ctx.shared.get(key)
     if found is not None:
         return found
     ratio = heads // kv_heads
-    rows, spans, longer, pages, width = [], [], [], 0, 0
+    rows, segments = [], []
     prompts = [seg for seg in ctx.segments if seg.q_len > 1]
     fits = {}                  # whether the segments of a tile, and the longer ones, go by rows
     for of_a_tile, most in ((False, FP4_ROWS), (True, FP4_ROWS_OF_A_TILE)):
@@ -607,19 +611,25 @@ def _fp4_portions(ctx, window: int, heads: int, kv_heads: int):
         if seg.q_len == 1 or ratio > 64 or fits[ratio * seg.q_len <= 64]:
             rows.extend(range(seg.q_start, seg.q_start + seg.q_len))
             continue
-        end = seg.pos_start + seg.q_len
-        first = _first_visible(seg.pos_start, window) // FP4_SCRATCH_ROWS * FP4_SCRATCH_ROWS
-        longer.append(SegmentView(len(spans), seg.q_start, seg.q_len, seg.pos_start))
-        spans.append((seg.slot, first, end, pages, seg.q_start, seg.q_len))
-        pages += -(-(end - first) // FP4_SCRATCH_ROWS)
-        width = max(width, -(-end // FP4_SCRATCH_ROWS))
-    if not spans:
+        segments.append(seg)
+    if not segments:
         found = ctx.shared[key] = (rows, None)
         return found
+    for page in (FP4_SCRATCH_ROWS, math.gcd(ctx.page_size, FP4_SCRATCH_ROWS)):
+        spans, longer, pages, width = [], [], 0, 0
+        for seg in segments:
+            end = seg.pos_start + seg.q_len
+            first = _first_visible(seg.pos_start, window) // page * page
+            longer.append(SegmentView(len(spans), seg.q_start, seg.q_len, seg.pos_start))
+            spans.append((seg.slot, first, end, pages, seg.q_start, seg.q_len))
+            pages += -(-(end - first) // page)
+            width = max(width, -(-end // page))
+        if pages * page <= capacity:
+            break
     own = torch.empty(ctx.num_tokens + len(spans) * width, dtype=torch.int32, device=ctx.positions.device)
     span_of_row, table = own[:ctx.num_tokens], own[ctx.num_tokens:].view(len(spans), width)
     inner = dataclasses.replace(ctx, segments=longer, num_segments=len(longer), token_slot=span_of_row, shared={},
-                                max_q_len=max(seg.q_len for seg in longer), page_size=FP4_SCRATCH_ROWS, real_tokens=ctx.num_tokens)
+                                max_q_len=max(seg.q_len for seg in longer), page_size=page, real_tokens=ctx.num_tokens)
     found = ctx.shared[key] = (rows, (spans, pages, table, span_of_row, inner, _View(table, width)))
     return found
 
@@ -636,8 +646,8 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
     of 64 or 128 features, pages of a multiple of 16 tokens, any number of query heads a kv head.
 
     Single tokens, and a few tokens more, read the 4-bit pages as they are (every step of single tokens may be captured in a
-    graph).  The keys and values of longer segments are read back in bfloat16, 128 tokens a page, for the time of
-    the call (4 * head_dim bytes a token and kv head of the segments' contexts), and go to the prompt kernels.  A page outside the cache,
+    graph).  The keys and values of longer segments are read back in bfloat16 for the time of the call (4 * head_dim bytes a token and kv
+    head of the segments' contexts, rounded up to 128 tokens where the cache has room for as many), and go to the prompt kernels.  A page outside the cache,
     and a position behind the block table, is not seen; a row that sees nothing is zeros.  Unless the step says that its pages are held
     (``ctx.pages_held``) the longer segments' pages are looked through for such ones.  A value that is NaN makes NaN of the rows that see
     it, and may of other rows of the same prompt portion."""
@@ -665,12 +675,12 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
         return out
     if tokens > ctx.real_tokens:
         out[ctx.real_tokens:].zero_()
-    rows, longer = _fp4_portions(ctx, window, heads, kv_heads)
+    rows, longer = _fp4_portions(ctx, window, heads, kv_heads, pages * page_size)
     if rows:
         _fp4_tokens(q, q_stride, out, cache, group, ctx, heads, head_dim, scale, window, rows)
     if longer is not None:
         spans, n, table, span_of_row, inner, view = longer
-        k, v = ops.fp4_spans(cache, head_dim, group.block_tables, spans, n, FP4_SCRATCH_ROWS, table, span_of_row)
+        k, v = ops.fp4_spans(cache, head_dim, group.block_tables, spans, n, inner.page_size, table, span_of_row)
         paged_attention(q, q_stride, out, _Pages(k, v), view, inner, heads, scale, window)
         if not ctx.pages_held:
             # what is read back has zeros in the places of keys that are not there: rows that see such ones are computed again

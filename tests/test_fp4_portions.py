@@ -104,3 +104,29 @@ def test_the_two_kinds_are_decided_apart():
     segments = [(i, 16, 100) for i in range(17)] + [(17, 20, 100)]
     rows, back = portioned(segments)
     assert back == list(range(17)) and sorted(rows) == rows_of(segments, (17,))
+
+
+@pytest.mark.parametrize("page, lengths, window", [
+    (16, [33] * 64, 0), (16, [150, 17, 300, 1000], 0), (48, [50] * 9, 0), (64, [65, 70, 200], 0), (256, [300, 257, 900], 0), (32, [700, 650, 800], 100),
+    (16, [700] * 5, -256), (16, [2000], 0)])
+def test_what_is_read_back_is_no_more_than_the_cache(monkeypatch, page, lengths, window):
+    """A memory budget sets aside the read back of as many tokens as the cache holds: also where the cache is full of short requests, each of
+    which would be rounded up to 128 tokens."""
+    calls = Calls(monkeypatch)
+    held = [(0 if window == 0 else attention._first_visible(n - n // 2, window) // page, -(-n // page)) for n in lengths]
+    pool = sum(end - first for first, end in held)
+    for pages in (pool, 20 * pool + 40):
+        ctx = step_of([(i, n // 2, n - n // 2) for i, n in enumerate(lengths)], page)
+        monkeypatch.setattr(attention, "FP4_ROWS", 0)
+        monkeypatch.setattr(attention, "FP4_ROWS_OF_A_TILE", 0)
+        attend(ctx, page=page, pages=pages, window=window)
+        spans, taken, table, _ = calls.spans[-1]
+        inner = calls.prompts[-1][1]
+        assert taken * inner.page_size <= pages * page and 128 % inner.page_size == 0 and inner.page_size >= 16
+        at = 0
+        for (slot, first, end, page0, _, _), n in zip(sorted(spans, key=lambda span: span[3]), sorted(lengths)):
+            assert page0 == at and end == n and first % inner.page_size == 0 and first <= attention._first_visible(n - n // 2, window)
+            at += -(-(end - first) // inner.page_size)
+            assert -(-end // inner.page_size) <= table.shape[1]
+        assert at == taken
+    assert inner.page_size == 128

@@ -100,3 +100,31 @@ def test_spans_that_leave_pages_or_name_no_row_are_refused():
     got = torch.cat([k[0], k[3]], 1).double().cpu().transpose(0, 1)
     assert torch.equal(got[:100], c.k[0]) and not got[100:].any() and not k[1:3].any() and not v[1:3].any()
     assert [x.shape[0] for x in ops.fp4_spans(c.cache, 64, table, [], 0, 64)] == [0, 0]
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, page, lengths, window", [
+    (8, 2, 128, 16, [150, 170, 300, 33], 0), (12, 3, 64, 48, [130, 300, 97], 0), (8, 2, 128, 64, [129, 200], 0), (8, 2, 64, 256, [300, 290], 0),
+    (8, 2, 128, 32, [400, 390], 100), (4, 2, 64, 16, [400, 390], -128)])
+def test_a_cache_that_is_full(heads, kv_heads, dim, page, lengths, window):
+    """No page is free: what is read back takes the cache's own pages in place of ones of 128 rows.  The bits are those of a cache with room."""
+    from mrun_b200.kernels import attention as module
+    c = Filled(lengths, kv_heads, dim, page, seed=7, spare=40)
+    segments = [(i, n - n // 4, n // 4) for i, n in enumerate(lengths)]
+    table = c.table.clone()
+    for i, (_, _, first) in enumerate(segments):               # what a window has passed is given back
+        table[i, :plain_fp4.first_visible(first, window) // page] = -1
+    kept = table[table >= 0].long()
+    new = torch.full((c.cache.shape[0],), -1, dtype=torch.int32)
+    new[kept] = torch.arange(kept.numel(), dtype=torch.int32)
+    full_table = torch.where(table >= 0, new[table.clamp(min=0).long()], table)
+    q = c.queries(sum(n for _, n, _ in segments), heads, dim)
+    outs, sizes = [], []
+    for cache, block_table in ((c.cache, table), (c.cache[kept.to(DEV)].contiguous(), full_table)):
+        ctx, group = step_of(segments, block_table.to(DEV), page)
+        outs.append(torch.empty(q.shape, dtype=torch.bfloat16, device=DEV))
+        attention(q.to(DEV), heads * dim, outs[-1], cache, group, ctx, heads, dim, dim ** -0.5, window)
+        close(outs[-1], wanted(c, q, segments, heads, dim, window), c.v, 2.0 ** -7)
+        longer = module._fp4_portions(ctx, window, heads, kv_heads, cache.shape[0] * page)[1]
+        sizes.append(longer[4].page_size)
+        assert longer[1] * sizes[-1] <= cache.shape[0] * page
+    assert sizes[0] == 128 and torch.equal(*outs)
