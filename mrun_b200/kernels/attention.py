@@ -21,8 +21,8 @@ the fused norm/rotary/cache kernel just before.
 """
 from __future__ import annotations
 
+import copy
 import ctypes
-import dataclasses
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -602,13 +602,14 @@ def _fp4_portions(ctx, window: int, heads: int, kv_heads: int, capacity: int = 1
         return found
     ratio = heads // kv_heads
     rows, segments = [], []
-    prompts = [seg for seg in ctx.segments if seg.q_len > 1]
-    fits = {}                  # whether the segments of a tile, and the longer ones, go by rows
-    for of_a_tile, most in ((False, FP4_ROWS), (True, FP4_ROWS_OF_A_TILE)):
-        fits[of_a_tile] = kv_heads * sum(seg.q_len for seg in prompts if (ratio * seg.q_len <= 64) == of_a_tile) <= most
+    tokens = [0, 0]            # of the segments of more than a tile, and of those that fill at most one
+    for seg in ctx.segments:
+        if seg.q_len > 1:
+            tokens[ratio * seg.q_len <= 64] += seg.q_len
+    by_rows = (kv_heads * tokens[0] <= FP4_ROWS, kv_heads * tokens[1] <= FP4_ROWS_OF_A_TILE)
     for seg in sorted(ctx.segments, key=lambda seg: seg.q_len):
         # a decoding token is a row; the prompt kernels over tensor cores take up to 64 query heads a kv head
-        if seg.q_len == 1 or ratio > 64 or fits[ratio * seg.q_len <= 64]:
+        if seg.q_len == 1 or ratio > 64 or by_rows[ratio * seg.q_len <= 64]:
             rows.extend(range(seg.q_start, seg.q_start + seg.q_len))
             continue
         segments.append(seg)
@@ -628,8 +629,9 @@ def _fp4_portions(ctx, window: int, heads: int, kv_heads: int, capacity: int = 1
             break
     own = torch.empty(ctx.num_tokens + len(spans) * width, dtype=torch.int32, device=ctx.positions.device)
     span_of_row, table = own[:ctx.num_tokens], own[ctx.num_tokens:].view(len(spans), width)
-    inner = dataclasses.replace(ctx, segments=longer, num_segments=len(longer), token_slot=span_of_row, shared={},
-                                max_q_len=max(seg.q_len for seg in longer), page_size=page, real_tokens=ctx.num_tokens)
+    inner = copy.copy(ctx)
+    inner.segments, inner.num_segments, inner.token_slot, inner.shared = longer, len(longer), span_of_row, {}
+    inner.max_q_len, inner.page_size, inner.real_tokens = max(seg.q_len for seg in longer), page, ctx.num_tokens
     found = ctx.shared[key] = (rows, (spans, pages, table, span_of_row, inner, _View(table, width)))
     return found
 
@@ -684,8 +686,10 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
         paged_attention(q, q_stride, out, _Pages(k, v), view, inner, heads, scale, window)
         if not ctx.pages_held:
             # what is read back has zeros in the places of keys that are not there: rows that see such ones are computed again
-            flat = (ctypes.c_int * (4 * len(spans)))(*[v for (slot, *_), seg in zip(spans, inner.segments)
-                                                      for v in (slot, seg.pos_start, seg.q_start, seg.q_len)])
+            flat = []
+            for span, seg in zip(spans, inner.segments):
+                flat += span[0], seg.pos_start, seg.q_start, seg.q_len
+            flat = (ctypes.c_int * len(flat))(*flat)
             tables = group.block_tables
             _lib.fp4().call("mrun_attn_fp4_unheld", q.data_ptr(), q_stride, out.data_ptr(), cache.data_ptr(), tables.data_ptr(), tables.shape[0],
                             tables.shape[1], ctypes.addressof(flat), len(spans), heads, kv_heads, head_dim, page_size, pages, scale, window, _queue())
