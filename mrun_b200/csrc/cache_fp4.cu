@@ -23,10 +23,10 @@ using bf16 = __nv_bfloat16;
 //
 // D / 8 lanes take a run of heads of a token, eight features a lane, with the token's cosines and sines loaded once and the features of
 // the next three heads on their way into shared memory, where a lane reads what it copied itself.  What bounds it is the chain of a head
-// (sum over the lanes, root, rotation across lanes) and its instructions, with 28 warps a multiprocessor to hide it: 14.4 us for 2,048 tokens of 32 + 8 + 8 heads
+// (sum over the lanes, root, rotation across lanes) and its instructions, with 28 warps a multiprocessor to hide it: 14.3 us for 2,048 tokens of 32 + 8 + 8 heads
 // of 128 in runs of 6, of which the queries alone take 9.4 (the bytes take 6.8, the write of bfloat16 pages 13.7); a copy to every two heads, in
 // registers, took 21.7.  Longer runs save instructions and leave fewer lanes at work, hence as long as the step has
-// heads for them (us in runs of 2 / 4 / 6 / 12: 512 tokens 8.3 / 8.1 / 8.5 / 9.9; 2,048 18.8 / 14.9 / 14.2 / 14.8; 8,192 72.5 / 55.5 / 50.5 / 47.1).
+// heads for them (us in runs of 2 / 4 / 6 / 12: 512 tokens 8.3 / 8.1 / 8.5 / 9.9; 2,048 18.8 / 14.9 / 14.3 / 14.8; 8,192 72.5 / 55.5 / 50.5 / 47.1).
 // ------------------------------------------------------------------------------------------
 constexpr int STORE_THREADS = 256;
 constexpr int RUN_THREADS = 128, RUN_DEPTH = 4;
@@ -358,7 +358,8 @@ __device__ __forceinline__ void store_held(const uint4& raw, bool is_k, int head
     if ((part & 1) == 0) unit[is_k ? Unit::k_scale(r, part / 2) : Unit::v_scale(r, part / 2)] = (unsigned char)scale;
 }
 
-// A head to every D / 8 lanes.  STAGED: rotary sizes that are no multiple of 16, and weights or tables off 16 bytes; keys in 64 bits throughout.
+// A head to every D / 8 lanes.  STAGED: rotary sizes that are no multiple of 16, and weights or tables off 16 bytes; keys in 64 bits throughout (2,048
+// tokens of 32 + 8 + 8 heads of 128 under a rotary size of 20 / 126: 32.7 / 46.5 us; 64 tokens 4.5 / 4.7, 3.6 by the other).
 template <int D, bool STAGED>
 __global__ void __launch_bounds__(STORE_THREADS, STAGED ? 1 : 4)
 qk_norm_rope_cache_fp4_kernel(const bf16* qkv, bf16* q_out /* may be qkv */, long q_stride,

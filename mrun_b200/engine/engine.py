@@ -92,7 +92,8 @@ class Engine:
         """``num_pages`` or ``context`` size the cache directly.  With ``memory`` (a budget from
         :func:`mrun_b200.engine.budget.plan`) the cache is what the budget leaves beside the
         weights and the step's scratch, or exactly ``context`` tokens if that fits.  ``kv_cache="fp4"`` holds keys and
-        values in 4 bits (bfloat16, models of grouped-query attention with heads of 64 or 128 features, ``page_size`` a multiple of 16)."""
+        values in 4 bits (bfloat16, models of grouped-query attention with heads of 64 or 128 features, ``page_size`` a multiple of 16); a budget
+        then also sets aside what reading a layer's keys and values back for a prompt takes."""
         sizing = None
         if memory is not None and num_pages is None:
             sizing = _sizing(memory, context, page_size, max_requests, max_batch_tokens)
