@@ -59,9 +59,9 @@ class StepContext:
     max_kv_len: int
     page_size: int
     real_tokens: int = 0         # rows that are not padding
-    pages_held: bool = False     # every page that a row sees is known to be held (the cache manager's books say so)
     upload: Optional[object] = None              # host int32 array -> device tensor (pinned staging)
     shared: dict = field(default_factory=dict)   # per-step results shared between layers
+    pages_held: bool = False     # every page that a row sees is known to be held (the cache manager's books say so)
 
     def group(self, key: tuple) -> GroupView:
         return self.groups[key]

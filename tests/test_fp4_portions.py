@@ -130,3 +130,10 @@ def test_what_is_read_back_is_no_more_than_the_cache(monkeypatch, page, lengths,
             assert -(-end // inner.page_size) <= table.shape[1]
         assert at == taken
     assert inner.page_size == 128
+
+
+def test_a_step_is_described_as_before():
+    """Callers that give a step's fields in their order still do; a step that says nothing of its pages has them looked through."""
+    from dataclasses import fields
+    assert [f.name for f in fields(StepContext)][-4:] == ["real_tokens", "upload", "shared", "pages_held"]
+    assert next(f.default for f in fields(StepContext) if f.name == "pages_held") is False
