@@ -656,6 +656,8 @@ def paged_attention_fp4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cache
     pages, kv_heads, page_size = ops.check_fp4_cache(cache, head_dim)
     if heads < 1 or heads % kv_heads:
         raise ops.KernelError(f"paged_attention_fp4: heads={heads} is not a multiple of kv_heads={kv_heads}")
+    if not 0.0 < scale < math.inf:
+        raise ops.KernelError(f"paged_attention_fp4: scale={scale} is not a positive number")
     tokens = ctx.num_tokens
     if out.shape != (tokens, heads * head_dim):
         raise ops.KernelError(f"paged_attention_fp4: out is {tuple(out.shape)}, expected {(tokens, heads * head_dim)}")

@@ -137,3 +137,15 @@ def test_a_step_is_described_as_before():
     from dataclasses import fields
     assert [f.name for f in fields(StepContext)][-4:] == ["real_tokens", "upload", "shared", "pages_held"]
     assert next(f.default for f in fields(StepContext) if f.name == "pages_held") is False
+
+
+@pytest.mark.parametrize("segments", [[(0, 1, 5)], [(0, 300, 0)], [(0, 300, 0), (1, 1, 9)]])
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf")])
+def test_a_scale_that_is_not_positive_is_refused_before_anything_runs(monkeypatch, segments, scale):
+    calls = Calls(monkeypatch)
+    q = torch.zeros(sum(n for _, n, _ in segments), 512, dtype=torch.bfloat16)
+    cache = torch.zeros(ops.fp4_cache_shape(4, 2, 16, 64), dtype=torch.uint8)
+    with pytest.raises(ops.KernelError, match="scale"):
+        attention.paged_attention_fp4(q, 512, torch.empty_like(q), cache, types.SimpleNamespace(block_tables=torch.zeros(8, 64, dtype=torch.int32)),
+                                      step_of(segments), 8, 64, scale)
+    assert not calls.rows and not calls.spans and not calls.prompts
