@@ -93,14 +93,14 @@ def test_scores_near_the_end_of_32_bits(monkeypatch, tiles, heads, n):
     c = Filled([n], 1, dim, 16, seed=1)
     g = torch.Generator().manual_seed(n)
     size = torch.tensor([61440.0, 43008.0])[torch.randint(0, 2, (n,), generator=g)]
-    size[n // 2] = 30720.0
+    size[n // 2] = 6 * 5120.0
     k, v = rows_of(size.tolist(), dim), torch.randn(n, 1, dim, generator=g).double()
     fill(c, k, v)
     k, v = plain_fp4.held(k)[0], plain_fp4.held(v)[0]
     assert torch.equal(k[:, 0, 0].float(), size)
     for sign in (-1.0, 1.0):
         q = torch.full((1, heads * dim), sign * 2.0 ** 105).bfloat16()
-        size[n // 2] = 30720.0 if sign < 0 else 61440.0
+        size[n // 2] = 6 * 5120.0 if sign < 0 else 61440.0
         score = q[0, 0].double() * dim * k[:, 0, 0] * 1.4426950408889634
         assert score.abs().min() > 1e38 and score.abs().max() < 3e38
         if sign > 0 and n > 1:          # one key above the others
